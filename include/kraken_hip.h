@@ -717,6 +717,138 @@ KRAKEN_API int kraken_hip_argmax_prob_f32_i32(kraken_hip_context* context, krake
                                               size_t size, kraken_buffer token_output,
                                               kraken_buffer probability_output);
 
+/* ---- Batched serving over a paged 8-bit KV cache ---------------------------
+ * No counterpart in the reference, which keeps one contiguous F16 cache per
+ * context (mps_backend.hpp:415-420; qwen35_runtime.cpp:35-45) and picks tokens
+ * greedily (mps_backend.hpp:384-390).  For servers that batch many sequences:
+ * the keys and values lie in pages of page_tokens tokens, 8 bits a value with
+ * one f32 scale for each page and KV head, half an F16 cache's bytes.
+ *
+ * A value is its code times its page's scale.  Codes are int8 in [-127, 127]:
+ *   key_pages    [pages][kv_heads][page_tokens][head_dim]
+ *   value_pages  [pages][kv_heads][page_tokens / 8][head_dim][8]: the eight
+ *                tokens of a run lie side by side for each dimension
+ *   key_scales, value_scales  f32 [pages][kv_heads], not negative
+ * page_tokens is 16, 32, 64 or 128; head_dim 64, 128 or 256; the page pools are
+ * 16-byte aligned.  Nothing needs initialising: a page's scale and codes are
+ * written when its first token is.
+ *
+ * A batch brings new tokens of `sequences` sequences in one list of `tokens`
+ * rows: sequence b's are rows query_starts[b] .. query_starts[b + 1] - 1 (it may
+ * bring none), and with them it is lengths[b] tokens long, so its row i stands at
+ * position lengths[b] - count + i.  page_table[b][p] is the page that holds
+ * positions p * page_tokens on; entries past the length are not read.
+ * max_query and max_keys bound every sequence's new tokens and length; they size
+ * the launches and need not be tight.  The arrays are device memory, read when
+ * the kernels run, so a captured graph replays with new ones in their place.
+ * A sequence that breaks a bound (query_starts that decrease or pass `tokens`,
+ * more new tokens than max_query or its length, a length above max_keys or
+ * table_width * page_tokens) is left out: nothing of it is read or written.
+ * Rows of no sequence stay as they were.  A page id outside [0, pages) is a
+ * page without tokens: its keys are not attended and nothing is appended to it.
+ * A page that a call appends to must stand once in the batch's tables; pages that
+ * are only read may be shared. */
+typedef struct kraken_paged_q8_cache {
+  kraken_buffer key_pages;
+  kraken_buffer value_pages;
+  kraken_buffer key_scales;
+  kraken_buffer value_scales;
+  size_t pages;
+  size_t page_tokens;
+  size_t kv_heads;
+  size_t head_dim;
+} kraken_paged_q8_cache;
+
+typedef struct kraken_paged_batch {
+  kraken_buffer page_table;   /* int32 [sequences][table_width] */
+  kraken_buffer query_starts; /* uint32 [sequences + 1] */
+  kraken_buffer lengths;      /* uint32 [sequences] */
+  size_t sequences;
+  size_t table_width;
+  size_t tokens;
+  size_t max_query;
+  size_t max_keys;
+} kraken_paged_batch;
+
+/* kraken_hip_qwen35_attention_prologue_f16_kv for a batch, with the new keys and
+ * values quantised into their pages: q_gate f32 [tokens][heads][2 * head_dim] is
+ * split, its queries and the keys [tokens][kv_heads][head_dim] normalised
+ * (q_norm, k_norm, eps) and rotated (n_dims, sections, theta); query_out and
+ * gate_out f32 [tokens][heads][head_dim].  positions is int32 [4][tokens];
+ * with positions.data == NULL every row holds the token's position in its
+ * sequence.  Norm and rotation are those of the F16 entry to f32 rounding (the
+ * angle in 64 bits).  For each page, KV head and of keys and values apart, with
+ * A the largest magnitude of the new rows that it takes: a page whose first
+ * token is among them, or whose scale is zero, gets the scale A / 127; any other
+ * keeps its scale s, doubled as often as A <= 127 s needs, its older codes
+ * divided by the same power of two and rounded to even, so that the older values
+ * lose at most one step of the final scale however often it grows.  The new
+ * codes are the rows over the scale, rounded to even.  Codes behind a page's
+ * last token stay as they were.  A new row with a NaN or an infinity makes its
+ * page's scale NaN for that head (its values then read as NaN) until the page is
+ * begun again; rows whose largest magnitude is below 127 times the smallest
+ * normal f32 are held as zeros.  One launch, no workspace. */
+KRAKEN_API int kraken_hip_qwen35_attention_prologue_paged_q8_kv(
+  kraken_hip_context* context, kraken_buffer q_gate, kraken_buffer key, kraken_buffer value,
+  kraken_buffer q_norm, kraken_buffer k_norm, kraken_buffer positions,
+  const kraken_paged_q8_cache* cache, const kraken_paged_batch* batch, size_t heads,
+  size_t n_dims, size_t section_0, size_t section_1, size_t section_2, size_t section_3,
+  float theta, float eps, kraken_buffer query_out, kraken_buffer gate_out);
+
+/* Causal attention of the batch's rows over their sequences' pages: query, output
+ * and gate f32 [tokens][heads][head_dim]; the row at position p attends keys
+ * 0..p, its own among them (appended before this call), with scale
+ * 1 / sqrt(head_dim).  gate.data == NULL: none; else out *= sigmoid(gate).
+ * heads is a multiple of kv_heads.  Products keep f32 accuracy: the codes are
+ * exact in the matrix cores' f16 and the f32 operands go in as two f16 parts.  A
+ * row without any key to attend (all its pages outside the pool) gets zeros.
+ * query, gate and output are 16-byte aligned; output overlaps neither.  Uses
+ * context workspace where the keys are split over workgroups. */
+KRAKEN_API int kraken_hip_attention_f32_paged_q8_kv(
+  kraken_hip_context* context, kraken_buffer query, kraken_buffer gate,
+  const kraken_paged_q8_cache* cache, const kraken_paged_batch* batch, size_t heads,
+  kraken_buffer output);
+
+/* The same with query and output in f16, without a gate: the softmax weights are
+ * rounded to f16 for their product, sums stay f32. */
+KRAKEN_API int kraken_hip_attention_f16q_paged_q8_kv(
+  kraken_hip_context* context, kraken_buffer query, const kraken_paged_q8_cache* cache,
+  const kraken_paged_batch* batch, size_t heads, kraken_buffer output);
+
+/* Pages read back as rows of an F16 cache: key_rows and value_rows f16
+ * [count][page_tokens][kv_heads][head_dim] receive the values of page
+ * page_ids[i] (int32); an id outside [0, pages) gives zero rows, as an id
+ * outside the matrix does in dequantize_rows_*.  Codes behind a page's last
+ * token come back as they lie there. */
+KRAKEN_API int kraken_hip_dequantize_kv_pages_q8_f16(
+  kraken_hip_context* context, const kraken_paged_q8_cache* cache, kraken_buffer page_ids,
+  size_t count, kraken_buffer key_rows, kraken_buffer value_rows);
+
+/* One token for each of `rows` rows of logits f32 [rows][row_stride], the first
+ * `size` of a row, by given random numbers: uniforms f32 [rows] in [0, 1).
+ * temperature f32, top_k int32, top_p f32 and min_p f32 are [rows] each; an
+ * empty buffer stands for 1, 0, 1 and 0.  With the tokens of a row in order of
+ * falling logit (equal ones: the lower index first) and w = exp((logit - largest)
+ * / temperature), those kept are the tokens that are among the first top_k
+ * (top_k <= 0: all), and before which less than top_p times the sum of w over
+ * those lies (top_p >= 1: all), and whose w is at least min_p; the first always
+ * is.  The token drawn is the first in order of index at which the running sum
+ * of the kept w passes uniform times their whole sum; token_output int32 [rows]
+ * receives it and probability_output f32 [rows] (may be empty) its share of that
+ * sum.  A temperature that is not above zero draws greedily: the first of the
+ * largest logits, probability 1.  NaN logits are never drawn and -inf only where
+ * nothing is larger (probability 0); all-NaN gives `size` and 0, as
+ * argmax_f32_i32 does; equal +inf logits share the whole weight.  A NaN
+ * temperature draws greedily, NaN top_p and min_p keep all, a uniform outside
+ * [0, 1) or NaN is taken as the nearest end (NaN as 0).  Weights are formed in 64
+ * bits and summed as integers (2^-44 of the largest up to 262144 tokens), so a
+ * result does not depend on the order of the sums.  Uses context workspace. */
+KRAKEN_API int kraken_hip_sample_f32_i32(
+  kraken_hip_context* context, kraken_buffer logits, size_t rows, size_t size,
+  size_t row_stride, kraken_buffer temperature, kraken_buffer top_k, kraken_buffer top_p,
+  kraken_buffer min_p, kraken_buffer uniforms, kraken_buffer token_output,
+  kraken_buffer probability_output);
+
 #ifdef __cplusplus
 }
 #endif

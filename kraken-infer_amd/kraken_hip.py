@@ -39,8 +39,26 @@ class KrakenError(RuntimeError):
         self.message = message
 
 
+class PagedQ8Cache(ctypes.Structure):
+    """kraken_paged_q8_cache: KV pages of 8-bit codes with their scales."""
+    _fields_ = [("key_pages", KrakenBuffer), ("value_pages", KrakenBuffer),
+                ("key_scales", KrakenBuffer), ("value_scales", KrakenBuffer),
+                ("pages", ctypes.c_size_t), ("page_tokens", ctypes.c_size_t),
+                ("kv_heads", ctypes.c_size_t), ("head_dim", ctypes.c_size_t)]
+
+
+class PagedBatch(ctypes.Structure):
+    """kraken_paged_batch: the new tokens of many sequences and their pages."""
+    _fields_ = [("page_table", KrakenBuffer), ("query_starts", KrakenBuffer),
+                ("lengths", KrakenBuffer), ("sequences", ctypes.c_size_t),
+                ("table_width", ctypes.c_size_t), ("tokens", ctypes.c_size_t),
+                ("max_query", ctypes.c_size_t), ("max_keys", ctypes.c_size_t)]
+
+
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
+_pages = ctypes.POINTER(PagedQ8Cache)
+_batch = ctypes.POINTER(PagedBatch)
 _B = KrakenBuffer
 _ctx = ctypes.c_void_p
 
@@ -122,6 +140,12 @@ SIGNATURES = {
                                                _B, _B],
     "kraken_hip_argmax_f32_i32": [_B, _sz, _B],
     "kraken_hip_argmax_prob_f32_i32": [_B, _sz, _B, _B],
+    "kraken_hip_qwen35_attention_prologue_paged_q8_kv": [_B] * 6 + [_pages, _batch] + [_sz] * 6
+                                                        + [_f, _f, _B, _B],
+    "kraken_hip_attention_f32_paged_q8_kv": [_B, _B, _pages, _batch, _sz, _B],
+    "kraken_hip_attention_f16q_paged_q8_kv": [_B, _pages, _batch, _sz, _B],
+    "kraken_hip_dequantize_kv_pages_q8_f16": [_pages, _B, _sz, _B, _B],
+    "kraken_hip_sample_f32_i32": [_B, _sz, _sz, _sz] + [_B] * 7,
     "kraken_hip_begin_graph": [],
     "kraken_hip_commit_graph": [],
     "kraken_hip_make_buffer": [_sz, ctypes.POINTER(_B)],
