@@ -1,100 +1,512 @@
-// Causal attention of a ragged batch over 8-bit KV pages.
+// Causal attention of a ragged batch over 8-bit KV pages: the sequences that bring few
+// rows (the single tokens of a decode step, drafted tokens to verify), and the join of
+// split results.  The arithmetic is described in attention_paged_q8_common.hpp.
+//
+// A workgroup takes one KV head of one sequence and a run of its keys; its four waves
+// take 32-key steps in turn, each with its own running maximum, sum and output, and
+// join them at the end.  Nothing passes through LDS before that: K and V go from the
+// pages to registers in the operand layout of the matrix cores.
+//  - S^T = K Q^T (16x16x32): a lane loads 16 bytes of its key row at a time, which
+//    are two operands; the order of the dimensions within a product is free, and Q is
+//    laid out the same way.  The key rows of a 32-key step are dealt to the two row
+//    tiles so that a lane's eight scores are those of one run of eight keys.
+//  - O^T += V^T P^T: that run is what a lane's operand of P must hold, so P needs no
+//    exchange between lanes, and since the pages keep the eight tokens of a run side
+//    by side, the operand of V is eight bytes as they lie.
+//  - The f32 operands need two f16 parts.  Up to 8 rows fill only half of the 16
+//    columns, so the high parts take columns 0..7 and the low parts 8..15 of the same
+//    product (kStacked) and the halves are added; up to 16 rows take two products.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
+#include "attention_paged_q8_common.hpp"
 #include "context_internal.hpp"
 #include "device_common.hpp"
-#include "paged_q8_internal.hpp"
 
 namespace kraken {
 namespace {
 
-// The plain form: a wave per row and head, one key at a time, softmax with a running
-// maximum and sum.
-template <class T, int kRegs>
-__global__ __launch_bounds__(64) void attention_paged_q8_plain(PagedAttentionArgs a) {
-  const int lane = threadIdx.x;
-  const uint32_t head = blockIdx.x % a.heads, row = blockIdx.x / a.heads;
-  const uint32_t d_head = a.cache.head_dim, shift = a.cache.page_shift;
+constexpr uint32_t kWaves = 4;
+
+template <int D, class T, bool kStacked>
+__global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAttentionArgs a,
+                                                                        PagedSplit split) {
+  constexpr uint32_t kRows = kStacked ? 8 : 16;
+  constexpr bool kTwo = !kStacked && std::is_same<T, float>::value;
+  constexpr int kLoads = D / 64;  // 16-byte loads of a key row per lane and row tile
+  constexpr int kStride = D + 4;  // of an output row in LDS, in floats
+  __shared__ float lds_o[kWaves * kRows * kStride];
+  __shared__ float lds_m[kWaves][kRows], lds_l[kWaves][kRows];
+
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t n = lane & 15u, g = lane >> 4;
+  const uint32_t kv_head = blockIdx.y, sequence = blockIdx.z;
+  const uint32_t shift = a.cache.page_shift, kv_heads = a.cache.kv_heads;
+  const uint32_t group = a.heads / kv_heads;
+  const PagedSequence s = paged_sequence(a.batch, sequence, shift);
+  const uint32_t rows = s.count * group;
+  const uint32_t begin = blockIdx.x * split.decode_keys;
+  if (s.count == 0 || rows > kRows || begin >= s.length) {
+    return;
+  }
+  const uint32_t end = min(s.length, begin + split.decode_keys);
+  const uint32_t steps = (end - begin + 31u) / 32u;
+  const int32_t* table = a.batch.table + (size_t)sequence * a.batch.width;
+  const uint32_t last_page = (s.length - 1u) >> shift;
+
+  // This lane's query row and the keys that it sees.
+  const uint32_t row = kStacked ? n & 7u : n;
+  const bool real = row < rows;
+  const uint32_t token = real ? row / group : 0u;
+  const uint32_t visible = s.length - s.count + token + 1u;
+  const size_t at = ((size_t)(s.start + token) * a.heads + kv_head * group +
+                     (real ? row % group : 0u)) * D;
+
+  // Page ids of the lane's key rows (run n / 4 of the step's four) and of its own run g.
+  auto page_of = [&](uint32_t key) {
+    return table[min(key >> shift, last_page)];
+  };
+  auto first_key = [&](uint32_t step) { return begin + step * 32u; };
+  u32x4_t k[2][kLoads], v[2 * kLoads];
+  float key_scale, val_scale;
+  bool inside;
+  auto load_k = [&](uint32_t step, int32_t page) {
+    const uint32_t key = first_key(step) + 8u * (n >> 2) + (n & 3u);
+    const uint32_t held = page >= 0 && (uint32_t)page < a.cache.pages ? (uint32_t)page : 0u;
+    const int8_t* p = a.cache.keys +
+                      ((((size_t)held * kv_heads + kv_head) << shift) +
+                       (key & ((1u << shift) - 1u))) * D + 16u * g;
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+      k[0][c] = *reinterpret_cast<const u32x4_t*>(p + 64 * c);
+      k[1][c] = *reinterpret_cast<const u32x4_t*>(p + 4 * D + 64 * c);
+    }
+  };
+  auto load_v = [&](uint32_t step, int32_t page) {
+    const uint32_t key = first_key(step) + 8u * g;
+    inside = page >= 0 && (uint32_t)page < a.cache.pages;
+    const size_t page_head = (size_t)(inside ? (uint32_t)page : 0u) * kv_heads + kv_head;
+    const int8_t* p = a.cache.values +
+                      ((page_head << shift) + (key & ((1u << shift) - 1u))) * D + 16u * n;
+#pragma unroll
+    for (int c = 0; c < 2 * kLoads; ++c) {
+      v[c] = *reinterpret_cast<const u32x4_t*>(p + 256 * c);
+    }
+    key_scale = a.cache.key_scales[page_head];
+    val_scale = a.cache.value_scales[page_head];
+  };
+
+  int32_t page_k = 0, page_v = 0;
+  if (wave < steps) {
+    page_k = page_of(first_key(wave) + 8u * (n >> 2));
+    page_v = page_of(first_key(wave) + 8u * g);
+  }
+
+  // The query: D / 4 values a lane, those of its dimensions 64 c + 16 g .. + 15.
+  half8_t q_hi[2 * kLoads], q_lo[kTwo ? 2 * kLoads : 1];
+  float row_factor;
+  {
+    float x[kLoads][16], largest = 0.0f;
+    const T* p = static_cast<const T*>(a.query) + at + 16u * g;
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        load4(p + 64 * c + 4 * i, &x[c][4 * i]);
+      }
+    }
+    if (wave < steps) {
+      load_k(wave, page_k);
+      load_v(wave, page_v);
+    }
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[c][i] = real ? x[c][i] : 0.0f;
+        largest = fmaxf(largest, fabsf(x[c][i]));
+      }
+    }
+    largest = xor32_max(xor16_max(largest));
+    const int e = query_exponent(largest);
+    // 1 / sqrt(D) in log2 units, over the row's power of two.
+    row_factor = ldexpf(kLog2e / (D == 64 ? 8.0f : D == 256 ? 16.0f : 11.313708498984761f), -e);
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        half8_t hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          half2_t u, w;
+          split_pair(ldexpf(x[c][8 * h + i], e), ldexpf(x[c][8 * h + i + 1], e), u, w);
+          hi[i] = u[0];
+          hi[i + 1] = u[1];
+          lo[i] = w[0];
+          lo[i + 1] = w[1];
+        }
+        if constexpr (kStacked) {
+          q_hi[2 * c + h] = n < 8u ? hi : lo;
+        } else {
+          q_hi[2 * c + h] = hi;
+          if constexpr (kTwo) {
+            q_lo[2 * c + h] = lo;
+          }
+        }
+      }
+    }
+  }
+
+  float4_t o[D / 16];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    o[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  float top = kLowestMax, sum = 0.0f;
+  // Keys that every row sees need no mask.
+  const uint32_t open = s.length - s.count + 1u;
+
+  for (uint32_t step = wave; step < steps; step += kWaves) {
+    const uint32_t next = step + kWaves;
+    if (next < steps) {
+      page_k = page_of(first_key(next) + 8u * (n >> 2));
+      page_v = page_of(first_key(next) + 8u * g);
+    }
+    float4_t score[2];
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      score[tile] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const half8_t x = codes_to_f16(k[tile][c][2 * h], k[tile][c][2 * h + 1]);
+          score[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q_hi[2 * c + h], score[tile],
+                                                               0, 0, 0);
+          if constexpr (kTwo) {
+            score[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q_lo[2 * c + h],
+                                                                 score[tile], 0, 0, 0);
+          }
+        }
+      }
+    }
+    const ValueScale sv = value_scale(val_scale);
+    const float factor = inside ? row_factor * key_scale : 0.0f;
+    const float offset = inside ? sv.exponent : -INFINITY;
+    float mantissa = inside ? sv.mantissa : 0.0f;
+    const uint32_t key = first_key(step) + 8u * g;
+    if (next < steps) {
+      load_k(next, page_k);
+    }
+    float w[8], largest = kLowestMax;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x = score[i / 4][i % 4];
+      if constexpr (kStacked) {
+        x += dpp<kDppRowRor8>(x);
+      }
+      w[i] = fmaf(x, factor, offset);
+    }
+    if (first_key(step) + 32u > open) {  // uniform
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = key + i < visible ? w[i] : -INFINITY;
+      }
+      // Of a page that the row does not see at all, the scale may be NaN.
+      mantissa = key < visible ? mantissa : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      largest = fmaxf(largest, w[i]);
+    }
+    largest = xor32_max(xor16_max(largest));
+    if (__any(largest > top)) {
+      const float up = fmaxf(top, largest);
+      const float keep = fast_exp2(top - up);
+      top = up;
+      sum *= keep;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        o[i] *= keep;
+      }
+    }
+    float all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = fast_exp2(w[i] - top);
+      all += w[i];
+    }
+    sum = fmaf(all, sv.shift, sum);
+    half8_t p_hi, p_lo;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      half2_t u, l;
+      if constexpr (!kStacked && !kTwo) {
+        u = half2_t{(half_t)(w[i] * mantissa), (half_t)(w[i + 1] * mantissa)};
+        l = u;
+      } else {
+        split_pair(w[i] * mantissa, w[i + 1] * mantissa, u, l);
+      }
+      p_hi[i] = u[0];
+      p_hi[i + 1] = u[1];
+      p_lo[i] = l[0];
+      p_lo[i + 1] = l[1];
+    }
+    if constexpr (kStacked) {
+      p_hi = n < 8u ? p_hi : p_lo;
+    }
+#pragma unroll
+    for (int c = 0; c < 2 * kLoads; ++c) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const half8_t x = codes_to_f16(v[c][2 * h], v[c][2 * h + 1]);
+        o[2 * c + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p_hi, o[2 * c + h], 0, 0, 0);
+        if constexpr (kTwo) {
+          o[2 * c + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p_lo, o[2 * c + h], 0, 0, 0);
+        }
+      }
+    }
+    if (next < steps) {
+      load_v(next, page_v);
+    }
+  }
+
+  // The waves' results to LDS, and their join.
+  sum = xor32_sum(xor16_sum(sum));
+  if constexpr (kStacked) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[i][j] += dpp<kDppRowRor8>(o[i][j]);
+      }
+    }
+  }
+  if (n < kRows) {
+    if (g == 0) {
+      lds_m[wave][n] = top;
+      lds_l[wave][n] = sum;
+    }
+    float* p = lds_o + (wave * kRows + n) * kStride;
+#pragma unroll
+    for (int c = 0; c < 2 * kLoads; ++c) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // Row 4 g + j of product (c, h) is dimension 32 c + 2 (4 g + j) + h.
+        *reinterpret_cast<float2*>(p + 32 * c + 8 * g + 2 * j) =
+          make_float2(o[2 * c][j], o[2 * c + 1][j]);
+      }
+    }
+  }
+  __syncthreads();
+  const bool whole = s.length <= split.decode_keys;
+  for (uint32_t i = threadIdx.x; i < rows * D; i += 256u) {
+    const uint32_t r = i / D, d = i % D;
+    float m = lds_m[0][r];
+#pragma unroll
+    for (uint32_t w = 1; w < kWaves; ++w) {
+      m = fmaxf(m, lds_m[w][r]);
+    }
+    float l = 0.0f, x = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+      const float keep = fast_exp2(lds_m[w][r] - m);
+      l = fmaf(keep, lds_l[w][r], l);
+      x = fmaf(keep, lds_o[(w * kRows + r) * kStride + d], x);
+    }
+    if (whole) {
+      const size_t out = ((size_t)(s.start + r / group) * a.heads + kv_head * group + r % group) * D;
+      store_output<T>(a, out + d, x, inverse_sum(l));
+    } else {
+      const size_t part = ((size_t)(blockIdx.x * a.batch.sequences + sequence) * kv_heads +
+                           kv_head) * split.decode_rows + r;
+      split.decode_o[part * D + d] = x;
+      if (d == 0) {
+        split.decode_ml[2 * part] = m;
+        split.decode_ml[2 * part + 1] = l;
+      }
+    }
+  }
+}
+
+// Joins split results: a wave per (row, head), D / 64 values a lane.
+template <int D, class T>
+__global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentionArgs a,
+                                                                   PagedSplit split) {
+  constexpr int kRegs = D / 64;
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint64_t item = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+  if (item >= (uint64_t)a.batch.tokens * a.heads) {
+    return;
+  }
+  const uint32_t token = (uint32_t)(item / a.heads), head = (uint32_t)(item % a.heads);
   uint32_t b = 0;
   for (uint32_t at = 1; at <= a.batch.sequences; at += 64) {
     const uint32_t i = at + lane;
-    b += (uint32_t)__popcll(__ballot(i <= a.batch.sequences && a.batch.starts[i] <= row));
+    b += (uint32_t)__popcll(__ballot(i <= a.batch.sequences && a.batch.starts[i] <= token));
   }
   if (b >= a.batch.sequences) {
     return;
   }
-  const PagedSequence s = paged_sequence(a.batch, b, shift);
-  if (row < s.start || row >= s.start + s.count) {
+  const PagedSequence s = paged_sequence(a.batch, b, a.cache.page_shift);
+  if (token < s.start || token >= s.start + s.count) {
     return;
   }
-  const uint32_t keys = s.length - s.count + (row - s.start) + 1u;
-  const uint32_t kv_head = head / (a.heads / a.cache.kv_heads);
-  const size_t at = ((size_t)row * a.heads + head) * d_head;
-  float q[kRegs], o[kRegs];
-  const float scale = 1.0f / sqrtf((float)d_head);
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i) {
-    q[i] = (float)static_cast<const T*>(a.query)[at + lane + 64 * i] * scale;
-    o[i] = 0.0f;
+  const uint32_t group = a.heads / a.cache.kv_heads;
+  const bool decode = s.count * group <= kDecodeRows;
+  const uint32_t per = decode ? split.decode_keys : split.tile_keys;
+  if (s.length <= per) {
+    return;  // written by its workgroup
   }
-  float m = -1e30f, l = 0.0f;
-  for (uint32_t j = 0; j < keys; ++j) {
-    const int32_t page = a.batch.table[(size_t)b * a.batch.width + (j >> shift)];
-    if (page < 0 || (uint32_t)page >= a.cache.pages) {
-      continue;
-    }
-    const uint32_t slot = j & ((1u << shift) - 1u);
-    const size_t page_head = (size_t)page * a.cache.kv_heads + kv_head;
-    const int8_t* k = a.cache.keys + ((page_head << shift) + slot) * d_head;
-    const int8_t* v = a.cache.values + (page_head << shift) * d_head +
-                      (size_t)(slot >> 3) * d_head * 8u + (slot & 7u);
-    float dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i) {
-      dot = fmaf(q[i], (float)k[lane + 64 * i], dot);
-    }
-    dot = wave_sum(dot) * a.cache.key_scales[page_head];
-    const float top = fmaxf(m, dot);
-    const float keep = expf(m - top), w = expf(dot - top);
-    m = top;
-    l = l * keep + w;
-    const float wv = w * a.cache.value_scales[page_head];
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i) {
-      o[i] = o[i] * keep + wv * (float)v[(size_t)(lane + 64 * i) * 8u];
-    }
+  // Splits whose first key the row sees.
+  const uint32_t visible = s.length - s.count + (token - s.start) + 1u;
+  const uint32_t splits = (visible + per - 1u) / per;
+  size_t first, stride;
+  const float *o, *ml;
+  if (decode) {
+    first = ((size_t)b * a.cache.kv_heads + head / group) * split.decode_rows +
+            (token - s.start) * group + head % group;
+    stride = (size_t)a.batch.sequences * a.cache.kv_heads * split.decode_rows;
+    o = split.decode_o;
+    ml = split.decode_ml;
+  } else {
+    first = (size_t)token * a.heads + head;
+    stride = (size_t)a.batch.tokens * a.heads;
+    o = split.tile_o;
+    ml = split.tile_ml;
+  }
+  float m = kLowestMax;
+  for (uint32_t i = lane; i < splits; i += 64) {
+    m = fmaxf(m, ml[2 * (first + i * stride)]);
   }
 #pragma unroll
-  for (int i = 0; i < kRegs; ++i) {
-    float x = l > 0.0f || l != l ? o[i] / l : 0.0f;
-    if (a.gate != nullptr) {
-      x *= 1.0f / (1.0f + expf(-a.gate[at + lane + 64 * i]));
+  for (int step = 1; step < 64; step *= 2) {
+    m = fmaxf(m, __shfl_xor(m, step, 64));
+  }
+  float l = 0.0f, x[kRegs] = {};
+  for (uint32_t at = 0; at < splits; at += 64) {
+    float keep = 0.0f;
+    if (at + lane < splits) {
+      const float2 part = *reinterpret_cast<const float2*>(&ml[2 * (first + (at + lane) * stride)]);
+      keep = fast_exp2(part.x - m);
+      l = fmaf(keep, part.y, l);
     }
-    static_cast<T*>(a.output)[at + lane + 64 * i] = static_cast<T>(x);
+    const uint32_t here = min(64u, splits - at);
+    // Eight parts' loads together; past the last they repeat it, with weight 0.
+    for (uint32_t i = 0; i < here; i += 8) {
+      float part[8][kRegs];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const float* p = o + (first + (at + min(i + j, here - 1u)) * stride) * D + lane * kRegs;
+#pragma unroll
+        for (int r = 0; r < kRegs; ++r) {
+          part[j][r] = p[r];
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const float k = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(keep), (int)(i + j)));
+#pragma unroll
+        for (int r = 0; r < kRegs; ++r) {
+          x[r] = i + j < here ? fmaf(k, part[j][r], x[r]) : x[r];
+        }
+      }
+    }
+  }
+  l = wave_sum(l);
+  const float inverse = inverse_sum(l);
+#pragma unroll
+  for (int r = 0; r < kRegs; ++r) {
+    store_output<T>(a, item * D + lane * kRegs + r, x[r], inverse);
+  }
+}
+
+PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
+  PagedSplit s{};
+  const uint64_t group = a.heads / a.cache.kv_heads;
+  const uint64_t rows = group * a.batch.max_query;
+  // Keys per workgroup: 128 (a 32-key step for each wave) while that gives no more than
+  // eight workgroups a CU at the longest length, up to 4096; more where the partial
+  // results of the longest lengths would take over 256 MiB.
+  const uint64_t lanes = (uint64_t)a.batch.sequences * a.cache.kv_heads;
+  const uint64_t part_bytes =
+    std::min<uint64_t>(rows, kDecodeRows) * (a.cache.head_dim + 2u) * sizeof(float);
+  auto parts = [&](uint64_t k) { return lanes * ((a.batch.max_keys + k - 1u) / k); };
+  uint64_t keys = 128;
+  while ((keys < 4096u && parts(keys) > 8u * (uint64_t)cu_count) ||
+         (parts(keys) > lanes && parts(keys) * part_bytes > (uint64_t{256} << 20))) {
+    keys *= 2u;
+  }
+  s.decode_keys = (uint32_t)keys;
+  s.decode_rows = (uint32_t)std::min<uint64_t>(rows, kDecodeRows);
+  s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
+  s.tile_keys = a.batch.max_keys;
+  s.tile_splits = 1;
+  return s;
+}
+
+size_t decode_parts(const PagedAttentionArgs& a, const PagedSplit& s) {
+  return s.decode_splits <= 1u ? 0u
+                               : (size_t)s.decode_splits * a.batch.sequences * a.cache.kv_heads *
+                                   s.decode_rows;
+}
+
+size_t tile_parts(const PagedAttentionArgs& a, const PagedSplit& s) {
+  return s.tile_splits <= 1u ? 0u : (size_t)s.tile_splits * a.batch.tokens * a.heads;
+}
+
+template <int D, class T>
+void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
+  const uint32_t group = a.heads / a.cache.kv_heads;
+  const uint64_t rows = (uint64_t)a.batch.max_query * group;
+  if (group <= kDecodeRows) {
+    const dim3 grid(split.decode_splits, a.cache.kv_heads, a.batch.sequences);
+    if (rows <= 8u) {
+      attention_paged_decode_kernel<D, T, true><<<grid, 256, 0, stream>>>(a, split);
+    } else {
+      attention_paged_decode_kernel<D, T, false><<<grid, 256, 0, stream>>>(a, split);
+    }
+  }
+  if (rows > kDecodeRows) {
+    (void)launch_attention_paged_q8_tiles(a, split, stream);
+  }
+  if (split.decode_splits > 1u || split.tile_splits > 1u) {
+    const uint64_t items = (uint64_t)a.batch.tokens * a.heads;
+    attention_paged_join_kernel<D, T><<<dim3((uint32_t)((items + 3u) / 4u)), 256, 0, stream>>>(
+      a, split);
   }
 }
 
 template <class T>
-void launch_plain(const PagedAttentionArgs& a, hipStream_t stream) {
-  const dim3 grid(a.batch.tokens * a.heads);
+void launch_type(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
   if (a.cache.head_dim == 256u) {
-    attention_paged_q8_plain<T, 4><<<grid, 64, 0, stream>>>(a);
+    launch_for<256, T>(a, split, stream);
   } else if (a.cache.head_dim == 128u) {
-    attention_paged_q8_plain<T, 2><<<grid, 64, 0, stream>>>(a);
+    launch_for<128, T>(a, split, stream);
   } else {
-    attention_paged_q8_plain<T, 1><<<grid, 64, 0, stream>>>(a);
+    launch_for<64, T>(a, split, stream);
   }
 }
 
 }  // namespace
 
-size_t attention_paged_q8_workspace_bytes(const PagedAttentionArgs&, int) { return 0; }
+size_t attention_paged_q8_workspace_bytes(const PagedAttentionArgs& a, int cu_count) {
+  const PagedSplit s = split_of(a, cu_count);
+  return (decode_parts(a, s) + tile_parts(a, s)) * (a.cache.head_dim + 2u) * sizeof(float);
+}
 
-hipError_t launch_attention_paged_q8(const PagedAttentionArgs& a, int, void*, hipStream_t stream) {
+hipError_t launch_attention_paged_q8(const PagedAttentionArgs& a, int cu_count, void* workspace,
+                                     hipStream_t stream) {
+  PagedSplit s = split_of(a, cu_count);
+  s.decode_o = static_cast<float*>(workspace);
+  s.tile_o = s.decode_o + decode_parts(a, s) * a.cache.head_dim;
+  s.decode_ml = s.tile_o + tile_parts(a, s) * a.cache.head_dim;
+  s.tile_ml = s.decode_ml + decode_parts(a, s) * 2u;
   if (a.f16) {
-    launch_plain<half_t>(a, stream);
+    launch_type<half_t>(a, s, stream);
   } else {
-    launch_plain<float>(a, stream);
+    launch_type<float>(a, s, stream);
   }
   return hipGetLastError();
 }

@@ -1,0 +1,133 @@
+// Parts shared by the attention kernels over 8-bit KV pages: codes as f16, query rows
+// as f16 parts, the softmax's bookkeeping and where split results lie.
+//
+// The arithmetic.  A code is an integer of at most 8 bits, exact in f16, so the matrix
+// cores take the codes themselves and the scales go elsewhere: a key page's scale into
+// the score (one multiply that the softmax scale needs anyhow), a value page's scale
+// sv = mu 2^b (b its exponent) into the weight.  With a = score in log2 units, the
+// running maximum M is kept of a + b, not of a, so that the weight that multiplies the
+// codes, 2^(a + b - M) mu, is at most 1 however far apart the scales of neighbouring
+// pages lie; the softmax's sum adds 2^(a + b - M) 2^-b, an exact shift.  Weights go into
+// f16 times 2^15, so that what falls below f16's normal range is 2^-29 of the largest.
+// A query row is multiplied by the power of two that takes its largest value to
+// [2^13, 2^14) and goes in as two f16 parts (hi, and what hi leaves), which holds 22
+// bits of each value down to 2^-16 of the row's largest; the weights likewise.  f16
+// queries are exact in the one part, and their weights are rounded once.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "device_common.hpp"
+#include "paged_q8_internal.hpp"
+
+namespace kraken {
+
+// Below every score that counts; a running maximum starts here, so that a masked
+// score's -inf gives a weight of 0 and not NaN.
+constexpr float kLowestMax = -1e30f;
+constexpr int kWeightShift = 15;
+
+// Sequences of at most this many rows (new tokens x query heads per KV head) take the
+// split decode kernel, longer ones the tiled one.
+constexpr uint32_t kDecodeRows = 16;
+
+// How a call's keys are split, and where the partial results lie: f32 sums [D] and
+// (M, l) of row r of (split, sequence, KV head) for the decode kernel, of (split, token,
+// head) for the tiled one.
+struct PagedSplit {
+  uint32_t decode_keys;   // keys per workgroup of the decode kernel
+  uint32_t decode_rows;   // rows held per (split, sequence, KV head)
+  uint32_t decode_splits;
+  uint32_t tile_keys;     // keys per workgroup of the tiled kernel
+  uint32_t tile_splits;
+  float* decode_o;
+  float* decode_ml;
+  float* tile_o;
+  float* tile_ml;
+};
+
+// Four codes (one dword, two's complement) as f16.  0x64uu is 1024 + uu in f16, so a
+// code offset to uu = code + 128 needs one byte permute for two values and one packed
+// subtraction of 1152.
+__device__ __forceinline__ half4_t codes_to_f16(uint32_t x) {
+  x ^= 0x80808080u;
+  const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u);
+  const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u);
+  const half2_t bias = {(half_t)-1152.0f, (half_t)-1152.0f};
+  const half2_t a = __builtin_bit_cast(half2_t, lo) + bias;
+  const half2_t b = __builtin_bit_cast(half2_t, hi) + bias;
+  return half4_t{a[0], a[1], b[0], b[1]};
+}
+
+__device__ __forceinline__ half8_t codes_to_f16(uint32_t x, uint32_t y) {
+  const half4_t a = codes_to_f16(x), b = codes_to_f16(y);
+  return half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// A value page's scale as mantissa and exponent for the weights.
+struct ValueScale {
+  float mantissa;  // times 2^kWeightShift
+  float exponent;  // added to the score
+  float shift;     // 2^-exponent, for the softmax's sum
+};
+
+__device__ __forceinline__ ValueScale value_scale(float s) {
+  // Not below 2^-100, so that 2^-b is finite.
+  const int b = max(__builtin_amdgcn_frexp_expf(s), -100);
+  return {ldexpf(s, kWeightShift - b), (float)b, ldexpf(1.0f, -b)};
+}
+
+// The exponent that takes a row's largest magnitude to [2^13, 2^14).
+__device__ __forceinline__ int query_exponent(float largest) {
+  return largest > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(largest) : 0;
+}
+
+// Two f32 as f16: hi rounded towards zero, lo what it leaves.
+__device__ __forceinline__ void split_pair(float x, float y, half2_t& hi, half2_t& lo) {
+  hi = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+  lo = __builtin_bit_cast(
+    half2_t, __builtin_amdgcn_cvt_pkrtz(x - (float)hi[0], y - (float)hi[1]));
+}
+
+template <class T>
+__device__ __forceinline__ void load4(const T* p, float v[4]) {
+  if constexpr (std::is_same<T, float>::value) {
+    const float4_t x = *reinterpret_cast<const float4_t*>(p);
+    v[0] = x[0];
+    v[1] = x[1];
+    v[2] = x[2];
+    v[3] = x[3];
+  } else {
+    const half4_t x = *reinterpret_cast<const half4_t*>(p);
+    v[0] = x[0];
+    v[1] = x[1];
+    v[2] = x[2];
+    v[3] = x[3];
+  }
+}
+
+// out[i] = sum / l, gated.  A sum without any key (l = 0) is zero.
+template <class T>
+__device__ __forceinline__ void store_output(const PagedAttentionArgs& a, size_t at, float sum,
+                                             float inverse) {
+  float x = sum * inverse;
+  if constexpr (std::is_same<T, float>::value) {
+    if (a.gate != nullptr) {
+      x *= 1.0f / (1.0f + expf(-a.gate[at]));
+    }
+  }
+  static_cast<T*>(a.output)[at] = static_cast<T>(x);
+}
+
+// 1 / l in the sums' unit; l = 0: no key, NaN: NaN.
+__device__ __forceinline__ float inverse_sum(float l) {
+  return l == 0.0f ? 0.0f : ldexpf(1.0f / l, -kWeightShift);
+}
+
+hipError_t launch_attention_paged_q8_tiles(const PagedAttentionArgs& a, const PagedSplit& split,
+                                           hipStream_t stream);
+
+}  // namespace kraken

@@ -15,6 +15,10 @@ using namespace kraken;
 namespace {
 
 constexpr size_t kInt32Max = 0x7fffffffu;
+// Limits of a launch's dimensions: sequences and KV heads are two of them, and the rows
+// (tokens x heads) four to a workgroup of 256 threads.
+constexpr size_t kMaxGrid = 65535;
+constexpr size_t kMaxRows = size_t{1} << 26;
 
 // The cache's checks; `w` begins the messages.
 int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c) {
@@ -53,7 +57,9 @@ int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c
   if (((uintptr_t)cache->key_pages.data | (uintptr_t)cache->value_pages.data) & 15u) {
     return invalid("HIP " + at + " pages must be 16-byte aligned");
   }
-  KRAKEN_TRY(check_u32(cache->kv_heads, w, " kv_heads"));
+  if (cache->kv_heads > kMaxGrid) {
+    return invalid("HIP " + at + " takes up to 65535 kv_heads");
+  }
   c.keys = static_cast<int8_t*>(cache->key_pages.data);
   c.values = static_cast<int8_t*>(cache->value_pages.data);
   c.key_scales = static_cast<float*>(cache->key_scales.data);
@@ -74,9 +80,11 @@ int batch_args(const kraken_paged_batch* batch, const char* w, PagedBatchArgs& b
       batch->max_query == 0 || batch->max_keys == 0) {
     return invalid("HIP " + at + " batch dimensions must be positive");
   }
-  if (batch->tokens > kInt32Max || batch->max_keys > kInt32Max ||
-      batch->sequences > kInt32Max) {
+  if (batch->tokens > kInt32Max || batch->max_keys > kInt32Max) {
     return invalid("HIP " + at + " batch exceeds int32 range");
+  }
+  if (batch->sequences > kMaxGrid) {
+    return invalid("HIP " + at + " takes up to 65535 sequences");
   }
   size_t entries = 0;
   if (!checked_mul(batch->sequences, batch->table_width, entries)) {
@@ -125,8 +133,8 @@ int paged_attention_entry(kraken_hip_context* ctx, const kraken_buffer& query,
   if (!checked_mul(batch->tokens, heads, rows) || !checked_mul(rows, cache->head_dim, values)) {
     return invalid("HIP paged attention value count overflow");
   }
-  if (rows > kInt32Max) {
-    return invalid("HIP paged attention row count exceeds int32 range");
+  if (rows > kMaxRows) {
+    return invalid("HIP paged attention takes up to 67108864 query rows");
   }
   const size_t element = f16 ? sizeof(uint16_t) : sizeof(float);
   KRAKEN_TRY(validate_buffer(query, values, element, w, " query"));

@@ -112,13 +112,14 @@ def append(cache, name, rows, batch):
 
 
 def attention(cache, query, batch, heads, gate=None):
-    """Returns (output, magnitude, score) [tokens][heads][dim]: magnitude is the sum
-    of the absolute weighted values, score [tokens][heads] the largest sum of absolute
-    products of a query with a key.  Rows of no sequence are NaN."""
+    """Returns (output, magnitude, score): magnitude [tokens][heads][dim] is the sum of
+    the absolute weighted values, score [tokens][heads][2] the largest sum of absolute
+    products of a query with a key, and the number of keys times the largest product of
+    a weight with its value page's scale.  Rows of no sequence are NaN."""
     table, starts, lengths, tokens, max_query, max_keys = batch
     d, g, pt = cache.head_dim, heads // cache.kv_heads, cache.page_tokens
     out = np.full((tokens, heads, d), np.nan)
-    size, score = np.full_like(out, np.nan), np.full((tokens, heads), np.nan)
+    size, score = np.full_like(out, np.nan), np.full((tokens, heads, 2), np.nan)
     for b, first, count, length in live_sequences(cache, *batch):
         if count == 0:
             continue
@@ -127,6 +128,7 @@ def attention(cache, query, batch, heads, gate=None):
         empty = np.zeros((pt, cache.kv_heads, d))
         k, v = (np.concatenate([cache.values_of(n, i) if inside(cache, i) else empty
                                 for i in ids])[where] for n in ("key", "value"))
+        steps = np.array([cache.scales["value"][ids[pos // pt]] for pos in where], np.float64)
         for i in range(count):
             seen = int((where <= length - count + i).sum())
             for h in range(heads):
@@ -141,7 +143,8 @@ def attention(cache, query, batch, heads, gate=None):
                 w /= w.sum()
                 out[first + i, h] = w @ vv
                 size[first + i, h] = w @ np.abs(vv)
-                score[first + i, h] = (np.abs(kk) @ np.abs(q)).max() / math.sqrt(d)
+                score[first + i, h] = ((np.abs(kk) @ np.abs(q)).max() / math.sqrt(d),
+                                       seen * (w * steps[:seen, h // g]).max())
     if gate is not None:
         out *= 1.0 / (1.0 + np.exp(-gate.astype(np.float64)))
     return out, size, score
@@ -154,7 +157,8 @@ def attention_tolerance(magnitude, out, score, head_dim, f16):
     and the division add at most 64 half steps.  With f16 a weight is off by half a
     step of f16, and so is the output."""
     step = 2.0 ** -24
-    tol = magnitude * step * (8.0 * math.sqrt(head_dim) * score[..., None] + 64.0)
+    tol = magnitude * step * (8.0 * math.sqrt(head_dim) * score[..., :1] + 64.0)
+    tol = tol + 127.0 * 2.0 ** -38 * score[..., 1:]
     if f16:
         tol = tol + magnitude * 2.0 ** -11 + np.abs(out) * 2.0 ** -11 + 2.0 ** -25
     return tol + 1e-30

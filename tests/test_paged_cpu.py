@@ -73,6 +73,7 @@ BATCH_ERRORS = [
     (dict(max_query=0), "batch dimensions must be positive"),
     (dict(tokens=0), "batch dimensions must be positive"),
     (dict(max_keys=1 << 31), "batch exceeds int32 range"),
+    (dict(sequences=65536), "takes up to 65535 sequences"),
     (dict(width=1 << 62), "overflow"),
     (dict(table=fake(23)), "page table buffer is too small"),
     (dict(starts=fake(12)), "query starts buffer is too small"),
@@ -128,7 +129,7 @@ def test_prologue_refusals(vctx, kw, fragment):
     (dict(o=kh.KrakenBuffer(None, 1 << 20)), "output buffer is not initialized"),
     (dict(q=fake(1 << 20, 0x1004)), "buffers must be 16-byte aligned"),
     (dict(batch=batch_of(tokens=(1 << 31) - 1), o=fake(1 << 62), q=fake(1 << 62)),
-     "row count exceeds int32 range"),
+     "takes up to 67108864 query rows"),
 ])
 def test_attention_refusals(vctx, kw, fragment, f16):
     name = "attention_f16q_paged_q8_kv" if f16 else "attention_f32_paged_q8_kv"
