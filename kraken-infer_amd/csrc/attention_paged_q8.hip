@@ -441,8 +441,24 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   s.decode_keys = (uint32_t)keys;
   s.decode_rows = (uint32_t)std::min<uint64_t>(rows, kDecodeRows);
   s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
-  s.tile_keys = a.batch.max_keys;
-  s.tile_splits = 1;
+  // The tiled kernel's keys in parts until there are two workgroups a CU, each of 512
+  // keys at least, and while their results take no more than 256 MiB.
+  const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows * a.cache.kv_heads;
+  const uint64_t all_tiles =
+    std::min<uint64_t>(tiles * a.batch.sequences,
+                       ((uint64_t)a.batch.tokens * group + kTileRows - 1u) / kTileRows *
+                           a.cache.kv_heads +
+                         (uint64_t)a.batch.sequences * a.cache.kv_heads);
+  const uint64_t row_bytes =
+    (uint64_t)a.batch.tokens * a.heads * (a.cache.head_dim + 2u) * sizeof(float);
+  uint64_t splits = 1;
+  while (rows > kDecodeRows && all_tiles * splits < 2u * (uint64_t)cu_count &&
+         a.batch.max_keys / (2u * splits) >= 512u &&
+         2u * splits * row_bytes <= (uint64_t{256} << 20)) {
+    splits *= 2u;
+  }
+  s.tile_keys = (uint32_t)((a.batch.max_keys + splits - 1u) / splits + 63u) & ~63u;
+  s.tile_splits = (uint32_t)((a.batch.max_keys + s.tile_keys - 1u) / s.tile_keys);
   return s;
 }
 
@@ -469,7 +485,7 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
     }
   }
   if (rows > kDecodeRows) {
-    (void)launch_attention_paged_q8_tiles(a, split, stream);
+    launch_attention_paged_q8_tiles(a, split, stream);
   }
   if (split.decode_splits > 1u || split.tile_splits > 1u) {
     const uint64_t items = (uint64_t)a.batch.tokens * a.heads;

@@ -33,6 +33,8 @@ constexpr int kWeightShift = 15;
 // Sequences of at most this many rows (new tokens x query heads per KV head) take the
 // split decode kernel, longer ones the tiled one.
 constexpr uint32_t kDecodeRows = 16;
+// Rows of the tiled kernel's workgroups.
+constexpr uint32_t kTileRows = 128;
 
 // How a call's keys are split, and where the partial results lie: f32 sums [D] and
 // (M, l) of row r of (split, sequence, KV head) for the decode kernel, of (split, token,
@@ -127,7 +129,7 @@ __device__ __forceinline__ float inverse_sum(float l) {
   return l == 0.0f ? 0.0f : ldexpf(1.0f / l, -kWeightShift);
 }
 
-hipError_t launch_attention_paged_q8_tiles(const PagedAttentionArgs& a, const PagedSplit& split,
-                                           hipStream_t stream);
+void launch_attention_paged_q8_tiles(const PagedAttentionArgs& a, const PagedSplit& split,
+                                     hipStream_t stream);
 
 }  // namespace kraken
