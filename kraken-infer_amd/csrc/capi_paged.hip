@@ -296,8 +296,8 @@ KRAKEN_API int kraken_hip_sample_f32_i32(kraken_hip_context* ctx, kraken_buffer 
   if (!checked_mul(rows - 1u, row_stride, values) || !checked_add(values, size, values)) {
     return invalid("HIP sample value count overflow");
   }
-  if (size > (size_t{1} << 24) || rows > 65535u) {
-    return invalid("HIP sample takes rows of up to 16777216 logits, and 65535 of them");
+  if (size > (size_t{1} << 22) || rows > 65535u) {
+    return invalid("HIP sample takes rows of up to 4194304 logits, and 65535 of them");
   }
   KRAKEN_TRY(validate_f32(logits, values, w, " logits"));
   const struct {

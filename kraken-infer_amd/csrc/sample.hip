@@ -11,14 +11,14 @@
 //
 // Four launches, the first three with a workgroup for each chunk of a row:
 //   top     the largest key of the chunk and its first index
-//   bins    the row's histogram over 1/8 octaves of weight: how many and how much, and
-//           each chunk's own weights by bin
+//   bins    the row's histogram over 1/8 octaves of weight (how much, and how many where
+//           top-k asks) and each chunk's own
 //   gather  the histogram says which bins a threshold can lie in (one, or a few where
-//           top-p depends on a top-k that is not resolved yet): their elements go to a
+//           top-p depends on a top-k that is not resolved yet); their elements go to a
 //           list, and what lies above them is summed by chunk from the chunk's bins
 //   draw    one workgroup a row: the threshold by radix selection in the list, then the
 //           chunk in which the draw falls, and the token by a scan of that chunk alone.
-// So a row is read three times, from memory once (the rest from the caches), and
+// So a row is read three times, from memory once (the rest from the caches), and its
 // exponentials are formed once.
 #include <hip/hip_runtime.h>
 
@@ -31,10 +31,12 @@
 namespace kraken {
 namespace {
 
-constexpr uint32_t kThreads = 256;       // of the chunk kernels
-constexpr uint32_t kDrawThreads = 1024;  // of the draw
-constexpr uint32_t kBins = 512;          // 1/8 octave each; the last takes all below 2^-63
-constexpr uint32_t kMaxChunks = 4096;
+constexpr uint32_t kThreads = 256;      // of the chunk kernels
+constexpr uint32_t kDrawThreads = 512;  // of the draw
+constexpr uint32_t kBins = 512;         // 1/8 octave each; the last takes all below 2^-63
+constexpr uint32_t kMaxChunk = 4096;    // logits of a chunk
+constexpr uint32_t kMaxChunks = 1024;   // of a row
+constexpr uint32_t kHeld = 8192;        // entries of the list that the draw holds in LDS
 constexpr uint32_t kMinusInfKey = 0x007fffffu;
 
 // Keys order as the logits do; 0 for NaN, which is below -inf's, and -0 as +0.
@@ -78,19 +80,49 @@ __device__ __forceinline__ bool takes_top(const RowRule& rule, uint32_t top) {
   return rule.greedy || rule.min_p > 1.0 || top <= kMinusInfKey;
 }
 
-// The weight of a key; `top` is the largest.
-__device__ __forceinline__ double weight_of(uint32_t key, uint32_t top, double inverse) {
-  if (key == top) {
-    return 1.0;
-  }
-  if (key <= kMinusInfKey) {
-    return 0.0;
-  }
-  return exp(((double)logit_of(key) - (double)logit_of(top)) * inverse);
+// A row's weights: exp((l - max) / T) 2^shift as an integer.
+struct Weights {
+  uint32_t top;
+  double top_logit, factor;  // of log2(e) / T
+  int shift;
+};
+
+__device__ __forceinline__ Weights weights_of(uint32_t top, const RowRule& rule, int shift) {
+  return {top, (double)logit_of(top), 1.4426950408889634074 * rule.inverse_temperature, shift};
 }
 
-__device__ __forceinline__ uint64_t fixed(double w, int shift) {
-  return (uint64_t)__double2ll_rn(ldexp(w, shift));
+// 2^y for y <= 0 (0 from -1000 down) times 2^shift: y = n + f with |f| <= 1/2, and the
+// Taylor series of e^(f ln 2), whose first term left out is (ln 2 / 2)^12 / 12! = 6e-15.
+__device__ __forceinline__ double exp2_scaled(double y, int shift) {
+  const double n = rint(y);
+  const double t = (y - n) * 0.69314718055994530942;
+  double r = 1.0 / 39916800.0;
+  r = fma(r, t, 1.0 / 3628800.0);
+  r = fma(r, t, 1.0 / 362880.0);
+  r = fma(r, t, 1.0 / 40320.0);
+  r = fma(r, t, 1.0 / 5040.0);
+  r = fma(r, t, 1.0 / 720.0);
+  r = fma(r, t, 1.0 / 120.0);
+  r = fma(r, t, 1.0 / 24.0);
+  r = fma(r, t, 1.0 / 6.0);
+  r = fma(r, t, 0.5);
+  r = fma(r, t, 1.0);
+  r = fma(r, t, 1.0);
+  return y > -1000.0 ? ldexp(r, (int)n + shift) : 0.0;
+}
+
+// In units of 2^-shift, before rounding to a whole number.
+__device__ __forceinline__ double weight_real(uint32_t key, const Weights& w) {
+  // The largest logit may be infinite, and so may the factor.
+  return key == w.top ? ldexp(1.0, w.shift)
+         : key <= kMinusInfKey
+           ? 0.0
+           : exp2_scaled(((double)logit_of(key) - w.top_logit) * w.factor, w.shift);
+}
+
+__device__ __forceinline__ uint64_t weight_fixed(uint32_t key, const Weights& w) {
+  // Up to 2^51, an addition of 2^52 leaves the rounded number in the low bits.
+  return (uint64_t)__double_as_longlong(weight_real(key, w) + 0x1p52) & ((uint64_t{1} << 52) - 1u);
 }
 
 // The bin of a key: falling weights fall into rising bins (each step of it is
@@ -100,15 +132,32 @@ __device__ __forceinline__ uint32_t bin_of(uint32_t key, uint32_t top, float sca
   return key == top ? 0u : (uint32_t)fminf(z, (float)(kBins - 1u));  // NaN: the last
 }
 
+// Which bins a row's threshold can lie in, and the row's largest.
+struct RowMeta {
+  uint64_t above;      // weight and number of the bins below `sure`
+  uint64_t total;      // weight of the row
+  uint32_t above_n;
+  uint32_t sure;       // bins below are kept whatever the threshold
+  uint32_t last;       // bins sure .. last are listed; none if last < sure
+  uint32_t cut;        // top-k or top-p cuts inside the list
+  uint32_t top, top_index;
+};
+
+struct Entry {
+  uint32_t index, key;
+  uint64_t weight;
+};
+
 // A row's place in the workspace.
 struct RowWork {
-  uint64_t* bin_weight;   // [kBins]
-  uint32_t* bin_count;    // [kBins]
-  uint32_t* listed;       // number of entries of the list
-  uint64_t* chunk_weight; // [chunks]: of what is kept whatever the threshold
-  uint64_t* chunk_top;    // [chunks]: key << 32 | ~index
-  uint64_t* chunk_bins;   // [chunks][kBins]
-  uint64_t* list;         // [size]: key << 32 | index
+  RowMeta* meta;
+  uint64_t* bin_weight;    // [kBins]
+  uint32_t* bin_count;     // [kBins]
+  uint64_t* chunk_weight;  // [chunks]: of what is kept whatever the threshold
+  uint64_t* chunk_top;     // [chunks]: key << 32 | ~index
+  uint32_t* chunk_listed;  // [chunks]: entries of the chunk's part of the list
+  uint64_t* chunk_bins;    // [chunks][kBins]
+  Entry* list;             // [chunks][chunk]
 };
 
 struct Plan {
@@ -118,43 +167,85 @@ struct Plan {
   size_t row_words;  // 8-byte words of the workspace per row
 };
 
-__host__ __device__ __forceinline__ size_t words_per_row(uint32_t chunks, uint32_t size) {
-  return kBins + kBins / 2u + 1u + (size_t)chunks * (2u + kBins) + size;
+constexpr size_t kMetaWords = 8;
+
+size_t words_per_row(const Plan& p) {
+  return kMetaWords + kBins + kBins / 2u + (size_t)p.chunks * (2u + kBins) +
+         ((size_t)p.chunks / 2u + 1u) / 2u * 2u + 2u + 2u * (size_t)p.chunks * p.chunk;
 }
 
 __device__ __forceinline__ RowWork row_work(const Plan& p, uint32_t row) {
+  static_assert(sizeof(RowMeta) <= kMetaWords * sizeof(uint64_t), "");
   RowWork w;
-  w.bin_weight = p.work + (size_t)row * p.row_words;
+  uint64_t* at = p.work + (size_t)row * p.row_words;
+  w.meta = reinterpret_cast<RowMeta*>(at);
+  w.bin_weight = at + kMetaWords;
   w.bin_count = reinterpret_cast<uint32_t*>(w.bin_weight + kBins);
-  w.listed = w.bin_count + kBins;
-  w.chunk_weight = w.bin_weight + kBins + kBins / 2u + 1u;
+  w.chunk_weight = w.bin_weight + kBins + kBins / 2u;
   w.chunk_top = w.chunk_weight + p.chunks;
   w.chunk_bins = w.chunk_top + p.chunks;
-  w.list = w.chunk_bins + (size_t)p.chunks * kBins;
+  // The list is 16-byte aligned: an even number of words before it.
+  w.list = reinterpret_cast<Entry*>(w.chunk_bins + (size_t)p.chunks * kBins);
+  w.chunk_listed = reinterpret_cast<uint32_t*>(w.list + (size_t)p.chunks * p.chunk);
   return w;
 }
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t x) {
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    const uint64_t y = (uint64_t)__shfl_xor((long long)x, step, 64);
-    x = y > x ? y : x;
-  }
+// Steps of a scan over a wave: lanes 1, 2, 4 and 8 before within a row of 16, then the
+// last of the row before, and of the two rows before.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t lanes_before(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, kRows, 0xf, true);
+}
+
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint64_t lanes_before(uint64_t x) {
+  return (uint64_t)lanes_before<kCtrl, kRows>((uint32_t)(x >> 32)) << 32 |
+         lanes_before<kCtrl, kRows>((uint32_t)x);
+}
+
+// Inclusive scan over the wave; 0 is the identity of `op`.
+template <class T, class Op>
+__device__ __forceinline__ T wave_scan(T x, Op op) {
+  x = op(x, lanes_before<0x111, 0xf>(x));
+  x = op(x, lanes_before<0x112, 0xf>(x));
+  x = op(x, lanes_before<0x114, 0xf>(x));
+  x = op(x, lanes_before<0x118, 0xf>(x));
+  x = op(x, lanes_before<0x142, 0xa>(x));
+  x = op(x, lanes_before<0x143, 0xc>(x));
   return x;
 }
 
-// Largest over the workgroup of kWaves waves.
-template <uint32_t kWaves>
-__device__ __forceinline__ uint64_t block_max(uint64_t x, uint64_t* s) {
-  x = wave_max_u64(x);
+__device__ __forceinline__ uint64_t last_lane(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+struct Sum {
+  template <class T>
+  __device__ __forceinline__ T operator()(T x, T y) const {
+    return x + y;
+  }
+};
+struct Largest {
+  template <class T>
+  __device__ __forceinline__ T operator()(T x, T y) const {
+    return x > y ? x : y;
+  }
+};
+
+// op over a workgroup of kWaves waves, the result in every thread.
+template <uint32_t kWaves, class Op>
+__device__ __forceinline__ uint64_t block_reduce(uint64_t x, Op op, uint64_t* s) {
+  x = last_lane(wave_scan(x, op));
   __syncthreads();
   if ((threadIdx.x & 63u) == 0) {
     s[threadIdx.x >> 6] = x;
   }
   __syncthreads();
   x = s[0];
+#pragma unroll
   for (uint32_t i = 1; i < kWaves; ++i) {
-    x = s[i] > x ? s[i] : x;
+    x = op(x, s[i]);
   }
   return x;
 }
@@ -166,13 +257,8 @@ __device__ __forceinline__ void block_scan(uint64_t& x, uint32_t& n, uint64_t& a
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint64_t own = x;
   const uint32_t own_n = n;
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    const uint64_t y = (uint64_t)__shfl_up((long long)x, step, 64);
-    const uint32_t m = (uint32_t)__shfl_up((int)n, step, 64);
-    x += lane >= (uint32_t)step ? y : 0u;
-    n += lane >= (uint32_t)step ? m : 0u;
-  }
+  x = wave_scan(x, Sum{});
+  n = wave_scan(n, Sum{});
   __syncthreads();
   if (lane == 63u) {
     sums[wave] = x;
@@ -192,24 +278,6 @@ __device__ __forceinline__ void block_scan(uint64_t& x, uint32_t& n, uint64_t& a
   }
   x = x - own + before;
   n = n - own_n + before_n;
-}
-
-template <uint32_t kWaves>
-__device__ __forceinline__ uint64_t block_sum(uint64_t x, uint64_t* s) {
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    x += (uint64_t)__shfl_xor((long long)x, step, 64);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63u) == 0) {
-    s[threadIdx.x >> 6] = x;
-  }
-  __syncthreads();
-  x = 0;
-  for (uint32_t i = 0; i < kWaves; ++i) {
-    x += s[i];
-  }
-  return x;
 }
 
 // Calls f(index, logit) for this thread's logits of [begin, end) of a row, four at a
@@ -249,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, Plan
     const uint64_t both = (uint64_t)key << 32 | (uint32_t)~i;
     top = key != 0u && both > top ? both : top;
   });
-  top = block_max<kThreads / 64u>(top, s);
+  top = block_reduce<kThreads / 64u>(top, Largest{}, s);
   if (threadIdx.x == 0) {
     w.chunk_top[chunk] = top;
   }
@@ -258,94 +326,37 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, Plan
       w.bin_weight[i] = 0;
       w.bin_count[i] = 0;
     }
-    if (threadIdx.x == 0) {
-      *w.listed = 0;
-    }
   }
 }
 
-// The row's largest key, from its chunks'.
-template <uint32_t kWaves>
-__device__ __forceinline__ uint64_t row_top(const RowWork& w, uint32_t chunks, uint64_t* s) {
-  uint64_t top = 0;
-  for (uint32_t i = threadIdx.x; i < chunks; i += kWaves * 64u) {
-    top = w.chunk_top[i] > top ? w.chunk_top[i] : top;
-  }
-  return block_max<kWaves>(top, s);
+// Whether the condition holds here and in no later lane of the wave.
+__device__ __forceinline__ bool last_that(bool condition) {
+  const uint64_t all = __ballot(condition);
+  return condition && (threadIdx.x & 63u) == 63u - (uint32_t)__builtin_clzll(all);
 }
-
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Plan p) {
-  constexpr uint32_t kWaves = kThreads / 64u;
-  __shared__ uint64_t s[kWaves];
-  __shared__ uint64_t weights[kBins];
-  __shared__ uint32_t counts[kBins];
-  const uint32_t row = blockIdx.y, chunk = blockIdx.x;
-  const RowRule rule = row_rule(a, row);
-  const RowWork w = row_work(p, row);
-  const uint32_t top = (uint32_t)(row_top<kWaves>(w, p.chunks, s) >> 32);
-  if (takes_top(rule, top)) {
-    return;
-  }
-  for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
-    weights[i] = 0;
-    counts[i] = 0;
-  }
-  __syncthreads();
-  const float scale = (float)(8.0 * 1.4426950408889634 * rule.inverse_temperature);
-  const uint32_t begin = chunk * p.chunk, end = min(a.size, begin + p.chunk);
-  each_logit(a.logits + (size_t)row * a.row_stride, begin, end, [&](uint32_t, float x) {
-    const uint32_t key = key_of(x);
-    if (key != 0u) {
-      const uint32_t bin = bin_of(key, top, scale);
-      const uint64_t v = fixed(weight_of(key, top, rule.inverse_temperature), p.shift);
-      atomicAdd((unsigned long long*)&weights[bin], (unsigned long long)v);
-      atomicAdd(&counts[bin], 1u);
-    }
-  });
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
-    w.chunk_bins[(size_t)chunk * kBins + i] = weights[i];
-    if (counts[i] != 0u) {
-      atomicAdd((unsigned long long*)&w.bin_weight[i], (unsigned long long)weights[i]);
-      atomicAdd(&w.bin_count[i], counts[i]);
-    }
-  }
-}
-
-// Which bins a row's threshold can lie in.
-struct Bounds {
-  uint32_t sure;       // bins below are kept whatever the threshold
-  uint32_t last;       // bins sure .. last are listed; none if last < sure
-  bool cut;            // top-k or top-p cuts inside the list
-  uint64_t above;      // weight and number of the bins below `sure`
-  uint32_t above_n;
-  uint64_t total;      // weight of the row
-};
 
 struct BoundScratch {
-  uint64_t sums[16];
-  uint32_t counts[16];
-  uint64_t before[kBins];    // weight of the bins before
-  uint64_t k_before, k_weight;
+  uint64_t before[kBins];  // weight of the bins before
   uint32_t before_n[kBins];
+  uint64_t k_before, k_weight;
   uint32_t k_bin, p_first, p_last;
 };
 
-// kWaves * 64 threads, kBins / that many bins each (at least one).
-template <uint32_t kWaves>
-__device__ Bounds row_bounds(const RowRule& rule, const RowWork& w, BoundScratch& s) {
-  constexpr uint32_t kPer = kBins > kWaves * 64u ? kBins / (kWaves * 64u) : 1u;
-  const bool holds = threadIdx.x * kPer < kBins;
+// The bins that the row's threshold can lie in, from its histogram.
+__device__ RowMeta row_bounds(const RowRule& rule, const RowWork& w, uint64_t* sums,
+                              uint32_t* counts, BoundScratch& s) {
+  constexpr uint32_t kWaves = kThreads / 64u, kPer = kBins / kThreads;
   uint64_t weight[kPer], x = 0, total;
   uint32_t count[kPer], n = 0, all_n;
 #pragma unroll
   for (uint32_t i = 0; i < kPer; ++i) {
-    weight[i] = holds ? w.bin_weight[threadIdx.x * kPer + i] : 0u;
-    count[i] = holds ? w.bin_count[threadIdx.x * kPer + i] : 0u;
+    const uint32_t bin = threadIdx.x * kPer + i;
+    weight[i] = w.bin_weight[bin];
+    count[i] = w.bin_count[bin];
     x += weight[i];
     n += count[i];
   }
-  block_scan<kWaves>(x, n, total, all_n, s.sums, s.counts);
+  block_scan<kWaves>(x, n, total, all_n, sums, counts);
   if (threadIdx.x == 0) {
     s.k_bin = kBins;
     s.k_before = total;
@@ -358,18 +369,16 @@ __device__ Bounds row_bounds(const RowRule& rule, const RowWork& w, BoundScratch
   uint32_t at_n = n;
 #pragma unroll
   for (uint32_t i = 0; i < kPer; ++i) {
-    if (holds) {
-      const uint32_t bin = threadIdx.x * kPer + i;
-      s.before[bin] = at;
-      s.before_n[bin] = at_n;
-      if (rule.top_k != 0u && at_n < rule.top_k && at_n + count[i] >= rule.top_k) {
-        s.k_bin = bin;  // one bin only
-        s.k_before = at;
-        s.k_weight = weight[i];
-      }
-      at += weight[i];
-      at_n += count[i];
+    const uint32_t bin = threadIdx.x * kPer + i;
+    s.before[bin] = at;
+    s.before_n[bin] = at_n;
+    if (rule.top_k != 0u && at_n < rule.top_k && at_n + count[i] >= rule.top_k) {
+      s.k_bin = bin;  // one bin only
+      s.k_before = at;
+      s.k_weight = weight[i];
     }
+    at += weight[i];
+    at_n += count[i];
   }
   __syncthreads();
   const uint32_t k_bin = s.k_bin;
@@ -379,75 +388,159 @@ __device__ Bounds row_bounds(const RowRule& rule, const RowWork& w, BoundScratch
     const double least = rule.top_p * (double)s.k_before;
     const double most = rule.top_p * (double)(s.k_before + s.k_weight);
     at = x;
+    uint32_t first = 0, last = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kPer; ++i) {
       const uint32_t bin = threadIdx.x * kPer + i;
-      if (holds && count[i] != 0u && bin <= k_bin) {
-        if ((double)at < least) {
-          atomicMax(&s.p_first, bin);
-        }
-        if ((double)at < most) {
-          atomicMax(&s.p_last, bin);
-        }
+      if (weight[i] != 0u && bin <= k_bin) {
+        first = (double)at < least ? bin : first;
+        last = (double)at < most ? bin : last;
       }
       at += weight[i];
     }
+    // One atomic a wave, of its last thread that found one.
+    if (last_that(first != 0u)) {
+      atomicMax(&s.p_first, first);
+    }
+    if (last_that(last != 0u)) {
+      atomicMax(&s.p_last, last);
+    }
   }
   __syncthreads();
-  Bounds b;
+  RowMeta b;
   b.total = total;
   b.cut = rule.top_k != 0u || rule.top_p < 1.0;
   b.sure = rule.top_p < 1.0 ? s.p_first : k_bin;
-  b.last = rule.top_k != 0u ? k_bin : rule.top_p < 1.0 ? s.p_last : 0u;
+  b.last = rule.top_k != 0u ? min(k_bin, kBins - 1u) : rule.top_p < 1.0 ? s.p_last : 0u;
   if (rule.min_p > 0.0) {
     // The border of min_p lies in its bin, or a neighbour of it by rounding.
     const uint32_t bin = (uint32_t)fmin(-8.0 * log2(rule.min_p), (double)(kBins - 1u));
     const uint32_t low = bin != 0u ? bin - 1u : 0u, high = min(bin + 1u, kBins - 1u);
     if (!b.cut || high < b.sure) {
-      b.cut = false;  // top-k and top-p keep all that min-p does
+      b.cut = 0;  // top-k and top-p keep all that min-p does
       b.last = high;
     }
     b.sure = min(b.sure, low);
-  } else if (!b.cut) {
-    b.sure = kBins;
+  }
+  if (b.sure == kBins) {
+    b.last = 0;  // no list: everything is kept
   }
   b.above = b.sure < kBins ? s.before[b.sure] : total;
   b.above_n = b.sure < kBins ? s.before_n[b.sure] : all_n;
   return b;
 }
 
-__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, Plan p) {
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Plan p) {
   constexpr uint32_t kWaves = kThreads / 64u;
   __shared__ uint64_t s[kWaves];
-  __shared__ BoundScratch bs;
+  __shared__ uint64_t bin_weight[kBins];
+  __shared__ uint32_t bin_count[kBins];
   const uint32_t row = blockIdx.y, chunk = blockIdx.x;
   const RowRule rule = row_rule(a, row);
   const RowWork w = row_work(p, row);
-  const uint32_t top = (uint32_t)(row_top<kWaves>(w, p.chunks, s) >> 32);
+  uint64_t first = 0;
+  for (uint32_t i = threadIdx.x; i < p.chunks; i += kThreads) {
+    first = w.chunk_top[i] > first ? w.chunk_top[i] : first;
+  }
+  for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
+    bin_weight[i] = 0;
+    bin_count[i] = 0;
+  }
+  first = block_reduce<kWaves>(first, Largest{}, s);
+  const uint32_t top = (uint32_t)(first >> 32);
+  if (chunk == 0 && threadIdx.x == 0) {
+    w.meta->top = top;
+    w.meta->top_index = ~(uint32_t)first;
+  }
   if (takes_top(rule, top)) {
     return;
   }
-  const Bounds b = row_bounds<kWaves>(rule, w, bs);
+  const Weights weights = weights_of(top, rule, p.shift);
+  const float scale = (float)(8.0 * weights.factor);
+  const bool counted = rule.top_k != 0u;
+  const uint32_t begin = chunk * p.chunk, end = min(a.size, begin + p.chunk);
+  each_logit(a.logits + (size_t)row * a.row_stride, begin, end, [&](uint32_t, float x) {
+    const uint32_t key = key_of(x);
+    if (key != 0u) {
+      const uint32_t bin = bin_of(key, top, scale);
+      atomicAdd((unsigned long long*)&bin_weight[bin],
+                (unsigned long long)weight_fixed(key, weights));
+      if (counted) {
+        atomicAdd(&bin_count[bin], 1u);
+      }
+    }
+  });
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
+    const uint64_t weight = bin_weight[i];
+    w.chunk_bins[(size_t)chunk * kBins + i] = weight;
+    if (weight != 0u) {
+      atomicAdd((unsigned long long*)&w.bin_weight[i], (unsigned long long)weight);
+    }
+    if (bin_count[i] != 0u) {
+      atomicAdd(&w.bin_count[i], bin_count[i]);
+    }
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, Plan p) {
+  constexpr uint32_t kWaves = kThreads / 64u;
+  __shared__ uint64_t s[kWaves];
+  __shared__ uint32_t wave_counts[kWaves];
+  __shared__ BoundScratch bounds;
+  __shared__ uint32_t found[kMaxChunk], founds;
+  const uint32_t row = blockIdx.y, chunk = blockIdx.x;
+  const RowRule rule = row_rule(a, row);
+  const RowWork w = row_work(p, row);
+  const uint32_t top = w.meta->top;
+  if (takes_top(rule, top)) {
+    return;
+  }
+  const RowMeta b = row_bounds(rule, w, s, wave_counts, bounds);
+  const uint32_t sure = b.sure, last = b.last;
+  if (chunk == 0 && threadIdx.x == 0) {
+    // All but the largest, which is there already.
+    w.meta->above = b.above;
+    w.meta->total = b.total;
+    w.meta->above_n = b.above_n;
+    w.meta->sure = sure;
+    w.meta->last = last;
+    w.meta->cut = b.cut;
+  }
   uint64_t sum = 0;
-  for (uint32_t i = threadIdx.x; i < b.sure; i += kThreads) {
+  for (uint32_t i = threadIdx.x; i < sure; i += kThreads) {
     sum += w.chunk_bins[(size_t)chunk * kBins + i];
   }
-  sum = block_sum<kWaves>(sum, s);
+  if (threadIdx.x == 0) {
+    founds = 0;
+  }
+  sum = block_reduce<kWaves>(sum, Sum{}, s);
   if (threadIdx.x == 0) {
     w.chunk_weight[chunk] = sum;
   }
-  if (b.last < b.sure || b.sure == kBins) {
-    return;  // no list
+  const Weights weights = weights_of(top, rule, p.shift);
+  if (last >= sure) {
+    const float scale = (float)(8.0 * weights.factor);
+    const uint32_t begin = chunk * p.chunk, end = min(a.size, begin + p.chunk);
+    each_logit(a.logits + (size_t)row * a.row_stride, begin, end, [&](uint32_t i, float x) {
+      const uint32_t key = key_of(x);
+      const uint32_t bin = bin_of(key, top, scale);
+      if (key != 0u && bin >= sure && bin <= last) {
+        found[atomicAdd(&founds, 1u)] = i;
+      }
+    });
   }
-  const float scale = (float)(8.0 * 1.4426950408889634 * rule.inverse_temperature);
-  const uint32_t begin = chunk * p.chunk, end = min(a.size, begin + p.chunk);
-  each_logit(a.logits + (size_t)row * a.row_stride, begin, end, [&](uint32_t i, float x) {
-    const uint32_t key = key_of(x);
-    const uint32_t bin = bin_of(key, top, scale);
-    if (key != 0u && bin >= b.sure && bin <= b.last) {
-      w.list[atomicAdd(w.listed, 1u)] = (uint64_t)key << 32 | i;
-    }
-  });
+  __syncthreads();
+  // The order of a list's entries changes nothing that is made of them.
+  const uint32_t n = founds;
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    const uint32_t index = found[i];
+    const uint32_t key = key_of(a.logits[(size_t)row * a.row_stride + index]);
+    w.list[(size_t)chunk * p.chunk + i] = {index, key, weight_fixed(key, weights)};
+  }
+  if (threadIdx.x == 0) {
+    w.chunk_listed[chunk] = n;
+  }
 }
 
 // The kept set within the list: keys above `key`, and those equal to it up to `index`.
@@ -458,87 +551,130 @@ struct Cut {
   }
 };
 
+constexpr uint32_t kDigits = 1024;  // of a step of the radix selection
+
 struct DrawScratch {
+  Entry held[kHeld];
   uint64_t chunk_weight[kMaxChunks];
-  union {
-    struct {
-      uint64_t bins[kDrawThreads];
-      uint32_t counts[kDrawThreads];
-    };
-    BoundScratch bounds;
-  };
-  uint64_t sums[16];
-  uint32_t wave_counts[16];
+  uint64_t bins[kDigits];
+  uint32_t counts[kDigits];
+  uint64_t sums[kDrawThreads / 64u];
+  uint32_t wave_counts[kDrawThreads / 64u];
   uint64_t found_weight;
   uint32_t found, found_count, found_here;
 };
 
-// Radix selection in the list, ten bits of `field` at a time from its highest that
-// differ.  Walking from the largest field down (each with its weight and count), the
-// last value before which less than `target` (by weight, at least the first value) or
-// fewer than `count` (by count) lie.  Returns the value; `before`, `before_n` become
-// what lies before it and `here` the number of entries that have it.
-template <class Field, class Weight>
-__device__ __forceinline__ uint32_t select_value(uint32_t entries, bool by_weight, double target,
-                                                 uint32_t count, Field field, Weight weight,
-                                                 uint64_t& before, uint32_t& before_n,
-                                                 uint32_t& here, DrawScratch& s) {
-  constexpr uint32_t kWaves = kDrawThreads / 64u;
-  // field(i, value) says whether entry i counts.
-  uint32_t low = 0xffffffffu, high = 0, counted = 0;
-  for (uint32_t i = threadIdx.x; i < entries; i += kDrawThreads) {
-    uint32_t v;
-    if (field(i, v)) {
-      low = min(low, v);
-      high = max(high, v);
-      ++counted;
-    }
-  }
-  here = (uint32_t)block_sum<kWaves>(counted, s.sums);
-  high = (uint32_t)block_max<kWaves>(high, s.sums);
-  low = ~(uint32_t)block_max<kWaves>((uint32_t)~low, s.sums);
-  const uint32_t differ = low ^ high;
-  int at = differ != 0u ? 32 - __builtin_clz(differ) : 0;
-  // The bits above `at` are the same in all.
-  uint32_t prefix = at < 32 ? high >> at << at : 0u;
-  while (at > 0) {
-    const int bits = min(at, 10), next = at - bits;
-    __syncthreads();
-    s.bins[threadIdx.x] = 0;
-    s.counts[threadIdx.x] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < entries; i += kDrawThreads) {
-      uint32_t v;
-      if (field(i, v) && (at >= 32 || v >> at == prefix >> at)) {
-        // The largest value first.
-        const uint32_t digit = kDrawThreads - 1u - (v >> next & ((1u << bits) - 1u));
-        atomicAdd(&s.counts[digit], 1u);
-        if (by_weight) {
-          atomicAdd((unsigned long long*)&s.bins[digit], (unsigned long long)weight(i));
+// The entries of the list: in LDS, or (a row whose threshold has more than kHeld logits
+// in its bins) in memory, chunk by chunk.
+struct Entries {
+  const RowWork* work;
+  const Plan* plan;
+  DrawScratch* s;
+  uint32_t count;
+  uint32_t low, high;  // their smallest and largest key
+
+  // f(key, index, weight) for each of this thread's entries.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    if (count <= kHeld) {
+      for (uint32_t i = threadIdx.x; i < count; i += kDrawThreads) {
+        const Entry e = s->held[i];
+        f(e.key, e.index, e.weight);
+      }
+    } else {
+      for (uint32_t c = 0; c < plan->chunks; ++c) {
+        const uint32_t n = work->chunk_listed[c];
+        for (uint32_t i = threadIdx.x; i < n; i += kDrawThreads) {
+          const Entry e = work->list[(size_t)c * plan->chunk + i];
+          f(e.key, e.index, e.weight);
         }
       }
     }
+  }
+};
+
+// Radix selection in the list, ten bits of a field at a time.  field(key, index, value)
+// says whether an entry counts, and its value, low <= value <= high.  Walking from the
+// largest value down, the last one before which less than `target` (by weight; at least
+// the first value) or fewer than `count` lie.  Returns the value; `before`, `before_n`
+// become what lies before it and `here` the number of entries that have it.
+template <bool kByWeight, class Field>
+__device__ __forceinline__ uint32_t select_value(const Entries& e, double target, uint32_t count,
+                                                 uint32_t low, uint32_t high, Field field,
+                                                 uint64_t& before, uint32_t& before_n,
+                                                 uint32_t& here, DrawScratch& s) {
+  constexpr uint32_t kWaves = kDrawThreads / 64u, kPer = kDigits / kDrawThreads;
+  const uint32_t differ = low ^ high;
+  // The bits above `at` are the same in all; one step at least, which counts them.
+  int at = differ != 0u ? 32 - __builtin_clz(differ) : 1;
+  uint32_t prefix = at < 32 ? high >> at << at : 0u;
+  here = 0;
+  while (at > 0) {
+    const int bits = min(at, 10), next = at - bits;
     __syncthreads();
-    uint64_t x = s.bins[threadIdx.x], all;
-    uint32_t n = s.counts[threadIdx.x], all_n;
-    const uint32_t own = n;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+      s.bins[threadIdx.x + i * kDrawThreads] = 0;
+      s.counts[threadIdx.x + i * kDrawThreads] = 0;
+    }
     if (threadIdx.x == 0) {
       s.found = 0;
     }
+    __syncthreads();
+    e.each([&](uint32_t key, uint32_t index, uint64_t weight) {
+      uint32_t v;
+      if (field(key, index, v) && (at >= 32 || v >> at == prefix >> at)) {
+        // The largest value first.
+        const uint32_t digit = kDigits - 1u - (v >> next & ((1u << bits) - 1u));
+        atomicAdd(&s.counts[digit], 1u);
+        if (kByWeight) {
+          atomicAdd((unsigned long long*)&s.bins[digit], (unsigned long long)weight);
+        }
+      }
+    });
+    __syncthreads();
+    uint64_t weights[kPer], x = 0, all;
+    uint32_t counts[kPer], n = 0, all_n;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+      weights[i] = s.bins[threadIdx.x * kPer + i];
+      counts[i] = s.counts[threadIdx.x * kPer + i];
+      x += weights[i];
+      n += counts[i];
+    }
     block_scan<kWaves>(x, n, all, all_n, s.sums, s.wave_counts);
-    const bool reaches = own != 0u && (n == 0u || (by_weight ? (double)(before + x) < target
-                                                             : before_n + n < count));
-    if (reaches) {
-      atomicMax(&s.found, threadIdx.x);
+    uint64_t at_x = x;
+    uint32_t at_n = n, best = 0;
+    bool any = false;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; ++i) {
+      if (counts[i] != 0u && (at_n == 0u || (kByWeight ? (double)(before + at_x) < target
+                                                       : before_n + at_n < count))) {
+        best = threadIdx.x * kPer + i;
+        any = true;
+      }
+      at_x += weights[i];
+      at_n += counts[i];
+    }
+    if (last_that(any)) {
+      atomicMax(&s.found, best);
     }
     __syncthreads();
-    if (s.found == threadIdx.x) {
-      s.found_weight = before + x;
-      s.found_count = before_n + n;
-      s.found_here = own;
+    const uint32_t digit = s.found;
+    if (digit / kPer == threadIdx.x) {
+#pragma unroll
+      for (uint32_t i = 0; i < kPer; ++i) {
+        if (digit % kPer == i) {
+          s.found_weight = before + x;
+          s.found_count = before_n + n;
+          s.found_here = counts[i];
+        }
+        x += weights[i];
+        n += counts[i];
+      }
     }
     __syncthreads();
-    prefix |= (kDrawThreads - 1u - s.found) << next;
+    prefix |= (kDigits - 1u - digit) << next;
     before = s.found_weight;
     before_n = s.found_count;
     here = s.found_here;
@@ -554,60 +690,91 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
   const float* logits = a.logits + (size_t)row * a.row_stride;
   const RowRule rule = row_rule(a, row);
   const RowWork w = row_work(p, row);
-  const uint64_t first = row_top<kWaves>(w, p.chunks, s.sums);
-  const uint32_t top = (uint32_t)(first >> 32), top_index = ~(uint32_t)first;
+  const RowMeta b = *w.meta;
+  const uint32_t top = b.top;
   if (takes_top(rule, top)) {
     if (threadIdx.x == 0) {
-      a.tokens[row] = (int32_t)top_index;
+      a.tokens[row] = (int32_t)b.top_index;
       if (a.probabilities != nullptr) {
         a.probabilities[row] = top > kMinusInfKey ? 1.0f : 0.0f;
       }
     }
     return;
   }
-  const double inverse = rule.inverse_temperature;
-  auto weight = [&](uint32_t key) { return fixed(weight_of(key, top, inverse), p.shift); };
-  const Bounds b = row_bounds<kWaves>(rule, w, s.bounds);
-  const uint32_t entries = b.last < b.sure || b.sure == kBins ? 0u : *w.listed;
+  const Weights weights = weights_of(top, rule, p.shift);
+
+  // The list into LDS: the chunks' places in it, then each entry from its chunk.
+  const uint32_t per = (p.chunks + kDrawThreads - 1u) / kDrawThreads;
+  const uint32_t run = min(p.chunks, threadIdx.x * per), run_end = min(p.chunks, run + per);
+  uint64_t none = 0, none_all;
+  uint32_t n = 0, all_n;
+  for (uint32_t i = run; i < run_end; ++i) {
+    n += w.chunk_listed[i];
+  }
+  block_scan<kWaves>(none, n, none_all, all_n, s.sums, s.wave_counts);
+  Entries e{&w, &p, &s, all_n, 0u, 0u};
+  for (uint32_t i = run; i < run_end; ++i) {
+    s.chunk_weight[i] = n;
+    n += w.chunk_listed[i];
+  }
+  __syncthreads();
+  uint32_t high = 0, low = 0xffffffffu;
+  if (all_n <= kHeld) {
+    for (uint32_t i = threadIdx.x; i < all_n; i += kDrawThreads) {
+      // The last chunk whose place is not behind i.
+      uint32_t c = 0;
+      for (uint32_t step = 1u << (31 - __builtin_clz(p.chunks)); step != 0u; step /= 2u) {
+        c += c + step < p.chunks && s.chunk_weight[c + step] <= i ? step : 0u;
+      }
+      const Entry x = w.list[(size_t)c * p.chunk + (i - (uint32_t)s.chunk_weight[c])];
+      s.held[i] = x;
+      high = max(high, x.key);
+      low = min(low, x.key);
+    }
+  } else {
+    e.each([&](uint32_t key, uint32_t, uint64_t) {
+      high = max(high, key);
+      low = min(low, key);
+    });
+  }
+  e.high = (uint32_t)block_reduce<kWaves>(high, Largest{}, s.sums);
+  e.low = ~(uint32_t)block_reduce<kWaves>((uint32_t)~low, Largest{}, s.sums);
+
   Cut cut{0u, 0xffffffffu};
-  if (b.cut) {
+  if (b.cut != 0u && all_n != 0u) {
     // The threshold's ties: all, or the first few by index.
     auto ties = [&](uint32_t key, uint32_t keep, uint32_t here) {
       cut.key = key;
       cut.index = 0xffffffffu;
       if (keep < here) {
-        // Of the inverted indices the keep-th largest.
+        // Of the indices counted down from the last, the keep-th largest.
         uint64_t before = 0;
         uint32_t before_n = 0, equal;
-        cut.index = ~select_value(
-          entries, false, 0.0, keep,
-          [&](uint32_t i, uint32_t& v) {
-            const uint64_t e = w.list[i];
-            v = ~(uint32_t)e;
-            return (uint32_t)(e >> 32) == key;
+        cut.index = size - 1u - select_value<false>(
+          e, 0.0, keep, 0u, size - 1u,
+          [&](uint32_t k, uint32_t index, uint32_t& v) {
+            v = size - 1u - index;
+            return k == key;
           },
-          [](uint32_t) { return (uint64_t)0; }, before, before_n, equal, s);
+          before, before_n, equal, s);
       }
     };
     uint64_t whole = b.total;
     if (rule.top_k != 0u) {
       uint64_t before = 0;
       uint32_t before_n = b.above_n, here;
-      const uint32_t key = select_value(
-        entries, false, 0.0, rule.top_k,
-        [&](uint32_t i, uint32_t& v) {
-          v = (uint32_t)(w.list[i] >> 32);
+      const uint32_t key = select_value<false>(
+        e, 0.0, rule.top_k, e.low, e.high,
+        [](uint32_t k, uint32_t, uint32_t& v) {
+          v = k;
           return true;
         },
-        [](uint32_t) { return (uint64_t)0; }, before, before_n, here, s);
+        before, before_n, here, s);
       ties(key, rule.top_k - before_n, here);
       if (rule.top_p < 1.0) {
         uint64_t sum = 0;
-        for (uint32_t i = threadIdx.x; i < entries; i += kDrawThreads) {
-          const uint64_t e = w.list[i];
-          sum += cut.keeps((uint32_t)(e >> 32), (uint32_t)e) ? weight((uint32_t)(e >> 32)) : 0u;
-        }
-        whole = b.above + block_sum<kWaves>(sum, s.sums);
+        e.each([&](uint32_t k, uint32_t index, uint64_t x) { sum += cut.keeps(k, index) ? x : 0u; });
+        whole = b.above + block_reduce<kWaves>(sum, Sum{}, s.sums);
       }
     }
     if (rule.top_p < 1.0) {
@@ -615,17 +782,15 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
       const double target = rule.top_p * (double)whole;
       uint64_t before = b.above;
       uint32_t before_n = b.above_n, here;
-      const uint32_t key = select_value(
-        entries, true, target, 0u,
-        [&](uint32_t i, uint32_t& v) {
-          const uint64_t e = w.list[i];
-          v = (uint32_t)(e >> 32);
-          return within.keeps(v, (uint32_t)e);
+      const uint32_t key = select_value<true>(
+        e, target, 0u, e.low, e.high,
+        [&](uint32_t k, uint32_t index, uint32_t& v) {
+          v = k;
+          return within.keeps(k, index);
         },
-        [&](uint32_t i) { return weight((uint32_t)(w.list[i] >> 32)); }, before, before_n, here,
-        s);
+        before, before_n, here, s);
       // The i-th tie is kept where before + i w < target.
-      const uint64_t each = weight(key);
+      const uint64_t each = weight_fixed(key, weights);
       uint32_t keep = here;
       if (each != 0u) {
         const double need = ceil((target - (double)before) / (double)each);
@@ -639,105 +804,99 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     }
   }
 
-  // The kept weight of an element of the list, and of any.
-  auto kept_listed = [&](uint32_t key, uint32_t i) {
-    const double x = weight_of(key, top, inverse);
-    return cut.keeps(key, i) && x >= rule.min_p ? fixed(x, p.shift) : (uint64_t)0;
+  // Each chunk's kept weight.
+  auto above_min = [&](uint32_t key) {
+    return rule.min_p == 0.0 || weight_real(key, weights) >= ldexp(rule.min_p, p.shift);
   };
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < p.chunks; i += kDrawThreads) {
     s.chunk_weight[i] = w.chunk_weight[i];
   }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < entries; i += kDrawThreads) {
-    const uint64_t e = w.list[i];
-    const uint64_t x = kept_listed((uint32_t)(e >> 32), (uint32_t)e);
-    if (x != 0u) {
-      atomicAdd((unsigned long long*)&s.chunk_weight[(uint32_t)e / p.chunk], (unsigned long long)x);
+  e.each([&](uint32_t key, uint32_t i, uint64_t x) {
+    if (x != 0u && cut.keeps(key, i) && above_min(key)) {
+      atomicAdd((unsigned long long*)&s.chunk_weight[i / p.chunk], (unsigned long long)x);
     }
+  });
+  // One running sum passes the target first; where none does (a uniform of 1), the last
+  // kept token is drawn.
+  if (threadIdx.x == 0) {
+    s.found = 0xffffffffu;
+    s.found_here = 0;
   }
   __syncthreads();
-  // The chunk: a run of chunks a thread.
-  const uint32_t per = (p.chunks + kDrawThreads - 1u) / kDrawThreads;
   uint64_t x = 0, total;
-  uint32_t n = 0, all_n;
-  for (uint32_t i = threadIdx.x * per; i < min(p.chunks, (threadIdx.x + 1u) * per); ++i) {
+  n = 0;
+  for (uint32_t i = run; i < run_end; ++i) {
     x += s.chunk_weight[i];
   }
   block_scan<kWaves>(x, n, total, all_n, s.sums, s.wave_counts);
-  const uint64_t row_total = total;
   const double target = rule.uniform * (double)total;
-  // Where no running sum passes the target (a uniform of 1), the last kept token.
-  if (threadIdx.x == 0) {
-    s.found = 0xffffffffu;
-    s.found_here = 0;
-  }
-  __syncthreads();
   uint64_t at = x;
-  for (uint32_t i = threadIdx.x * per; i < min(p.chunks, (threadIdx.x + 1u) * per); ++i) {
+  for (uint32_t i = run; i < run_end; ++i) {
     const uint64_t here = s.chunk_weight[i];
-    at += here;
-    if (here != 0u) {
-      if ((double)at > target) {
-        atomicMin(&s.found, i);
-      }
-      atomicMax(&s.found_here, i);
+    if ((double)at <= target && (double)(at + here) > target) {
+      s.found = i;
     }
+    if (here != 0u && at + here == total) {
+      s.found_here = i;
+    }
+    at += here;
   }
   __syncthreads();
   const uint32_t chunk = s.found != 0xffffffffu ? s.found : s.found_here;
-  if (threadIdx.x == chunk / per) {
-    at = x;
-    for (uint32_t i = threadIdx.x * per; i < chunk; ++i) {
-      at += s.chunk_weight[i];
+  if (run <= chunk && chunk < run_end) {
+    for (uint32_t i = run; i < chunk; ++i) {
+      x += s.chunk_weight[i];
     }
-    s.found_weight = at;
+    s.found_weight = x;
   }
   __syncthreads();
   uint64_t before = s.found_weight;
-  const float scale = (float)(8.0 * 1.4426950408889634 * inverse);
-  const uint32_t begin = chunk * p.chunk, end = min(size, begin + p.chunk);
   if (threadIdx.x == 0) {
     s.found = 0xffffffffu;
     s.found_here = 0;
   }
-  // p.chunk is at most four logits a thread.
-  uint64_t kept[4], sum = 0;
+  // The chunk's logits, kPer a thread.
+  constexpr uint32_t kPer = kMaxChunk / kDrawThreads;
+  const float scale = (float)(8.0 * weights.factor);
+  const uint32_t begin = chunk * p.chunk + kPer * threadIdx.x;
+  const uint32_t end = min(size, (chunk + 1u) * p.chunk);
+  uint64_t kept[kPer], sum = 0, rest;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t i = begin + 4u * threadIdx.x + j;
+  for (uint32_t j = 0; j < kPer; ++j) {
     kept[j] = 0;
+    const uint32_t i = begin + j;
     if (i < end) {
       const uint32_t key = key_of(logits[i]);
       const uint32_t bin = bin_of(key, top, scale);
-      if (key != 0u && bin < b.sure) {
-        kept[j] = weight(key);
-      } else if (key != 0u && entries != 0u && bin <= b.last) {
-        kept[j] = kept_listed(key, i);
+      if (key != 0u && (bin < b.sure || (bin <= b.last && cut.keeps(key, i) && above_min(key)))) {
+        kept[j] = weight_fixed(key, weights);
       }
     }
     sum += kept[j];
   }
-  block_scan<kWaves>(sum, n, total, all_n, s.sums, s.wave_counts);
+  n = 0;
+  block_scan<kWaves>(sum, n, rest, all_n, s.sums, s.wave_counts);
+  const uint64_t chunk_end = before + rest;
   before += sum;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    before += kept[j];
-    if (kept[j] != 0u) {
-      const uint32_t i = begin + 4u * threadIdx.x + j;
-      if ((double)before > target) {
-        atomicMin(&s.found, i);
-      }
-      atomicMax(&s.found_here, i);
+  for (uint32_t j = 0; j < kPer; ++j) {
+    if ((double)before <= target && (double)(before + kept[j]) > target) {
+      s.found = begin + j;
     }
+    if (kept[j] != 0u && before + kept[j] == chunk_end) {
+      s.found_here = begin + j;
+    }
+    before += kept[j];
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     const uint32_t token = s.found != 0xffffffffu ? s.found : s.found_here;
     a.tokens[row] = (int32_t)token;
     if (a.probabilities != nullptr) {
-      const double x = weight_of(key_of(logits[token]), top, inverse);
-      a.probabilities[row] = (float)(ldexp(x, p.shift) / (double)row_total);
+      a.probabilities[row] =
+        (float)(weight_real(key_of(logits[token]), weights) / (double)total);
     }
   }
 }
@@ -745,7 +904,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
 Plan plan_of(const SampleArgs& a) {
   Plan p{};
   // 1024 logits a workgroup while that gives few of them (a single row is a matter of
-  // latency), else 4096, the most that the draw scans.
+  // latency), else 4096, the most that the draw scans at once.
   const uint64_t small = ((uint64_t)a.size + 1023u) / 1024u;
   p.chunk = small * a.rows <= 2048u && small <= kMaxChunks ? 1024u : 4096u;
   p.chunks = (a.size + p.chunk - 1u) / p.chunk;
@@ -753,7 +912,8 @@ Plan plan_of(const SampleArgs& a) {
   for (uint64_t n = a.size; n > 1u; n = (n + 1u) / 2u) {
     --p.shift;
   }
-  p.row_words = words_per_row(p.chunks, a.size);
+  p.shift = std::min(p.shift, 51);
+  p.row_words = words_per_row(p);
   return p;
 }
 

@@ -195,11 +195,11 @@ def test_sample_refusals(vctx):
         args[at] = value
         assert vctx.status("sample_f32_i32", *args) == kh.INVALID_ARGUMENT
         assert fragment in kh.last_error(), kh.last_error()
-    for rows, size in ((1, (1 << 24) + 1), (65536, 5)):
+    for rows, size in ((1, (1 << 22) + 1), (65536, 5)):
         args = list(base)
         args[0], args[1], args[2], args[3] = fake(1 << 40), rows, size, size
         assert vctx.status("sample_f32_i32", *args) == kh.INVALID_ARGUMENT
-        assert "rows of up to 16777216 logits" in kh.last_error()
+        assert "rows of up to 4194304 logits" in kh.last_error()
 
 
 # ------------------------------------------------------- the plain forms ----
