@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
       largest = fmaxf(largest, w[i]);
     }
     largest = xor32_max(xor16_max(largest));
-    if (__any(largest > top)) {
+    if (__any(largest > top + kMaxLead)) {
       const float up = fmaxf(top, largest);
       const float keep = fast_exp2(top - up);
       top = up;
@@ -441,8 +441,8 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   s.decode_keys = (uint32_t)keys;
   s.decode_rows = (uint32_t)std::min<uint64_t>(rows, kDecodeRows);
   s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
-  // The tiled kernel's keys in parts until there are two workgroups a CU, each of 512
-  // keys at least, and while their results take no more than 256 MiB.
+  // The tiled kernel's keys in parts until there are as many workgroups as the CUs hold
+  // (one of head_dim 256, two of less), each of 128 keys at least, and while their results take no more than 256 MiB.
   const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows * a.cache.kv_heads;
   const uint64_t all_tiles =
     std::min<uint64_t>(tiles * a.batch.sequences,
@@ -452,8 +452,8 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   const uint64_t row_bytes =
     (uint64_t)a.batch.tokens * a.heads * (a.cache.head_dim + 2u) * sizeof(float);
   uint64_t splits = 1;
-  while (rows > kDecodeRows && all_tiles * splits < 2u * (uint64_t)cu_count &&
-         a.batch.max_keys / (2u * splits) >= 512u &&
+  while (rows > kDecodeRows && all_tiles * splits < (a.cache.head_dim == 256u ? 1u : 2u) * (uint64_t)cu_count &&
+         a.batch.max_keys / (2u * splits) >= 128u &&
          2u * splits * row_bytes <= (uint64_t{256} << 20)) {
     splits *= 2u;
   }

@@ -7,8 +7,11 @@
 // sv = mu 2^b (b its exponent) into the weight.  With a = score in log2 units, the
 // running maximum M is kept of a + b, not of a, so that the weight that multiplies the
 // codes, 2^(a + b - M) mu, is at most 1 however far apart the scales of neighbouring
-// pages lie; the softmax's sum adds 2^(a + b - M) 2^-b, an exact shift.  Weights go into
-// f16 times 2^15, so that what falls below f16's normal range is 2^-29 of the largest.
+// pages lie; the softmax's sum adds 2^(a + b - M) 2^-b, an exact shift.  M follows the
+// largest score only when that leads it by more than four octaves, which after the first
+// keys it hardly does: the sums in registers (64 to 128 of them a lane) are seldom
+// rescaled.  Weights, up to 2^4 then, go into f16 times 2^11: below f16's smallest normal
+// value lies what is 2^-25 of the largest, and below its last place 2^-35.
 // A query row is multiplied by the power of two that takes its largest value to
 // [2^13, 2^14) and goes in as two f16 parts (hi, and what hi leaves), which holds 22
 // bits of each value down to 2^-16 of the row's largest; the weights likewise.  f16
@@ -28,12 +31,13 @@ namespace kraken {
 // Below every score that counts; a running maximum starts here, so that a masked
 // score's -inf gives a weight of 0 and not NaN.
 constexpr float kLowestMax = -1e30f;
-constexpr int kWeightShift = 15;
+constexpr int kWeightShift = 11;
+constexpr float kMaxLead = 4.0f;
 
 // Sequences of at most this many rows (new tokens x query heads per KV head) take the
 // split decode kernel, longer ones the tiled one.
 constexpr uint32_t kDecodeRows = 16;
-// Rows of the tiled kernel's workgroups.
+// Rows of the tiled kernel's workgroups: 32 a wave.
 constexpr uint32_t kTileRows = 128;
 
 // How a call's keys are split, and where the partial results lie: f32 sums [D] and

@@ -2,10 +2,10 @@
 // rows (chunks of prompts).  The arithmetic is described in
 // attention_paged_q8_common.hpp.
 //
-// A workgroup takes 128 rows (token x query head) of one KV head of one sequence, 32 a
-// wave, and a run of its keys, a tile of kKeys at a time.  The next tile's codes are on
+// A workgroup takes 128 or 256 rows (token x query head) of one KV head of one sequence,
+// 32 a wave, and a run of its keys, a tile of kKeys at a time.  The next tile's codes are on
 // their way into registers while a tile is multiplied; they become f16 as they go into
-// LDS, once for the four waves.  Both products are transposed, S^T = K Q^T and
+// LDS, once for all waves.  Both products are transposed, S^T = K Q^T and
 // O^T += V^T P^T (32x32x16), so that a query row is a lane: its maximum and sum are
 // lane values that two lanes share.  The key rows of a product are read in an order that
 // gives a lane the scores of whole runs of eight keys, which is the operand that P has to
@@ -13,27 +13,44 @@
 // f16 parts: a second product with the same operand from LDS.
 #include <hip/hip_runtime.h>
 
+#include <utility>
+
 #include "attention_paged_q8_common.hpp"
 #include "device_common.hpp"
 
 namespace kraken {
 namespace {
 
-constexpr uint32_t kThreads = 256;
+constexpr int kThreads = 256;
 
-template <int D, class T, int kKeys, int kWavesPerSimd>
+// f(0), f(1), .. f(N - 1) with compile-time indices.
+template <class F, int... I>
+__device__ __forceinline__ void static_for(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+template <int N, class F>
+__device__ __forceinline__ void static_for(F f) {
+  static_for(f, std::make_integer_sequence<int, N>{});
+}
+
+// KEYS = 32 kSub keys a tile, 4 waves.
+template <int D, class T, int kSub, int kWavesPerSimd>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_kernel(
   PagedAttentionArgs a, PagedSplit split) {
   constexpr bool kTwo = std::is_same<T, float>::value;
-  constexpr int kStride = D + 8;                   // of a key row in LDS, in halves
-  constexpr int kGranules = kKeys / 16;            // runs of 16 keys: of one page each
-  constexpr int kChunks = kKeys * D / 16 / 256;    // 16-byte chunks of K, and of V, a thread
-  constexpr int kSub = kKeys / 32;                 // 32-key products a tile
-  constexpr int kBuffer = kKeys * kStride + kKeys * D;
+  constexpr int kKeys = 32 * kSub;
+  constexpr int kStride = D + 8;                      // of a key row in LDS, in halves
+  constexpr int kGranules = kKeys / 16;               // runs of 16 keys: of one page each
+  constexpr int kChunks = kKeys * D / 16 / kThreads;  // 16-byte chunks of K, and of V, a thread
+  constexpr int kSteps = D / 16;                      // of a score product
+  constexpr int kDims = D / 32;                       // tiles of the output
+  constexpr int kTileK = kKeys * kStride, kTileV = kKeys * D;
   static_assert(kChunks >= 1, "a tile has a chunk for every thread");
-  __shared__ __attribute__((aligned(16))) half_t lds[2 * kBuffer];
+  __shared__ __attribute__((aligned(16))) half_t lds[2 * (kTileK + kTileV)];
 
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t n = lane & 31u, h = lane >> 5;
   const uint32_t part = blockIdx.x % split.tile_splits, tile = blockIdx.x / split.tile_splits;
   const uint32_t kv_head = blockIdx.y, sequence = blockIdx.z;
@@ -64,47 +81,69 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   const uint32_t visible = real ? before + token + 1u : 0u;
   const size_t at = ((size_t)(s.start + token) * a.heads + kv_head * group +
                      (real ? row % group : 0u)) * D;
-  // What every row of the wave sees, and what any does.
-  const uint32_t open = before + wave_row / group + 1u;
-  const uint32_t reach =
-    wave_row < rows ? before + (min(wave_row + 32u, rows) - 1u) / group + 1u : 0u;
+  // What every row of the wave sees (0: a row without a query sees nothing).
+  const uint32_t open = wave_row + 32u <= rows ? before + wave_row / group + 1u : 0u;
 
-  // Lane l holds the page of granule l % kGranules of a tile.
+  // Lane l holds the page of granule l % kGranules of a tile; past the last tile, the
+  // last one's again.
   auto pages_of = [&](uint32_t t) {
-    const uint32_t key = begin + t * kKeys + 16u * (lane % kGranules);
+    const uint32_t key = begin + min(t, tiles - 1u) * kKeys + 16u * (lane % kGranules);
     return table[min(key >> shift, last_page)];
   };
+  auto held_page = [&](int32_t page) {
+    return page >= 0 && (uint32_t)page < a.cache.pages ? (uint32_t)page : 0u;
+  };
   u32x4_t k[kChunks], v[kChunks];
-  float key_scale = 0.0f, val_scale = 0.0f;
-  bool inside = false;
-  auto load = [&](uint32_t t, int32_t pages) {
-    inside = pages >= 0 && (uint32_t)pages < a.cache.pages;
-    const uint32_t held = inside ? (uint32_t)pages : 0u;
-    const size_t scale_at = (size_t)held * kv_heads + kv_head;
-    key_scale = a.cache.key_scales[scale_at];
-    val_scale = a.cache.value_scales[scale_at];
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const uint32_t c = tid + 256u * i;
-      const uint32_t granule = (uint32_t)__builtin_amdgcn_readfirstlane((int)(c / D));
-      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)held, (int)granule);
-      const uint32_t key = begin + t * kKeys + 16u * granule;
-      const size_t from =
-        ((((size_t)page * kv_heads + kv_head) << shift) + (key & ((1u << shift) - 1u))) * D;
-      k[i] = *reinterpret_cast<const u32x4_t*>(a.cache.keys + from + (c % D) * 16u);
-      v[i] = *reinterpret_cast<const u32x4_t*>(a.cache.values + from + (c % D) * 16u);
-    }
+  // Where chunk i of tile t lies.
+  auto place = [&](uint32_t t, int32_t pages, int i) {
+    const uint32_t c = tid + kThreads * i;
+    const uint32_t granule = (uint32_t)__builtin_amdgcn_readfirstlane((int)(c / D));
+    const uint32_t page =
+      (uint32_t)__builtin_amdgcn_readlane((int)held_page(pages), (int)granule);
+    const uint32_t key = begin + min(t, tiles - 1u) * kKeys + 16u * granule;
+    return ((((size_t)page * kv_heads + kv_head) << shift) + (key & ((1u << shift) - 1u))) * D;
+  };
+  auto load_k = [&](uint32_t t, int32_t pages, int i) {
+    k[i] = *reinterpret_cast<const u32x4_t*>(a.cache.keys + place(t, pages, i) +
+                                             (tid + kThreads * i) % D * 16u);
+  };
+  auto load_v = [&](uint32_t t, int32_t pages, int i) {
+    v[i] = *reinterpret_cast<const u32x4_t*>(a.cache.values + place(t, pages, i) +
+                                             (tid + kThreads * i) % D * 16u);
+  };
+  // A tile's scales, a granule a lane; outside the pool NaN stands for none.
+  struct Scales {
+    float key, value;
+    bool inside;
+  };
+  auto scales_of = [&](int32_t page) {
+    const size_t i = (size_t)held_page(page) * kv_heads + kv_head;
+    return Scales{a.cache.key_scales[i], a.cache.value_scales[i],
+                  page >= 0 && (uint32_t)page < a.cache.pages};
+  };
+  // Half of a chunk as f16 into LDS.
+  auto convert = [&](const u32x4_t& x, half_t* to, int half) {
+    *reinterpret_cast<half8_t*>(to + 8 * half) = codes_to_f16(x[2 * half], x[2 * half + 1]);
+  };
+  half_t* const lds_k = lds;
+  half_t* const lds_v = lds + 2 * kTileK;
+  auto store_k = [&](uint32_t t, int i, int half) {
+    const uint32_t c = tid + kThreads * i;
+    convert(k[i], lds_k + (t & 1u) * kTileK + c / kSteps * kStride + c % kSteps * 16, half);
+  };
+  auto store_v = [&](uint32_t t, int i, int half) {
+    convert(v[i], lds_v + (t & 1u) * kTileV + (tid + kThreads * i) * 16u, half);
   };
 
-  int32_t pages = pages_of(0);
+  int32_t pages_0 = pages_of(0), pages_1 = pages_of(1), pages_2 = pages_of(2);
   // The query rows as operands: dimensions 16 c + 8 h .. + 7 of row n.
-  half8_t q_hi[D / 16], q_lo[kTwo ? D / 16 : 1];
+  half8_t q_hi[kSteps], q_lo[kTwo ? kSteps : 1];
   float row_factor;
   {
     const T* p = static_cast<const T*>(a.query) + at + 8u * h;
     float largest = 0.0f;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
+    for (int c = 0; c < kSteps; ++c) {
       float x[8];
       load4(p + 16 * c, x);
       load4(p + 16 * c + 4, x + 4);
@@ -118,7 +157,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
     row_factor = ldexpf(kLog2e / (D == 64 ? 8.0f : D == 256 ? 16.0f : 11.313708498984761f), -e);
     // Read again (from the caches) rather than held: the operands take their registers.
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
+    for (int c = 0; c < kSteps; ++c) {
       float x[8];
       load4(p + 16 * c, x);
       load4(p + 16 * c + 4, x + 4);
@@ -136,151 +175,265 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
       if constexpr (kTwo) {
         q_lo[c] = lo;
       }
+      if constexpr (D == 256) {
+        // Into accumulator registers, where the products read them: the others are for
+        // what the vector units work on.
+        asm volatile("" : "+a"(q_hi[c]));
+        if constexpr (kTwo) {
+          asm volatile("" : "+a"(q_lo[c]));
+        }
+      }
     }
   }
-  load(0, pages);
-  pages = pages_of(min(1u, tiles - 1u));
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    load_k(0, pages_0, i);
+    load_v(0, pages_0, i);
+  }
+  Scales scales = scales_of(pages_0), next_scales = scales_of(pages_1);
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    store_k(0, i, 0);
+    store_k(0, i, 1);
+    load_k(1, pages_1, i);
+  }
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    store_v(0, i, 0);
+    store_v(0, i, 1);
+    load_v(1, pages_1, i);
+  }
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    store_k(1, i, 0);
+    store_k(1, i, 1);
+    load_k(2, pages_2, i);
+  }
+  // From here on: pages_1 of the tile whose values are loaded next, pages_2 of its keys'.
+  pages_1 = pages_2;
+  pages_2 = pages_of(3);
 
-  float16_t o[D / 32];
+  float16_t o[kDims];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      o[i][j] = 0.0f;
-    }
+  for (int i = 0; i < kDims; ++i) {
+    o[i] = float16_t{};
   }
   float top = kLowestMax, sum = 0.0f;
   // Row r of a product is key swap(r): bits 2 and 3 change places.
   const uint32_t key_row = (n & 19u) | (n & 4u) << 1 | (n & 8u) >> 1;
 
+  // Fragment i of a tile's keys: step i / kSub, 32-key half i % kSub.
+  constexpr int kKeyFrags = kSteps * kSub, kValueFrags = 2 * kSub * kDims, kRing = 4;
+  auto key_frag = [&](uint32_t t, int i) {
+    return *reinterpret_cast<const half8_t*>(lds_k + (t & 1u) * kTileK +
+                                             (32u * (i % kSub) + key_row) * kStride + 8u * h +
+                                             16 * (i / kSub));
+  };
+  // Fragment i of a tile's values: 16-key step i / kDims, dimensions 32 (i % kDims) on.
+  auto value_frag = [&](uint32_t t, int i) {
+    return *reinterpret_cast<const half8_t*>(lds_v + (t & 1u) * kTileV +
+                                             ((2u * (i / kDims) + h) * D + n) * 8u +
+                                             256 * (i % kDims));
+  };
+  auto score_product = [&](float16_t (&score)[kSub], const half8_t& x, int i) {
+    score[i % kSub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+      x, q_hi[i / kSub], i < kSub ? float16_t{} : score[i % kSub], 0, 0, 0);
+    if constexpr (kTwo) {
+      score[i % kSub] =
+        __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_lo[i / kSub], score[i % kSub], 0, 0, 0);
+    }
+  };
+
+  __syncthreads();
+  float16_t score[kSub];
+  {
+    half8_t ring[kRing];
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) {
+      ring[i] = key_frag(0, i);
+    }
+    static_for<kKeyFrags>([&](auto slot) {
+      constexpr int i = decltype(slot)::value;
+      score_product(score, ring[i % kRing], i);
+      if constexpr (i + kRing < kKeyFrags) {
+        ring[i % kRing] = key_frag(0, i + kRing);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+
+  auto of = [&](float x, int granule) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), granule));
+  };
+  // Step t.  The scores of tile t are there.  The matrix cores do the scores of tile
+  // t + 1 while the vector units turn those of t into weights, then O += V^T P^T of tile
+  // t while the codes that arrived (keys of t + 2, values of t + 1) become f16 in LDS and
+  // those of the tiles after set out.  One barrier a step: what it publishes was written
+  // in the step before, to buffers last read before the barrier before.
   for (uint32_t t = 0; t < tiles; ++t) {
-    half_t* lds_k = lds + (t & 1u) * kBuffer;
-    half_t* lds_v = lds_k + kKeys * kStride;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const uint32_t c = tid + 256u * i;
-      half8_t* to = reinterpret_cast<half8_t*>(lds_k + c / (D / 16) * kStride + c % (D / 16) * 16);
-      to[0] = codes_to_f16(k[i][0], k[i][1]);
-      to[1] = codes_to_f16(k[i][2], k[i][3]);
-      to = reinterpret_cast<half8_t*>(lds_v + c * 16u);
-      to[0] = codes_to_f16(v[i][0], v[i][1]);
-      to[1] = codes_to_f16(v[i][2], v[i][3]);
-    }
-    // The tile's scales; its granules' are lane values, read where they are needed.
-    const ValueScale sv = value_scale(val_scale);
-    const float tile_key_scale = inside ? key_scale : 0.0f;
-    const float tile_exponent = inside ? sv.exponent : -INFINITY;
-    const float tile_mantissa = inside ? sv.mantissa : 0.0f;
-    const float tile_shift = sv.shift;
-    // One barrier a tile: a wave that writes this buffer has passed the barrier that
-    // every wave reached after it read the same buffer two tiles ago.
     __syncthreads();
-    if (t + 1u < tiles) {
-      load(t + 1u, pages);
-      pages = pages_of(min(t + 2u, tiles - 1u));
-    }
     const uint32_t first_key = begin + t * kKeys;
-    if (first_key >= reach) {
-      continue;  // no row of the wave sees the tile
-    }
-    float16_t score[kSub];
-#pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        score[u][j] = 0.0f;
-      }
-      const half_t* p = lds_k + (32u * u + key_row) * kStride + 8u * h;
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        const half8_t x = *reinterpret_cast<const half8_t*>(p + 16 * c);
-        score[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_hi[c], score[u], 0, 0, 0);
-        if constexpr (kTwo) {
-          score[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_lo[c], score[u], 0, 0, 0);
-        }
-      }
-    }
-    auto of = [&](float x, int granule) {
-      return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), granule));
-    };
-    float largest = kLowestMax;
     const bool masked = first_key + kKeys > open;  // uniform
+    const bool more = t + 1u < tiles;              // uniform
+    half8_t ring[kRing];
+    float16_t next[kSub];
+    if (more) {
 #pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float factor = row_factor * of(tile_key_scale, 2 * u + b);
-        const float offset = of(tile_exponent, 2 * u + b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          score[u][8 * b + i] = fmaf(score[u][8 * b + i], factor, offset);
-        }
-        if (masked) {
-          const uint32_t key = first_key + 32u * u + 16u * b + 8u * h;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            score[u][8 * b + i] = key + i < visible ? score[u][8 * b + i] : -INFINITY;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          largest = fmaxf(largest, score[u][8 * b + i]);
-        }
+      for (int i = 0; i < kRing; ++i) {
+        ring[i] = key_frag(t + 1u, i);
       }
     }
-    largest = xor32_max(largest);
-    if (__any(largest > top)) {
-      const float up = fmaxf(top, largest);
-      const float keep = fast_exp2(top - up);
-      top = up;
-      sum *= keep;
+    // The tile's scales by granule: of the scores, and of the weights.
+    const ValueScale sv = value_scale(scales.value);
+    const float lane_key = scales.inside ? scales.key : 0.0f;
+    const float lane_exponent = scales.inside ? sv.exponent : -INFINITY;
+    const float lane_mantissa = scales.inside ? sv.mantissa : 0.0f;
+    float factor[2 * kSub], mantissa[2 * kSub];
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
+    for (int b = 0; b < 2 * kSub; ++b) {
+      // Not zero: a masked score's -inf has to stay one (a NaN stays NaN).
+      const float f = row_factor * of(lane_key, b);
+      factor[b] = f < 1e-37f ? 1e-37f : f;
+      mantissa[b] = of(lane_mantissa, b);
+    }
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < 2 * kSub; ++b) {
+        const uint32_t key = first_key + 16u * b + 8u * h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          score[b / 2][8 * (b % 2) + i] =
+            key + i < visible ? score[b / 2][8 * (b % 2) + i] : -INFINITY;
+        }
+        // A page that the row does not see at all may have NaN scales.
+        factor[b] = key < visible ? factor[b] : 1.0f;
+        mantissa[b] = key < visible ? mantissa[b] : 0.0f;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    float base[2 * kSub], all[2 * kSub], largest = kLowestMax, keep = 1.0f;
+    bool lead = false;
+    half8_t p_hi[2 * kSub], p_lo[kTwo ? 2 * kSub : 1];
+    // The softmax in pieces, placed after the products of the scores: the largest of
+    // each granule (a = score * factor + exponent), their join, and the weights by
+    // pairs.  Each ends in an empty asm on its results, without which it would sink to
+    // their first use.
+    constexpr int kPieces = 2 * kSub + 1 + 8 * kSub;
+    auto soft_piece = [&](auto piece) {
+      constexpr int kPiece = decltype(piece)::value;
+      if constexpr (kPiece < 2 * kSub) {
+        constexpr int b = kPiece, r = 8 * (b % 2);
+        const float16_t& x = score[b / 2];
+        float run = fmaxf(fmaxf(x[r], x[r + 1]), x[r + 2]);
+        run = fmaxf(fmaxf(run, x[r + 3]), x[r + 4]);
+        run = fmaxf(fmaxf(run, x[r + 5]), x[r + 6]);
+        largest = fmaxf(largest, fmaf(fmaxf(run, x[r + 7]), factor[b], of(lane_exponent, b)));
+        asm volatile("" : "+v"(largest));
+      } else if constexpr (kPiece == 2 * kSub) {
+        largest = xor32_max(largest);
+        lead = largest > top + kMaxLead;
+        const float up = lead ? largest : top;
+        keep = fast_exp2(top - up);
+        top = up;
+        sum *= keep;
+#pragma unroll
+        for (int b = 0; b < 2 * kSub; ++b) {
+          base[b] = of(lane_exponent, b) - top;
+        }
+        asm volatile("" : "+v"(top), "+v"(keep), "+v"(sum));
+      } else {
+        constexpr int b = (kPiece - 2 * kSub - 1) / 4, j = (kPiece - 2 * kSub - 1) % 4;
+        constexpr int r = 8 * (b % 2) + 2 * j;
+        const float x = fast_exp2(fmaf(score[b / 2][r], factor[b], base[b]));
+        const float y = fast_exp2(fmaf(score[b / 2][r + 1], factor[b], base[b]));
+        all[b] = j == 0 ? x + y : all[b] + (x + y);
+        if constexpr (j == 3) {
+          sum = fmaf(all[b], of(sv.shift, b), sum);
+          asm volatile("" : "+v"(sum));
+        }
+        half2_t hi, lo;
+        if constexpr (kTwo) {
+          split_pair(x * mantissa[b], y * mantissa[b], hi, lo);
+          asm volatile("" : "+v"(hi), "+v"(lo));
+          p_lo[b][2 * j] = lo[0];
+          p_lo[b][2 * j + 1] = lo[1];
+        } else {
+          hi = half2_t{(half_t)(x * mantissa[b]), (half_t)(y * mantissa[b])};
+          asm volatile("" : "+v"(hi));
+        }
+        p_hi[b][2 * j] = hi[0];
+        p_hi[b][2 * j + 1] = hi[1];
+      }
+    };
+    // Pieces [slot kPieces / slots, (slot + 1) kPieces / slots) after slot `slot`.
+    if (more) {
+      static_for<kKeyFrags>([&](auto slot) {
+        constexpr int i = decltype(slot)::value;
+        constexpr int kFrom = i * kPieces / kKeyFrags, kTo = (i + 1) * kPieces / kKeyFrags;
+        score_product(next, ring[i % kRing], i);
+        if constexpr (i + kRing < kKeyFrags) {
+          ring[i % kRing] = key_frag(t + 1u, i + kRing);
+        }
+        static_for<kTo - kFrom>([&](auto j) {
+          soft_piece(std::integral_constant<int, kFrom + decltype(j)::value>{});
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    } else {
+      static_for<kPieces>(soft_piece);
+    }
+
+    // O += V^T P^T, and the codes' pieces: halves of K's and V's chunks in turn.
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) {
+      ring[i] = value_frag(t, i);
+    }
+    if (__any(lead)) {
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) {
         o[i] *= keep;
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int kCodePieces = 4 * kChunks;
+    // (Past the last tiles they fill buffers that nothing reads.)
+    static_for<kValueFrags>([&](auto slot) {
+      constexpr int i = decltype(slot)::value;
+      constexpr int kFrom = i * kCodePieces / kValueFrags;
+      constexpr int kTo = (i + 1) * kCodePieces / kValueFrags;
+      o[i % kDims] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], p_hi[i / kDims],
+                                                            o[i % kDims], 0, 0, 0);
+      if constexpr (kTwo) {
+        o[i % kDims] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], p_lo[i / kDims],
+                                                              o[i % kDims], 0, 0, 0);
+      }
+      if constexpr (i + kRing < kValueFrags) {
+        ring[i % kRing] = value_frag(t, i + kRing);
+      }
+      static_for<kTo - kFrom>([&](auto piece) {
+        constexpr int j = kFrom + decltype(piece)::value, chunk = j / 4, half = j % 2;
+        if constexpr (j % 4 < 2) {
+          store_k(t, chunk, half);  // of tile t + 2
+          if constexpr (half == 1) {
+            load_k(t + 3u, pages_2, chunk);
+          }
+        } else {
+          store_v(t + 1u, chunk, half);
+          if constexpr (half == 1) {
+            load_v(t + 2u, pages_1, chunk);
+          }
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    scales = next_scales;
+    next_scales = scales_of(pages_1);
+    pages_1 = pages_2;
+    pages_2 = pages_of(t + 4u);
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        // A page that the row does not see at all may have a NaN scale.
-        const uint32_t key = first_key + 32u * u + 16u * b + 8u * h;
-        float mantissa = of(tile_mantissa, 2 * u + b);
-        if (masked) {
-          mantissa = key < visible ? mantissa : 0.0f;
-        }
-        float w[8], all = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          w[i] = fast_exp2(score[u][8 * b + i] - top);
-          all += w[i];
-        }
-        sum = fmaf(all, of(tile_shift, 2 * u + b), sum);
-        half8_t p_hi, p_lo;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          half2_t x, y;
-          if constexpr (kTwo) {
-            split_pair(w[i] * mantissa, w[i + 1] * mantissa, x, y);
-          } else {
-            x = half2_t{(half_t)(w[i] * mantissa), (half_t)(w[i + 1] * mantissa)};
-            y = x;
-          }
-          p_hi[i] = x[0];
-          p_hi[i + 1] = x[1];
-          p_lo[i] = y[0];
-          p_lo[i + 1] = y[1];
-        }
-        const half_t* p = lds_v + ((4u * u + 2u * b + h) * D + n) * 8u;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const half8_t x = *reinterpret_cast<const half8_t*>(p + 256 * i);
-          o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_hi, o[i], 0, 0, 0);
-          if constexpr (kTwo) {
-            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_lo, o[i], 0, 0, 0);
-          }
-        }
-      }
+      score[u] = next[u];
     }
   }
 
@@ -317,12 +470,14 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
 
 template <int D, class T>
 void launch_tiles(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
+  // One wave a SIMD where the operands take its 512 registers: two waves' 256 would
+  // spill.
+  constexpr int kWavesPerSimd =
+    D == 256 || (D == 128 && std::is_same<T, float>::value) ? 1 : 2;
   const uint64_t rows = (uint64_t)a.batch.max_query * (a.heads / a.cache.kv_heads);
   const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows;
   const dim3 grid((uint32_t)(tiles * split.tile_splits), a.cache.kv_heads, a.batch.sequences);
-  constexpr int kKeys = D == 64 ? 64 : 32;
-  constexpr int kWavesPerSimd = D == 256 && std::is_same<T, float>::value ? 1 : 2;
-  attention_paged_tile_kernel<D, T, kKeys, kWavesPerSimd><<<grid, kThreads, 0, stream>>>(a, split);
+  attention_paged_tile_kernel<D, T, 2, kWavesPerSimd><<<grid, kThreads, 0, stream>>>(a, split);
 }
 
 template <class T>
