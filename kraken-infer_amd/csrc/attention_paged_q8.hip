@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
     const ValueScale sv = value_scale(val_scale);
     const float factor = inside ? row_factor * key_scale : 0.0f;
     const float offset = inside ? sv.exponent : -INFINITY;
-    float mantissa = inside ? sv.mantissa : 0.0f;
+    float inverse = inside ? sv.inverse : 0.0f;
     const uint32_t key = first_key(step) + 8u * g;
     if (next < steps) {
       load_k(next, page_k);
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
         w[i] = key + i < visible ? w[i] : -INFINITY;
       }
       // Of a page that the row does not see at all, the scale may be NaN.
-      mantissa = key < visible ? mantissa : 0.0f;
+      inverse = key < visible ? inverse : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -234,19 +234,19 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
     float all = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      w[i] = fast_exp2(w[i] - top);
+      w[i] = fast_exp2(w[i] - (top - kWeightShift));
       all += w[i];
     }
-    sum = fmaf(all, sv.shift, sum);
+    sum = fmaf(all, inverse, sum);
     half8_t p_hi, p_lo;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       half2_t u, l;
       if constexpr (!kStacked && !kTwo) {
-        u = half2_t{(half_t)(w[i] * mantissa), (half_t)(w[i + 1] * mantissa)};
+        u = half2_t{(half_t)w[i], (half_t)w[i + 1]};
         l = u;
       } else {
-        split_pair(w[i] * mantissa, w[i + 1] * mantissa, u, l);
+        split_pair(w[i], w[i + 1], u, l);
       }
       p_hi[i] = u[0];
       p_hi[i + 1] = u[1];

@@ -4,14 +4,14 @@
 // The arithmetic.  A code is an integer of at most 8 bits, exact in f16, so the matrix
 // cores take the codes themselves and the scales go elsewhere: a key page's scale into
 // the score (one multiply that the softmax scale needs anyhow), a value page's scale
-// sv = mu 2^b (b its exponent) into the weight.  With a = score in log2 units, the
-// running maximum M is kept of a + b, not of a, so that the weight that multiplies the
-// codes, 2^(a + b - M) mu, is at most 1 however far apart the scales of neighbouring
-// pages lie; the softmax's sum adds 2^(a + b - M) 2^-b, an exact shift.  M follows the
-// largest score only when that leads it by more than four octaves, which after the first
-// keys it hardly does: the sums in registers (64 to 128 of them a lane) are seldom
-// rescaled.  Weights, up to 2^4 then, go into f16 times 2^11: below f16's smallest normal
-// value lies what is 2^-25 of the largest, and below its last place 2^-35.
+// sv = 2^b into the weight's exponent.  With a = score in log2 units, the running maximum
+// M is kept of a + b, not of a, and the weight that multiplies the codes is 2^(a + b - M),
+// at most 1 however far apart the scales of neighbouring pages lie; the softmax's sum
+// takes its quotient with sv.  M follows the largest score only when that leads it by
+// more than four octaves, which after the first keys it hardly does: the sums in
+// registers (64 to 128 of them a lane) are seldom rescaled.  Weights, up to 2^4 then, are
+// formed times 2^11 for f16: below its smallest normal value lies what is 2^-25 of the
+// largest, and below its last place 2^-35.
 // A query row is multiplied by the power of two that takes its largest value to
 // [2^13, 2^14) and goes in as two f16 parts (hi, and what hi leaves), which holds 22
 // bits of each value down to 2^-16 of the row's largest; the weights likewise.  f16
@@ -31,7 +31,7 @@ namespace kraken {
 // Below every score that counts; a running maximum starts here, so that a masked
 // score's -inf gives a weight of 0 and not NaN.
 constexpr float kLowestMax = -1e30f;
-constexpr int kWeightShift = 11;
+constexpr float kWeightShift = 11.0f;
 constexpr float kMaxLead = 4.0f;
 
 // Sequences of at most this many rows (new tokens x query heads per KV head) take the
@@ -73,17 +73,17 @@ __device__ __forceinline__ half8_t codes_to_f16(uint32_t x, uint32_t y) {
   return half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// A value page's scale as mantissa and exponent for the weights.
+// A value page's scale as what its weights are formed with.
 struct ValueScale {
-  float mantissa;  // times 2^kWeightShift
-  float exponent;  // added to the score
-  float shift;     // 2^-exponent, for the softmax's sum
+  float exponent;  // b
+  float inverse;   // 2^-b, for the softmax's sum
 };
 
+// Not below 2^-100, so that the sum of quotients stays finite; the prologue holds rows
+// that would need less as zeros.  (A NaN stays one.)
 __device__ __forceinline__ ValueScale value_scale(float s) {
-  // Not below 2^-100, so that 2^-b is finite.
-  const int b = max(__builtin_amdgcn_frexp_expf(s), -100);
-  return {ldexpf(s, kWeightShift - b), (float)b, ldexpf(1.0f, -b)};
+  const float held = s < 0x1p-100f ? 0x1p-100f : s;
+  return {log2f(held), 1.0f / held};
 }
 
 // The exponent that takes a row's largest magnitude to [2^13, 2^14).
@@ -128,10 +128,8 @@ __device__ __forceinline__ void store_output(const PagedAttentionArgs& a, size_t
   static_cast<T*>(a.output)[at] = static_cast<T>(x);
 }
 
-// 1 / l in the sums' unit; l = 0: no key, NaN: NaN.
-__device__ __forceinline__ float inverse_sum(float l) {
-  return l == 0.0f ? 0.0f : ldexpf(1.0f / l, -kWeightShift);
-}
+// 1 / l; l = 0: no key, NaN: NaN.
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
 void launch_attention_paged_q8_tiles(const PagedAttentionArgs& a, const PagedSplit& split,
                                      hipStream_t stream);

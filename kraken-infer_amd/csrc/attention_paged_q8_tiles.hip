@@ -127,15 +127,18 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   };
   half_t* const lds_k = lds;
   half_t* const lds_v = lds + 2 * kTileK;
-  auto store_k = [&](uint32_t t, int i, int half) {
+  auto store_k = [&](int parity, int i, int half) {
     const uint32_t c = tid + kThreads * i;
-    convert(k[i], lds_k + (t & 1u) * kTileK + c / kSteps * kStride + c % kSteps * 16, half);
+    convert(k[i], lds_k + parity * kTileK + c / kSteps * kStride + c % kSteps * 16, half);
   };
-  auto store_v = [&](uint32_t t, int i, int half) {
-    convert(v[i], lds_v + (t & 1u) * kTileV + (tid + kThreads * i) * 16u, half);
+  auto store_v = [&](int parity, int i, int half) {
+    convert(v[i], lds_v + parity * kTileV + (tid + kThreads * i) * 16u, half);
   };
 
-  int32_t pages_0 = pages_of(0), pages_1 = pages_of(1), pages_2 = pages_of(2);
+  // By the parity of the tile: the pages of the tiles whose codes are loaded next, and
+  // the scales of the tiles whose scores come next.
+  int32_t pages[2] = {pages_of(0), pages_of(1)};
+  const int32_t third = pages_of(2);
   // The query rows as operands: dimensions 16 c + 8 h .. + 7 of row n.
   half8_t q_hi[kSteps], q_lo[kTwo ? kSteps : 1];
   float row_factor;
@@ -187,31 +190,30 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   }
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    load_k(0, pages_0, i);
-    load_v(0, pages_0, i);
+    load_k(0, pages[0], i);
+    load_v(0, pages[0], i);
   }
-  Scales scales = scales_of(pages_0), next_scales = scales_of(pages_1);
+  Scales scales[2] = {scales_of(pages[0]), scales_of(pages[1])};
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
     store_k(0, i, 0);
     store_k(0, i, 1);
-    load_k(1, pages_1, i);
+    load_k(1, pages[1], i);
   }
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
     store_v(0, i, 0);
     store_v(0, i, 1);
-    load_v(1, pages_1, i);
+    load_v(1, pages[1], i);
   }
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
     store_k(1, i, 0);
     store_k(1, i, 1);
-    load_k(2, pages_2, i);
+    load_k(2, third, i);
   }
-  // From here on: pages_1 of the tile whose values are loaded next, pages_2 of its keys'.
-  pages_1 = pages_2;
-  pages_2 = pages_of(3);
+  pages[0] = third;
+  pages[1] = pages_of(3);
 
   float16_t o[kDims];
 #pragma unroll
@@ -224,14 +226,14 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
 
   // Fragment i of a tile's keys: step i / kSub, 32-key half i % kSub.
   constexpr int kKeyFrags = kSteps * kSub, kValueFrags = 2 * kSub * kDims, kRing = 4;
-  auto key_frag = [&](uint32_t t, int i) {
-    return *reinterpret_cast<const half8_t*>(lds_k + (t & 1u) * kTileK +
+  auto key_frag = [&](int parity, int i) {
+    return *reinterpret_cast<const half8_t*>(lds_k + parity * kTileK +
                                              (32u * (i % kSub) + key_row) * kStride + 8u * h +
                                              16 * (i / kSub));
   };
   // Fragment i of a tile's values: 16-key step i / kDims, dimensions 32 (i % kDims) on.
-  auto value_frag = [&](uint32_t t, int i) {
-    return *reinterpret_cast<const half8_t*>(lds_v + (t & 1u) * kTileV +
+  auto value_frag = [&](int parity, int i) {
+    return *reinterpret_cast<const half8_t*>(lds_v + parity * kTileV +
                                              ((2u * (i / kDims) + h) * D + n) * 8u +
                                              256 * (i % kDims));
   };
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   };
 
   __syncthreads();
-  float16_t score[kSub];
+  float16_t scores[2][kSub];
   {
     half8_t ring[kRing];
 #pragma unroll
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
     }
     static_for<kKeyFrags>([&](auto slot) {
       constexpr int i = decltype(slot)::value;
-      score_product(score, ring[i % kRing], i);
+      score_product(scores[0], ring[i % kRing], i);
       if constexpr (i + kRing < kKeyFrags) {
         ring[i % kRing] = key_frag(0, i + kRing);
       }
@@ -270,31 +272,37 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   // t while the codes that arrived (keys of t + 2, values of t + 1) become f16 in LDS and
   // those of the tiles after set out.  One barrier a step: what it publishes was written
   // in the step before, to buffers last read before the barrier before.
-  for (uint32_t t = 0; t < tiles; ++t) {
+  // Registers and buffers go by the parity of t, so that nothing is copied from step to
+  // step: a copy of what is still loading would wait for it.
+  auto step = [&](auto even_odd, uint32_t t) __attribute__((always_inline)) {
+    constexpr int kParity = decltype(even_odd)::value;
+    float16_t(&score)[kSub] = scores[kParity];
+    float16_t(&next)[kSub] = scores[1 - kParity];
     __syncthreads();
     const uint32_t first_key = begin + t * kKeys;
     const bool masked = first_key + kKeys > open;  // uniform
     const bool more = t + 1u < tiles;              // uniform
     half8_t ring[kRing];
-    float16_t next[kSub];
     if (more) {
 #pragma unroll
       for (int i = 0; i < kRing; ++i) {
-        ring[i] = key_frag(t + 1u, i);
+        ring[i] = key_frag(1 - kParity, i);
       }
     }
     // The tile's scales by granule: of the scores, and of the weights.
-    const ValueScale sv = value_scale(scales.value);
-    const float lane_key = scales.inside ? scales.key : 0.0f;
-    const float lane_exponent = scales.inside ? sv.exponent : -INFINITY;
-    const float lane_mantissa = scales.inside ? sv.mantissa : 0.0f;
-    float factor[2 * kSub], mantissa[2 * kSub];
+    const Scales held = scales[kParity];
+    const ValueScale sv = value_scale(held.value);
+    const float lane_key = held.inside ? held.key : 0.0f;
+    const float lane_exponent = held.inside ? sv.exponent : -INFINITY;
+    const float lane_inverse = held.inside ? sv.inverse : 0.0f;
+    float factor[2 * kSub], exponent[2 * kSub], inverse[2 * kSub];
 #pragma unroll
     for (int b = 0; b < 2 * kSub; ++b) {
       // Not zero: a masked score's -inf has to stay one (a NaN stays NaN).
       const float f = row_factor * of(lane_key, b);
       factor[b] = f < 1e-37f ? 1e-37f : f;
-      mantissa[b] = of(lane_mantissa, b);
+      exponent[b] = of(lane_exponent, b);
+      inverse[b] = of(lane_inverse, b);
     }
     if (masked) {
 #pragma unroll
@@ -307,7 +315,8 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
         }
         // A page that the row does not see at all may have NaN scales.
         factor[b] = key < visible ? factor[b] : 1.0f;
-        mantissa[b] = key < visible ? mantissa[b] : 0.0f;
+        exponent[b] = key < visible ? exponent[b] : 0.0f;
+        inverse[b] = key < visible ? inverse[b] : 0.0f;
       }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -328,7 +337,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
         float run = fmaxf(fmaxf(x[r], x[r + 1]), x[r + 2]);
         run = fmaxf(fmaxf(run, x[r + 3]), x[r + 4]);
         run = fmaxf(fmaxf(run, x[r + 5]), x[r + 6]);
-        largest = fmaxf(largest, fmaf(fmaxf(run, x[r + 7]), factor[b], of(lane_exponent, b)));
+        largest = fmaxf(largest, fmaf(fmaxf(run, x[r + 7]), factor[b], exponent[b]));
         asm volatile("" : "+v"(largest));
       } else if constexpr (kPiece == 2 * kSub) {
         largest = xor32_max(largest);
@@ -339,7 +348,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
         sum *= keep;
 #pragma unroll
         for (int b = 0; b < 2 * kSub; ++b) {
-          base[b] = of(lane_exponent, b) - top;
+          base[b] = exponent[b] - (top - kWeightShift);
         }
         asm volatile("" : "+v"(top), "+v"(keep), "+v"(sum));
       } else {
@@ -347,20 +356,22 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
         constexpr int r = 8 * (b % 2) + 2 * j;
         const float x = fast_exp2(fmaf(score[b / 2][r], factor[b], base[b]));
         const float y = fast_exp2(fmaf(score[b / 2][r + 1], factor[b], base[b]));
+        // In f32: a page of small or zero scale counts whole in the sum though its
+        // weights vanish in f16.
         all[b] = j == 0 ? x + y : all[b] + (x + y);
-        if constexpr (j == 3) {
-          sum = fmaf(all[b], of(sv.shift, b), sum);
-          asm volatile("" : "+v"(sum));
-        }
         half2_t hi, lo;
         if constexpr (kTwo) {
-          split_pair(x * mantissa[b], y * mantissa[b], hi, lo);
-          asm volatile("" : "+v"(hi), "+v"(lo));
+          split_pair(x, y, hi, lo);
+          asm volatile("" : "+v"(hi), "+v"(lo), "+v"(all[b]));
           p_lo[b][2 * j] = lo[0];
           p_lo[b][2 * j + 1] = lo[1];
         } else {
-          hi = half2_t{(half_t)(x * mantissa[b]), (half_t)(y * mantissa[b])};
-          asm volatile("" : "+v"(hi));
+          hi = half2_t{(half_t)x, (half_t)y};
+          asm volatile("" : "+v"(hi), "+v"(all[b]));
+        }
+        if constexpr (j == 3) {
+          sum = fmaf(all[b], inverse[b], sum);
+          asm volatile("" : "+v"(sum));
         }
         p_hi[b][2 * j] = hi[0];
         p_hi[b][2 * j + 1] = hi[1];
@@ -373,7 +384,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
         constexpr int kFrom = i * kPieces / kKeyFrags, kTo = (i + 1) * kPieces / kKeyFrags;
         score_product(next, ring[i % kRing], i);
         if constexpr (i + kRing < kKeyFrags) {
-          ring[i % kRing] = key_frag(t + 1u, i + kRing);
+          ring[i % kRing] = key_frag(1 - kParity, i + kRing);
         }
         static_for<kTo - kFrom>([&](auto j) {
           soft_piece(std::integral_constant<int, kFrom + decltype(j)::value>{});
@@ -387,7 +398,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
     // O += V^T P^T, and the codes' pieces: halves of K's and V's chunks in turn.
 #pragma unroll
     for (int i = 0; i < kRing; ++i) {
-      ring[i] = value_frag(t, i);
+      ring[i] = value_frag(kParity, i);
     }
     if (__any(lead)) {
 #pragma unroll
@@ -409,31 +420,35 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
                                                               o[i % kDims], 0, 0, 0);
       }
       if constexpr (i + kRing < kValueFrags) {
-        ring[i % kRing] = value_frag(t, i + kRing);
+        ring[i % kRing] = value_frag(kParity, i + kRing);
       }
       static_for<kTo - kFrom>([&](auto piece) {
         constexpr int j = kFrom + decltype(piece)::value, chunk = j / 4, half = j % 2;
         if constexpr (j % 4 < 2) {
-          store_k(t, chunk, half);  // of tile t + 2
+          store_k(kParity, chunk, half);  // of tile t + 2
           if constexpr (half == 1) {
-            load_k(t + 3u, pages_2, chunk);
+            load_k(t + 3u, pages[1 - kParity], chunk);
           }
         } else {
-          store_v(t + 1u, chunk, half);
+          store_v(1 - kParity, chunk, half);  // of tile t + 1
           if constexpr (half == 1) {
-            load_v(t + 2u, pages_1, chunk);
+            load_v(t + 2u, pages[kParity], chunk);
           }
         }
       });
       __builtin_amdgcn_sched_barrier(0);
     });
-    scales = next_scales;
-    next_scales = scales_of(pages_1);
-    pages_1 = pages_2;
-    pages_2 = pages_of(t + 4u);
-#pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-      score[u] = next[u];
+    scales[kParity] = scales_of(pages[kParity]);
+    pages[kParity] = pages_of(t + 4u);
+  };
+  for (uint32_t t = 0;;) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (++t == tiles) {
+      break;
+    }
+    step(std::integral_constant<int, 1>{}, t);
+    if (++t == tiles) {
+      break;
     }
   }
 
@@ -477,7 +492,9 @@ void launch_tiles(const PagedAttentionArgs& a, const PagedSplit& split, hipStrea
   const uint64_t rows = (uint64_t)a.batch.max_query * (a.heads / a.cache.kv_heads);
   const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows;
   const dim3 grid((uint32_t)(tiles * split.tile_splits), a.cache.kv_heads, a.batch.sequences);
-  attention_paged_tile_kernel<D, T, 2, kWavesPerSimd><<<grid, kThreads, 0, stream>>>(a, split);
+  // 64 keys a tile; 32 where two f32 parts of 256 dimensions leave no registers for more.
+  constexpr int kSub = D == 256 && std::is_same<T, float>::value ? 1 : 2;
+  attention_paged_tile_kernel<D, T, kSub, kWavesPerSimd><<<grid, kThreads, 0, stream>>>(a, split);
 }
 
 template <class T>

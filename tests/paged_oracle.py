@@ -93,7 +93,7 @@ def append(cache, name, rows, batch):
                     continue
                 if lo == p * pt or scale == 0:
                     scale = np.float32(np.float32(largest) / np.float32(127))
-                    if scale < np.finfo(np.float32).tiny:
+                    if scale < 2.0 ** -100:
                         scale = np.float32(0)
                     codes[:lo - p * pt] = 0
                 else:
@@ -154,11 +154,16 @@ def attention_tolerance(magnitude, out, score, head_dim, f16):
     """Per value.  A score is a sum of head_dim products in f32: its error is about
     sqrt(head_dim) half steps of the absolute products' sum, taken 8 times, and a
     score's error is its weight's relative one; the sums over keys, the exponential
-    and the division add at most 64 half steps.  With f16 a weight is off by half a
-    step of f16, and so is the output."""
+    and the division add at most 64 half steps.  The exponent of a page's value scale is
+    at most 128 in size, so that it and what it is added to are off by half a step of 128
+    (2^-18) times ln 2 in the weight.  Beside these, a weight times its scale is held in
+    f16 parts whose last place is 2^-24 of a unit that is at least 2^-11 of the largest:
+    what lies below is lost, 2^-35 of the largest weight times scale, for codes of up to
+    127 and each key.  With f16 a weight is off by half a step of f16, and so is the
+    output."""
     step = 2.0 ** -24
     tol = magnitude * step * (8.0 * math.sqrt(head_dim) * score[..., :1] + 64.0)
-    tol = tol + 127.0 * 2.0 ** -38 * score[..., 1:]
+    tol = tol + magnitude * 2.0 ** -18 + 127.0 * 2.0 ** -35 * score[..., 1:]
     if f16:
         tol = tol + magnitude * 2.0 ** -11 + np.abs(out) * 2.0 ** -11 + 2.0 ** -25
     return tol + 1e-30
