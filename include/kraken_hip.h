@@ -739,7 +739,7 @@ KRAKEN_API int kraken_hip_argmax_prob_f32_i32(kraken_hip_context* context, krake
  * rows: sequence b's are rows query_starts[b] .. query_starts[b + 1] - 1 (it may
  * bring none), and with them it is lengths[b] tokens long, so its row i stands at
  * position lengths[b] - count + i.  page_table[b][p] is the page that holds
- * positions p * page_tokens on; entries past the length are not read.
+ * positions p * page_tokens on; entries past the length have no effect.
  * max_query and max_keys bound every sequence's new tokens and length; they size
  * the launches and need not be tight.  The arrays are device memory, read when
  * the kernels run, so a captured graph replays with new ones in their place.

@@ -29,6 +29,11 @@ namespace {
 
 constexpr uint32_t kWaves = 4;
 
+// Codes of a decode step are read by one workgroup, once.
+__device__ __forceinline__ u32x4_t load_once(const int8_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+}
+
 template <int D, class T, bool kStacked>
 __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAttentionArgs a,
                                                                         PagedSplit split) {
@@ -41,19 +46,40 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
 
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t n = lane & 15u, g = lane >> 4;
-  const uint32_t kv_head = blockIdx.y, sequence = blockIdx.z;
   const uint32_t shift = a.cache.page_shift, kv_heads = a.cache.kv_heads;
   const uint32_t group = a.heads / kv_heads;
-  const PagedSequence s = paged_sequence(a.batch, sequence, shift);
+  const uint32_t kv_head = blockIdx.x % kv_heads;
+  uint32_t part = blockIdx.x / kv_heads, sequence = 0;
+  PagedSequence s;
+  if (a.batch.sequences > 1u) {
+    // The sequences' parts one after another: no workgroup without keys stands between
+    // two with, and the XCDs, which take workgroups in turn, get as many each.
+    const PagedItem found = paged_item(a.batch, part, shift, [&](const PagedSequence& q) {
+      return q.count * group <= kRows ? (q.length + split.decode_keys - 1u) / split.decode_keys
+                                      : 0u;
+    });
+    s = found.sequence;
+    sequence = found.index;
+    part = found.item;
+  }
+  const uint32_t begin = part * split.decode_keys;
+  // The first pages' ids are asked for together with a single sequence's length (in the
+  // bounds of the table whatever that is): K and V wait for two loads in a row, not three.
+  const int32_t* table = a.batch.table + (size_t)sequence * a.batch.width;
+  auto page_of = [&](uint32_t key) { return table[min(key >> shift, a.batch.width - 1u)]; };
+  auto first_key = [&](uint32_t step) { return begin + step * 32u; };
+  // Of the lane's key rows (run n / 4 of the step's four) and of its own run g.
+  int32_t page_k = page_of(first_key(wave) + 8u * (n >> 2));
+  int32_t page_v = page_of(first_key(wave) + 8u * g);
+  if (a.batch.sequences == 1u) {
+    s = paged_sequence(a.batch, 0, shift);
+  }
   const uint32_t rows = s.count * group;
-  const uint32_t begin = blockIdx.x * split.decode_keys;
   if (s.count == 0 || rows > kRows || begin >= s.length) {
     return;
   }
   const uint32_t end = min(s.length, begin + split.decode_keys);
   const uint32_t steps = (end - begin + 31u) / 32u;
-  const int32_t* table = a.batch.table + (size_t)sequence * a.batch.width;
-  const uint32_t last_page = (s.length - 1u) >> shift;
 
   // This lane's query row and the keys that it sees.
   const uint32_t row = kStacked ? n & 7u : n;
@@ -63,11 +89,6 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   const size_t at = ((size_t)(s.start + token) * a.heads + kv_head * group +
                      (real ? row % group : 0u)) * D;
 
-  // Page ids of the lane's key rows (run n / 4 of the step's four) and of its own run g.
-  auto page_of = [&](uint32_t key) {
-    return table[min(key >> shift, last_page)];
-  };
-  auto first_key = [&](uint32_t step) { return begin + step * 32u; };
   u32x4_t k[2][kLoads], v[2 * kLoads];
   float key_scale, val_scale;
   bool inside;
@@ -78,9 +99,8 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
                       ((((size_t)held * kv_heads + kv_head) << shift) +
                        (key & ((1u << shift) - 1u))) * D + 16u * g;
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c) {
-      k[0][c] = *reinterpret_cast<const u32x4_t*>(p + 64 * c);
-      k[1][c] = *reinterpret_cast<const u32x4_t*>(p + 4 * D + 64 * c);
+    for (int i = 0; i < 2 * kLoads; ++i) {
+      k[i / kLoads][i % kLoads] = load_once(p + i / kLoads * 4 * D + 64 * (i % kLoads));
     }
   };
   auto load_v = [&](uint32_t step, int32_t page) {
@@ -91,17 +111,11 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
                       ((page_head << shift) + (key & ((1u << shift) - 1u))) * D + 16u * n;
 #pragma unroll
     for (int c = 0; c < 2 * kLoads; ++c) {
-      v[c] = *reinterpret_cast<const u32x4_t*>(p + 256 * c);
+      v[c] = load_once(p + 256 * c);
     }
     key_scale = a.cache.key_scales[page_head];
     val_scale = a.cache.value_scales[page_head];
   };
-
-  int32_t page_k = 0, page_v = 0;
-  if (wave < steps) {
-    page_k = page_of(first_key(wave) + 8u * (n >> 2));
-    page_v = page_of(first_key(wave) + 8u * g);
-  }
 
   // The query: D / 4 values a lane, those of its dimensions 64 c + 16 g .. + 15.
   half8_t q_hi[2 * kLoads], q_lo[kTwo ? 2 * kLoads : 1];
@@ -173,14 +187,13 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
       page_k = page_of(first_key(next) + 8u * (n >> 2));
       page_v = page_of(first_key(next) + 8u * g);
     }
-    float4_t score[2];
+    float4_t score[2] = {float4_t{0.0f, 0.0f, 0.0f, 0.0f}, float4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-    for (int tile = 0; tile < 2; ++tile) {
-      score[tile] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < kLoads; ++c) {
 #pragma unroll
-      for (int c = 0; c < kLoads; ++c) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int tile = 0; tile < 2; ++tile) {
           const half8_t x = codes_to_f16(k[tile][c][2 * h], k[tile][c][2 * h + 1]);
           score[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q_hi[2 * c + h], score[tile],
                                                                0, 0, 0);
@@ -301,8 +314,8 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   }
   __syncthreads();
   const bool whole = s.length <= split.decode_keys;
-  for (uint32_t i = threadIdx.x; i < rows * D; i += 256u) {
-    const uint32_t r = i / D, d = i % D;
+  for (uint32_t e = threadIdx.x; e < rows * D; e += 256u) {
+    const uint32_t r = e / D, d = e % D;
     float m = lds_m[0][r];
 #pragma unroll
     for (uint32_t w = 1; w < kWaves; ++w) {
@@ -319,53 +332,46 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
       const size_t out = ((size_t)(s.start + r / group) * a.heads + kv_head * group + r % group) * D;
       store_output<T>(a, out + d, x, inverse_sum(l));
     } else {
-      const size_t part = ((size_t)(blockIdx.x * a.batch.sequences + sequence) * kv_heads +
-                           kv_head) * split.decode_rows + r;
-      split.decode_o[part * D + d] = x;
+      const size_t i = (((size_t)part * a.batch.sequences + sequence) * kv_heads + kv_head) *
+                         split.decode_rows + r;
+      split.decode_o[i * D + d] = x;
       if (d == 0) {
-        split.decode_ml[2 * part] = m;
-        split.decode_ml[2 * part + 1] = l;
+        split.decode_ml[2 * i] = m;
+        split.decode_ml[2 * i + 1] = l;
       }
     }
   }
 }
 
-// Joins split results: a wave per (row, head), D / 64 values a lane.
-template <int D, class T>
+// Joins split results: kParts waves per (row, head), which take its parts in turn, D / 64
+// values a lane.
+template <int D, class T, int kParts>
 __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentionArgs a,
                                                                    PagedSplit split) {
   constexpr int kRegs = D / 64;
+  __shared__ float lds[kParts > 1 ? kParts : 1][64 * kRegs];
   const uint32_t lane = threadIdx.x & 63u;
-  const uint64_t item = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint64_t item = kParts > 1 ? blockIdx.x : (uint64_t)blockIdx.x * 4u + wave;
   if (item >= (uint64_t)a.batch.tokens * a.heads) {
     return;
   }
   const uint32_t token = (uint32_t)(item / a.heads), head = (uint32_t)(item % a.heads);
-  uint32_t b = 0;
-  for (uint32_t at = 1; at <= a.batch.sequences; at += 64) {
-    const uint32_t i = at + lane;
-    b += (uint32_t)__popcll(__ballot(i <= a.batch.sequences && a.batch.starts[i] <= token));
-  }
-  if (b >= a.batch.sequences) {
-    return;
-  }
-  const PagedSequence s = paged_sequence(a.batch, b, a.cache.page_shift);
-  if (token < s.start || token >= s.start + s.count) {
-    return;
-  }
+  const PagedRow found = paged_row(a.batch, token, a.cache.page_shift);
+  const PagedSequence s = found.sequence;
   const uint32_t group = a.heads / a.cache.kv_heads;
-  const bool decode = s.count * group <= kDecodeRows;
+  const bool decode = s.count * group <= split.decode_most;
   const uint32_t per = decode ? split.decode_keys : split.tile_keys;
-  if (s.length <= per) {
-    return;  // written by its workgroup
+  if (s.count == 0 || s.length <= per) {
+    return;  // of no sequence, or written by its workgroup
   }
-  // Splits whose first key the row sees.
+  // Parts whose first key the row sees.
   const uint32_t visible = s.length - s.count + (token - s.start) + 1u;
-  const uint32_t splits = (visible + per - 1u) / per;
+  const uint32_t parts = (visible + per - 1u) / per;
   size_t first, stride;
   const float *o, *ml;
   if (decode) {
-    first = ((size_t)b * a.cache.kv_heads + head / group) * split.decode_rows +
+    first = ((size_t)found.index * a.cache.kv_heads + head / group) * split.decode_rows +
             (token - s.start) * group + head % group;
     stride = (size_t)a.batch.sequences * a.cache.kv_heads * split.decode_rows;
     o = split.decode_o;
@@ -376,49 +382,78 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
     o = split.tile_o;
     ml = split.tile_ml;
   }
-  float m = kLowestMax;
-  for (uint32_t i = lane; i < splits; i += 64) {
-    m = fmaxf(m, ml[2 * (first + i * stride)]);
-  }
+  // This wave's parts are part0, part0 + kParts, ..; eight at a time, whose loads go out
+  // together (past the last they repeat it, with weight 0).  Each wave keeps a maximum of
+  // its own.
+  const uint32_t part0 = kParts > 1 ? wave : 0u;
+  float m = kLowestMax, l = 0.0f, x[kRegs] = {};
+  for (uint32_t at = part0; at < parts; at += 8u * kParts) {
+    float2 here[8];
+    float sums[8][kRegs];
 #pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    m = fmaxf(m, __shfl_xor(m, step, 64));
-  }
-  float l = 0.0f, x[kRegs] = {};
-  for (uint32_t at = 0; at < splits; at += 64) {
-    float keep = 0.0f;
-    if (at + lane < splits) {
-      const float2 part = *reinterpret_cast<const float2*>(&ml[2 * (first + (at + lane) * stride)]);
-      keep = fast_exp2(part.x - m);
-      l = fmaf(keep, part.y, l);
-    }
-    const uint32_t here = min(64u, splits - at);
-    // Eight parts' loads together; past the last they repeat it, with weight 0.
-    for (uint32_t i = 0; i < here; i += 8) {
-      float part[8][kRegs];
+    for (uint32_t j = 0; j < 8; ++j) {
+      const size_t i = first + min(at + j * kParts, parts - 1u) * stride;
+      here[j] = *reinterpret_cast<const float2*>(&ml[2 * i]);
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        const float* p = o + (first + (at + min(i + j, here - 1u)) * stride) * D + lane * kRegs;
-#pragma unroll
-        for (int r = 0; r < kRegs; ++r) {
-          part[j][r] = p[r];
-        }
-      }
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        const float k = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(keep), (int)(i + j)));
-#pragma unroll
-        for (int r = 0; r < kRegs; ++r) {
-          x[r] = i + j < here ? fmaf(k, part[j][r], x[r]) : x[r];
-        }
+      for (int r = 0; r < kRegs; ++r) {
+        sums[j][r] = o[i * D + lane * kRegs + r];
       }
     }
-  }
-  l = wave_sum(l);
-  const float inverse = inverse_sum(l);
+    float up = m;
 #pragma unroll
-  for (int r = 0; r < kRegs; ++r) {
-    store_output<T>(a, item * D + lane * kRegs + r, x[r], inverse);
+    for (uint32_t j = 0; j < 8; ++j) {
+      up = fmaxf(up, here[j].x);
+    }
+    const float keep = fast_exp2(m - up);
+    m = up;
+    l *= keep;
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r) {
+      x[r] *= keep;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      const float w = at + j * kParts < parts ? fast_exp2(here[j].x - m) : 0.0f;
+      l = fmaf(w, here[j].y, l);
+#pragma unroll
+      for (int r = 0; r < kRegs; ++r) {
+        x[r] = at + j * kParts < parts ? fmaf(w, sums[j][r], x[r]) : x[r];
+      }
+    }
+  }
+  if constexpr (kParts > 1) {
+    __shared__ float lds_m[kParts], lds_l[kParts];
+    if (lane == 0) {
+      lds_m[wave] = m;
+      lds_l[wave] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r) {
+      lds[wave][lane * kRegs + r] = x[r];
+    }
+    __syncthreads();
+    // Thread i takes value i of the row.
+    if (threadIdx.x >= (uint32_t)D) {
+      return;
+    }
+    float top = lds_m[0], sum = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int w = 1; w < kParts; ++w) {
+      top = fmaxf(top, lds_m[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < kParts; ++w) {
+      const float keep = fast_exp2(lds_m[w] - top);
+      sum = fmaf(keep, lds_l[w], sum);
+      value = fmaf(keep, lds[w][threadIdx.x], value);
+    }
+    store_output<T>(a, item * D + threadIdx.x, value, inverse_sum(sum));
+  } else {
+    const float inverse = inverse_sum(l);
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r) {
+      store_output<T>(a, item * D + lane * kRegs + r, x[r], inverse);
+    }
   }
 }
 
@@ -426,23 +461,30 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   PagedSplit s{};
   const uint64_t group = a.heads / a.cache.kv_heads;
   const uint64_t rows = group * a.batch.max_query;
-  // Keys per workgroup: 128 (a 32-key step for each wave) while that gives no more than
-  // eight workgroups a CU at the longest length, up to 4096; more where the partial
-  // results of the longest lengths would take over 256 MiB.
+  // Keys per workgroup: 128 (a 32-key step for each wave) while all sequences at the
+  // longest length make no more than eleven workgroups a CU, else as many as make so few,
+  // up to 4096; more where the partial results would take over 256 MiB.  (64 sequences of
+  // up to 32768 keys, 2 KV heads: 512 keys 226 us, 1024 205, 1280 197, 1536 194, 2048 205.
+  // One of 4096, 32 workgroups of 128: 12.8 us.)
   const uint64_t lanes = (uint64_t)a.batch.sequences * a.cache.kv_heads;
   const uint64_t part_bytes =
     std::min<uint64_t>(rows, kDecodeRows) * (a.cache.head_dim + 2u) * sizeof(float);
+  const uint64_t most = 11u * (uint64_t)cu_count;
   auto parts = [&](uint64_t k) { return lanes * ((a.batch.max_keys + k - 1u) / k); };
-  uint64_t keys = 128;
-  while ((keys < 4096u && parts(keys) > 8u * (uint64_t)cu_count) ||
-         (parts(keys) > lanes && parts(keys) * part_bytes > (uint64_t{256} << 20))) {
+  uint64_t keys = (lanes * a.batch.max_keys + most - 1u) / most;
+  keys = std::min<uint64_t>((keys + 127u) / 128u * 128u, 4096u);
+  while (parts(keys) > lanes && parts(keys) * part_bytes > (uint64_t{256} << 20)) {
     keys *= 2u;
   }
+  // A single sequence with many rows needs no second kernel beside the tiled one.
+  s.decode_most = rows <= kDecodeRows || a.batch.sequences > 1u ? kDecodeRows : 0u;
   s.decode_keys = (uint32_t)keys;
   s.decode_rows = (uint32_t)std::min<uint64_t>(rows, kDecodeRows);
   s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
   // The tiled kernel's keys in parts until there are as many workgroups as the CUs hold
-  // (one of head_dim 256, two of less), each of 128 keys at least, and while their results take no more than 256 MiB.
+  // (one of head_dim 256, two of less), or four times as many where sequences of several
+  // lengths share the device (17 of up to 4200 keys: 87 us with twice, 84 with four
+  // times), each of 128 keys at least, and while their results take no more than 256 MiB.
   const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows * a.cache.kv_heads;
   const uint64_t all_tiles =
     std::min<uint64_t>(tiles * a.batch.sequences,
@@ -452,18 +494,21 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   const uint64_t row_bytes =
     (uint64_t)a.batch.tokens * a.heads * (a.cache.head_dim + 2u) * sizeof(float);
   uint64_t splits = 1;
-  while (rows > kDecodeRows && all_tiles * splits < (a.cache.head_dim == 256u ? 1u : 2u) * (uint64_t)cu_count &&
+  const uint64_t enough = (a.cache.head_dim == 256u ? 1u : 2u) *
+                          (a.batch.sequences > 1u ? 4u : 1u) * (uint64_t)cu_count;
+  while (rows > kDecodeRows && all_tiles * splits < enough &&
          a.batch.max_keys / (2u * splits) >= 128u &&
          2u * splits * row_bytes <= (uint64_t{256} << 20)) {
     splits *= 2u;
   }
   s.tile_keys = (uint32_t)((a.batch.max_keys + splits - 1u) / splits + 63u) & ~63u;
   s.tile_splits = (uint32_t)((a.batch.max_keys + s.tile_keys - 1u) / s.tile_keys);
+  s.tile_blocks = (uint32_t)(all_tiles * s.tile_splits);
   return s;
 }
 
 size_t decode_parts(const PagedAttentionArgs& a, const PagedSplit& s) {
-  return s.decode_splits <= 1u ? 0u
+  return s.decode_splits <= 1u || s.decode_most == 0u ? 0u
                                : (size_t)s.decode_splits * a.batch.sequences * a.cache.kv_heads *
                                    s.decode_rows;
 }
@@ -476,8 +521,8 @@ template <int D, class T>
 void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
   const uint32_t group = a.heads / a.cache.kv_heads;
   const uint64_t rows = (uint64_t)a.batch.max_query * group;
-  if (group <= kDecodeRows) {
-    const dim3 grid(split.decode_splits, a.cache.kv_heads, a.batch.sequences);
+  if (group <= split.decode_most) {
+    const dim3 grid(split.decode_splits * a.cache.kv_heads * a.batch.sequences);
     if (rows <= 8u) {
       attention_paged_decode_kernel<D, T, true><<<grid, 256, 0, stream>>>(a, split);
     } else {
@@ -487,9 +532,15 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
   if (rows > kDecodeRows) {
     launch_attention_paged_q8_tiles(a, split, stream);
   }
-  if (split.decode_splits > 1u || split.tile_splits > 1u) {
-    const uint64_t items = (uint64_t)a.batch.tokens * a.heads;
-    attention_paged_join_kernel<D, T><<<dim3((uint32_t)((items + 3u) / 4u)), 256, 0, stream>>>(
+  const uint64_t items = (uint64_t)a.batch.tokens * a.heads;
+  const uint32_t parts = std::max(split.decode_most != 0u ? split.decode_splits : 1u,
+                                  rows > kDecodeRows ? split.tile_splits : 1u);
+  // Four waves a row where there are many parts (one row of 33 parts 7.3 -> 4 us), and not
+  // more rows than a grid holds of them.
+  if (parts > 8u && items <= (uint64_t{1} << 22)) {
+    attention_paged_join_kernel<D, T, 4><<<dim3((uint32_t)items), 256, 0, stream>>>(a, split);
+  } else if (parts > 1u) {
+    attention_paged_join_kernel<D, T, 1><<<dim3((uint32_t)((items + 3u) / 4u)), 256, 0, stream>>>(
       a, split);
   }
 }

@@ -44,11 +44,13 @@ constexpr uint32_t kTileRows = 128;
 // (M, l) of row r of (split, sequence, KV head) for the decode kernel, of (split, token,
 // head) for the tiled one.
 struct PagedSplit {
+  uint32_t decode_most;   // rows of a sequence up to which the decode kernel takes it
   uint32_t decode_keys;   // keys per workgroup of the decode kernel
   uint32_t decode_rows;   // rows held per (split, sequence, KV head)
   uint32_t decode_splits;
   uint32_t tile_keys;     // keys per workgroup of the tiled kernel
   uint32_t tile_splits;
+  uint32_t tile_blocks;   // its workgroups, as many as a batch can need
   float* decode_o;
   float* decode_ml;
   float* tile_o;

@@ -52,16 +52,28 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t n = lane & 31u, h = lane >> 5;
-  const uint32_t part = blockIdx.x % split.tile_splits, tile = blockIdx.x / split.tile_splits;
-  const uint32_t kv_head = blockIdx.y, sequence = blockIdx.z;
   const uint32_t shift = a.cache.page_shift, kv_heads = a.cache.kv_heads;
   const uint32_t group = a.heads / kv_heads;
-  const PagedSequence s = paged_sequence(a.batch, sequence, shift);
-  const uint32_t rows = s.count * group;
-  const uint32_t first_row = tile * kTileRows;
-  if (rows <= kDecodeRows || first_row >= rows) {
+  // The sequences' (tile, part) pairs one after another, so that no workgroup without
+  // work stands between two with; the parts of a tile side by side, so that an XCD, which
+  // gets every eighth workgroup, reads few parts of a sequence's keys.
+  const uint32_t kv_head = blockIdx.x % kv_heads;
+  const PagedItem found =
+    paged_item(a.batch, blockIdx.x / kv_heads, shift, [&](const PagedSequence& q) {
+      const uint32_t r = q.count * group;
+      return r > split.decode_most ? (r + kTileRows - 1u) / kTileRows *
+                                       ((q.length + split.tile_keys - 1u) / split.tile_keys)
+                                   : 0u;
+    });
+  const PagedSequence s = found.sequence;
+  const uint32_t sequence = found.index;
+  if (s.count == 0) {
     return;
   }
+  const uint32_t parts = (s.length + split.tile_keys - 1u) / split.tile_keys;
+  const uint32_t tile = found.item / parts, part = found.item % parts;
+  const uint32_t rows = s.count * group;
+  const uint32_t first_row = tile * kTileRows;
   // The keys that the tile's last row sees, of this part.
   const uint32_t before = s.length - s.count;
   const uint32_t last_row = min(first_row + kTileRows, rows) - 1u;
@@ -72,7 +84,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   }
   const uint32_t tiles = (end - begin + kKeys - 1u) / kKeys;
   const int32_t* table = a.batch.table + (size_t)sequence * a.batch.width;
-  const uint32_t last_page = (s.length - 1u) >> shift;
 
   const uint32_t wave_row = first_row + wave * 32u;
   const uint32_t row = wave_row + n;
@@ -88,7 +99,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   // last one's again.
   auto pages_of = [&](uint32_t t) {
     const uint32_t key = begin + min(t, tiles - 1u) * kKeys + 16u * (lane % kGranules);
-    return table[min(key >> shift, last_page)];
+    return table[min(key >> shift, a.batch.width - 1u)];
   };
   auto held_page = [&](int32_t page) {
     return page >= 0 && (uint32_t)page < a.cache.pages ? (uint32_t)page : 0u;
@@ -139,36 +150,41 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   // the scales of the tiles whose scores come next.
   int32_t pages[2] = {pages_of(0), pages_of(1)};
   const int32_t third = pages_of(2);
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    load_k(0, pages[0], i);
+    load_v(0, pages[0], i);
+  }
+  Scales scales[2] = {scales_of(pages[0]), scales_of(pages[1])};
   // The query rows as operands: dimensions 16 c + 8 h .. + 7 of row n.
   half8_t q_hi[kSteps], q_lo[kTwo ? kSteps : 1];
   float row_factor;
   {
     const T* p = static_cast<const T*>(a.query) + at + 8u * h;
-    float largest = 0.0f;
+    float x[kSteps][8], largest = 0.0f;
 #pragma unroll
     for (int c = 0; c < kSteps; ++c) {
-      float x[8];
-      load4(p + 16 * c, x);
-      load4(p + 16 * c + 4, x + 4);
+      load4(p + 16 * c, x[c]);
+      load4(p + 16 * c + 4, x[c] + 4);
+    }
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        largest = fmaxf(largest, fabsf(x[i]));
+        x[c][i] = real ? x[c][i] : 0.0f;
+        largest = fmaxf(largest, fabsf(x[c][i]));
       }
     }
-    largest = xor32_max(real ? largest : 0.0f);
+    largest = xor32_max(largest);
     const int e = query_exponent(largest);
     row_factor = ldexpf(kLog2e / (D == 64 ? 8.0f : D == 256 ? 16.0f : 11.313708498984761f), -e);
-    // Read again (from the caches) rather than held: the operands take their registers.
 #pragma unroll
     for (int c = 0; c < kSteps; ++c) {
-      float x[8];
-      load4(p + 16 * c, x);
-      load4(p + 16 * c + 4, x + 4);
       half8_t hi, lo;
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         half2_t u, w;
-        split_pair(real ? ldexpf(x[i], e) : 0.0f, real ? ldexpf(x[i + 1], e) : 0.0f, u, w);
+        split_pair(ldexpf(x[c][i], e), ldexpf(x[c][i + 1], e), u, w);
         hi[i] = u[0];
         hi[i + 1] = u[1];
         lo[i] = w[0];
@@ -190,12 +206,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   }
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    load_k(0, pages[0], i);
-    load_v(0, pages[0], i);
-  }
-  Scales scales[2] = {scales_of(pages[0]), scales_of(pages[1])};
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
     store_k(0, i, 0);
     store_k(0, i, 1);
     load_k(1, pages[1], i);
@@ -206,14 +216,6 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
     store_v(0, i, 1);
     load_v(1, pages[1], i);
   }
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    store_k(1, i, 0);
-    store_k(1, i, 1);
-    load_k(2, third, i);
-  }
-  pages[0] = third;
-  pages[1] = pages_of(3);
 
   float16_t o[kDims];
 #pragma unroll
@@ -248,6 +250,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
 
   __syncthreads();
   float16_t scores[2][kSub];
+  // The scores of tile 0 while the keys of tile 1 arrive.
   {
     half8_t ring[kRing];
 #pragma unroll
@@ -263,6 +266,15 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
       __builtin_amdgcn_sched_barrier(0);
     });
   }
+
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) {
+    store_k(1, i, 0);
+    store_k(1, i, 1);
+    load_k(2, third, i);
+  }
+  pages[0] = third;
+  pages[1] = pages_of(3);
 
   auto of = [&](float x, int granule) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), granule));
@@ -485,16 +497,14 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
 
 template <int D, class T>
 void launch_tiles(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
-  // One wave a SIMD where the operands take its 512 registers: two waves' 256 would
-  // spill.
-  constexpr int kWavesPerSimd =
-    D == 256 || (D == 128 && std::is_same<T, float>::value) ? 1 : 2;
-  const uint64_t rows = (uint64_t)a.batch.max_query * (a.heads / a.cache.kv_heads);
-  const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows;
-  const dim3 grid((uint32_t)(tiles * split.tile_splits), a.cache.kv_heads, a.batch.sequences);
-  // 64 keys a tile; 32 where two f32 parts of 256 dimensions leave no registers for more.
-  constexpr int kSub = D == 256 && std::is_same<T, float>::value ? 1 : 2;
-  attention_paged_tile_kernel<D, T, kSub, kWavesPerSimd><<<grid, kThreads, 0, stream>>>(a, split);
+  // One wave a SIMD for head_dim 256, whose operands take its 512 registers.  64 keys a
+  // tile; 32 where two f32 parts of 256 dimensions, or two waves of 128, leave no
+  // registers for more (a spilled one waits for every load under way: 17 sequences,
+  // head_dim 128: 119 us with 64 keys, 104 with 32).
+  constexpr int kWavesPerSimd = D == 256 ? 1 : 2;
+  constexpr int kSub = D == 64 || (D == 256 && !std::is_same<T, float>::value) ? 2 : 1;
+  attention_paged_tile_kernel<D, T, kSub, kWavesPerSimd>
+    <<<dim3(split.tile_blocks), kThreads, 0, stream>>>(a, split);
 }
 
 template <class T>

@@ -15,9 +15,9 @@ using namespace kraken;
 namespace {
 
 constexpr size_t kInt32Max = 0x7fffffffu;
-// Limits of a launch's dimensions: sequences and KV heads are two of them, and the rows
-// (tokens x heads) four to a workgroup of 256 threads.
-constexpr size_t kMaxGrid = 65535;
+// Limits that keep a launch's workgroups of 256 threads within a grid: pairs of a sequence
+// and a KV head, and rows (tokens x heads), four of which share a workgroup.
+constexpr size_t kMaxPairs = size_t{1} << 20;
 constexpr size_t kMaxRows = size_t{1} << 26;
 
 // The cache's checks; `w` begins the messages.
@@ -57,8 +57,8 @@ int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c
   if (((uintptr_t)cache->key_pages.data | (uintptr_t)cache->value_pages.data) & 15u) {
     return invalid("HIP " + at + " pages must be 16-byte aligned");
   }
-  if (cache->kv_heads > kMaxGrid) {
-    return invalid("HIP " + at + " takes up to 65535 kv_heads");
+  if (cache->kv_heads > kMaxPairs) {
+    return invalid("HIP " + at + " takes up to 1048576 kv_heads");
   }
   c.keys = static_cast<int8_t*>(cache->key_pages.data);
   c.values = static_cast<int8_t*>(cache->value_pages.data);
@@ -71,7 +71,8 @@ int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c
   return KRAKEN_OK;
 }
 
-int batch_args(const kraken_paged_batch* batch, const char* w, PagedBatchArgs& b) {
+int batch_args(const kraken_paged_batch* batch, size_t kv_heads, const char* w,
+               PagedBatchArgs& b) {
   const std::string at(w);
   if (batch == nullptr) {
     return invalid("HIP " + at + " batch must not be null");
@@ -83,8 +84,8 @@ int batch_args(const kraken_paged_batch* batch, const char* w, PagedBatchArgs& b
   if (batch->tokens > kInt32Max || batch->max_keys > kInt32Max) {
     return invalid("HIP " + at + " batch exceeds int32 range");
   }
-  if (batch->sequences > kMaxGrid) {
-    return invalid("HIP " + at + " takes up to 65535 sequences");
+  if (batch->sequences > kMaxPairs / kv_heads) {
+    return invalid("HIP " + at + " takes up to 1048576 pairs of a sequence and a KV head");
   }
   size_t entries = 0;
   if (!checked_mul(batch->sequences, batch->table_width, entries)) {
@@ -128,7 +129,7 @@ int paged_attention_entry(kraken_hip_context* ctx, const kraken_buffer& query,
   if (heads % cache->kv_heads != 0) {
     return invalid("HIP paged attention heads must be divisible by kv_heads");
   }
-  KRAKEN_TRY(batch_args(batch, w, a.batch));
+  KRAKEN_TRY(batch_args(batch, cache->kv_heads, w, a.batch));
   size_t rows = 0, values = 0;
   if (!checked_mul(batch->tokens, heads, rows) || !checked_mul(rows, cache->head_dim, values)) {
     return invalid("HIP paged attention value count overflow");
@@ -190,7 +191,7 @@ KRAKEN_API int kraken_hip_qwen35_attention_prologue_paged_q8_kv(
   if (!(theta > 0.0f) || std::isinf(theta)) {
     return invalid("HIP MRoPE theta must be positive and finite");
   }
-  KRAKEN_TRY(batch_args(batch, w, a.batch));
+  KRAKEN_TRY(batch_args(batch, cache->kv_heads, w, a.batch));
   const size_t tokens = batch->tokens;
   size_t rows = 0, query_values = 0, joint_values = 0, kv_rows = 0, kv_values = 0;
   if (!checked_mul(tokens, heads, rows) || !checked_mul(rows, cache->head_dim, query_values) ||

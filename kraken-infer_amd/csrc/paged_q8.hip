@@ -113,27 +113,11 @@ __device__ __forceinline__ void norm_rotate(const float v_in[4], const float w[4
   }
 }
 
-// The sequence that row `token` belongs to, from the starts, 64 at a time: those at
-// or below the token are counted (they do not decrease).
-__device__ __forceinline__ uint32_t sequence_of(const PagedBatchArgs& b, uint32_t token, int lane) {
-  uint32_t sequence = 0;
-  for (uint32_t at = 1; at <= b.sequences; at += 64) {
-    const uint32_t i = at + lane;
-    const bool below = i <= b.sequences && b.starts[i] <= token;
-    sequence += (uint32_t)__popcll(__ballot(below));
-  }
-  return sequence;
-}
-
 // A wave: one token's query heads [first, last).
 __device__ __forceinline__ void query_heads(const PagedPrologueArgs& a, uint32_t token,
                                             uint32_t first, uint32_t last, int lane) {
-  const uint32_t b = sequence_of(a.batch, token, lane);
-  if (b >= a.batch.sequences) {
-    return;
-  }
-  const PagedSequence s = paged_sequence(a.batch, b, a.cache.page_shift);
-  if (token < s.start || token >= s.start + s.count) {
+  const PagedSequence s = paged_row(a.batch, token, a.cache.page_shift).sequence;
+  if (s.count == 0) {
     return;
   }
   const Rotation rot = rotation_of(a, lane);

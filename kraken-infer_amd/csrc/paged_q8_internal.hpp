@@ -89,4 +89,78 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatchArgs& b,
   return {start, fits ? count : 0u, fits ? length : 0u};
 }
 
+// The sequence that row `token` of the batch belongs to, looked for by a wave, 64
+// sequences at a time; count 0 where none has it.
+struct PagedRow {
+  PagedSequence sequence;
+  uint32_t index;
+};
+
+__device__ __forceinline__ PagedRow paged_row(const PagedBatchArgs& b, uint32_t token,
+                                              uint32_t page_shift) {
+  const uint32_t lane = threadIdx.x & 63u;
+  for (uint32_t at = 0; at < b.sequences; at += 64) {
+    const uint32_t i = at + lane;
+    PagedSequence s{0u, 0u, 0u};
+    if (i < b.sequences) {
+      s = paged_sequence(b, i, page_shift);
+    }
+    const uint64_t has = __ballot(token - s.start < s.count);
+    if (has != 0) {
+      const int from = __builtin_ctzll(has);
+      return {{(uint32_t)__builtin_amdgcn_readlane((int)s.start, from),
+               (uint32_t)__builtin_amdgcn_readlane((int)s.count, from),
+               (uint32_t)__builtin_amdgcn_readlane((int)s.length, from)},
+              at + (uint32_t)from};
+    }
+  }
+  return {{0u, 0u, 0u}, 0u};
+}
+
+// Sum over a wave's lanes up to each (row_shr within 16 lanes, then the rows before).
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, true);
+  return x;
+}
+
+// Item `want` of a batch whose sequences have count(sequence) items each, looked for by
+// every wave of a workgroup, 64 sequences at a time: its sequence (index and rows; count 0
+// past the last item) and its number there.
+struct PagedItem {
+  PagedSequence sequence;
+  uint32_t index, item;
+};
+
+template <class Count>
+__device__ __forceinline__ PagedItem paged_item(const PagedBatchArgs& b, uint32_t want,
+                                                uint32_t page_shift, Count count) {
+  const uint32_t lane = threadIdx.x & 63u;
+  for (uint32_t at = 0; at < b.sequences; at += 64) {
+    const uint32_t i = at + lane;
+    PagedSequence s{0u, 0u, 0u};
+    uint32_t items = 0;
+    if (i < b.sequences) {
+      s = paged_sequence(b, i, page_shift);
+      items = s.count != 0 ? count(s) : 0u;
+    }
+    const uint32_t upto = wave_prefix(items);
+    const uint64_t past = __ballot(upto > want);
+    if (past != 0) {
+      const int from = __builtin_ctzll(past);
+      return {{(uint32_t)__builtin_amdgcn_readlane((int)s.start, from),
+               (uint32_t)__builtin_amdgcn_readlane((int)s.count, from),
+               (uint32_t)__builtin_amdgcn_readlane((int)s.length, from)},
+              at + (uint32_t)from,
+              want - (uint32_t)__builtin_amdgcn_readlane((int)(upto - items), from)};
+    }
+    want -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  }
+  return {{0u, 0u, 0u}, 0u, 0u};
+}
+
 }  // namespace kraken

@@ -73,7 +73,7 @@ BATCH_ERRORS = [
     (dict(max_query=0), "batch dimensions must be positive"),
     (dict(tokens=0), "batch dimensions must be positive"),
     (dict(max_keys=1 << 31), "batch exceeds int32 range"),
-    (dict(sequences=65536), "takes up to 65535 sequences"),
+    (dict(sequences=(1 << 19) + 1), "takes up to 1048576 pairs"),
     (dict(width=1 << 62), "overflow"),
     (dict(table=fake(23)), "page table buffer is too small"),
     (dict(starts=fake(12)), "query starts buffer is too small"),
