@@ -11,8 +11,8 @@
 //
 // One workgroup owns the new rows of one (sequence, page, KV head, keys or values):
 // it needs the largest magnitude of all of them before it can write the first code,
-// so it holds them in registers (8 waves, one row at a time each, up to 16 rows a
-// wave), and no second pass or launch is needed.  The codes go through LDS, from
+// so it holds them in registers (up to 8 rows a wave of 16), and no second pass or launch
+// is needed.  The codes go through LDS, from
 // which they leave in the layout of the pages: rows for keys, runs of eight tokens a
 // dimension for values.  The query heads are further workgroups of the same launch,
 // a wave per token and run of heads.
@@ -27,9 +27,6 @@
 
 namespace kraken {
 namespace {
-
-constexpr int kWaves = 8;
-constexpr uint32_t kThreads = 64 * kWaves;
 
 // The rotation of elements lane + 64 i below n_dims: turns per position (the angle
 // over 2 pi, in double, so that a position of any size keeps its fraction), and the
@@ -67,7 +64,8 @@ __device__ __forceinline__ void sin_cos_of(const PagedPrologueArgs& a, const Rot
     const uint32_t e = lane + 64u * i;
     if (e < a.n_dims) {
       const int32_t p = a.positions != nullptr
-                          ? a.positions[token + (size_t)a.batch.tokens * rot.row[i]]
+                          ? a.positions[min(token, a.batch.tokens - 1u) +
+                                        (size_t)a.batch.tokens * rot.row[i]]
                           : (int32_t)position;
       const double t = (double)p * rot.turns[i];
       sincospif((float)(2.0 * (t - rint(t))), &sn[i], &cs[i]);
@@ -113,9 +111,29 @@ __device__ __forceinline__ void norm_rotate(const float v_in[4], const float w[4
   }
 }
 
-// A wave: one token's query heads [first, last).
+// A wave: kHeads query heads of one token from `first` on.
+template <int kHeads>
 __device__ __forceinline__ void query_heads(const PagedPrologueArgs& a, uint32_t token,
-                                            uint32_t first, uint32_t last, int lane) {
+                                            uint32_t first, int lane) {
+  const uint32_t d_head = a.cache.head_dim;
+  // Every load first; past the last head, its own again.
+  float v[kHeads][4], g[kHeads][4], w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t d = lane + 64u * i;
+    w[i] = d < d_head ? a.q_norm[d] : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    const uint32_t head = min(first + k, a.heads - 1u);
+    const float* src = a.q_gate + ((size_t)token * a.heads + head) * 2u * d_head;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t d = lane + 64u * i;
+      v[k][i] = d < d_head ? src[d] : 0.0f;
+      g[k][i] = d < d_head ? src[d_head + d] : 0.0f;
+    }
+  }
   const PagedSequence s = paged_row(a.batch, token, a.cache.page_shift).sequence;
   if (s.count == 0) {
     return;
@@ -123,20 +141,20 @@ __device__ __forceinline__ void query_heads(const PagedPrologueArgs& a, uint32_t
   const Rotation rot = rotation_of(a, lane);
   float sn[4], cs[4];
   sin_cos_of(a, rot, token, s.length - s.count + (token - s.start), lane, sn, cs);
-  const uint32_t d_head = a.cache.head_dim;
-  for (uint32_t head = first; head < last; ++head) {
-    const float* src = a.q_gate + ((size_t)token * a.heads + head) * 2u * d_head;
-    float v[4], w[4], r[4];
-    load_head(src, a.q_norm, d_head, lane, v, w);
-    norm_rotate(v, w, d_head, a.eps, a.n_dims, sn, cs, lane, r);
-    float* q_out = a.query_out + ((size_t)token * a.heads + head) * d_head;
-    float* g_out = a.gate_out + ((size_t)token * a.heads + head) * d_head;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t d = lane + 64u * i;
-      if (d < d_head) {
-        q_out[d] = r[i];
-        g_out[d] = src[d_head + d];
+  for (int k = 0; k < kHeads; ++k) {
+    float r[4];
+    norm_rotate(v[k], w, d_head, a.eps, a.n_dims, sn, cs, lane, r);
+    if (first + k < a.heads) {
+      float* q_out = a.query_out + ((size_t)token * a.heads + first + k) * d_head;
+      float* g_out = a.gate_out + ((size_t)token * a.heads + first + k) * d_head;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t d = lane + 64u * i;
+        if (d < d_head) {
+          q_out[d] = r[i];
+          g_out[d] = g[k][i];
+        }
       }
     }
   }
@@ -171,20 +189,30 @@ __device__ __forceinline__ void grow_scale(uint32_t largest_bits, float old_scal
 
 // A page's new rows [first, last) (slots of the page), row `row` + slot - first of
 // the batch; kRows rows a wave.
-template <int kRows>
+template <int kRows, int kWaves>
 __device__ __forceinline__ void page_rows(const PagedPrologueArgs& a, bool is_value, uint32_t page,
                                           uint32_t kv_head, uint32_t first, uint32_t last,
                                           uint32_t row, uint32_t position, int8_t* codes,
                                           uint32_t* wave_largest) {
+  constexpr uint32_t kThreads = 64 * kWaves;
   const int lane = threadIdx.x & 63;
   const uint32_t wave = threadIdx.x >> 6;
   const uint32_t d_head = a.cache.head_dim;
   const uint32_t rows = last - first;
+  const uint32_t page_tokens = 1u << a.cache.page_shift;
   const size_t kv_dim = (size_t)a.cache.kv_heads * d_head;
   const float* src = (is_value ? a.value : a.key) + (size_t)row * kv_dim + (size_t)kv_head * d_head;
   const size_t page_head = (size_t)page * a.cache.kv_heads + kv_head;
   float* scale_at = (is_value ? a.cache.value_scales : a.cache.key_scales) + page_head;
   const float old_scale = *scale_at;
+  int8_t* out = (is_value ? a.cache.values : a.cache.keys) + page_head * page_tokens * d_head;
+  // The eight tokens of a dimension that this thread will write first, should some of them
+  // be older ones; asked for here so that they arrive with the rows.
+  uint64_t early = 0;
+  if (is_value && first % 8u != 0 && threadIdx.x < d_head) {
+    early = *reinterpret_cast<const uint64_t*>(
+      out + ((size_t)(first / 8u) * d_head + threadIdx.x) * 8u);
+  }
 
   float r[kRows][4];
 #pragma unroll
@@ -206,15 +234,14 @@ __device__ __forceinline__ void page_rows(const PagedPrologueArgs& a, bool is_va
     const Rotation rot = rotation_of(a, lane);
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
+      // (Past the last row: of zeros.)
       const uint32_t at = wave + kWaves * k;
-      if (at < rows) {  // whole wave
-        float sn[4], cs[4], out[4];
-        sin_cos_of(a, rot, row + at, position + at, lane, sn, cs);
-        norm_rotate(r[k], w, d_head, a.eps, a.n_dims, sn, cs, lane, out);
+      float sn[4], cs[4], turned[4];
+      sin_cos_of(a, rot, row + at, position + at, lane, sn, cs);
+      norm_rotate(r[k], w, d_head, a.eps, a.n_dims, sn, cs, lane, turned);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          r[k][i] = out[i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        r[k][i] = turned[i];
       }
     }
   }
@@ -265,8 +292,6 @@ __device__ __forceinline__ void page_rows(const PagedPrologueArgs& a, bool is_va
 
   // Older codes change where the scale grew.
   const uint32_t older = factor == 1.0f ? 0u : first;
-  const uint32_t page_tokens = 1u << a.cache.page_shift;
-  int8_t* out = (is_value ? a.cache.values : a.cache.keys) + page_head * page_tokens * d_head;
   auto shrink = [&](int8_t c) { return (int8_t)(int)rintf((float)c * factor); };
   if (!is_value) {
     // 16 bytes of a row at a time.
@@ -295,7 +320,11 @@ __device__ __forceinline__ void page_rows(const PagedPrologueArgs& a, bool is_va
       const uint32_t octet = from + i / d_head, d = i % d_head;
       uint64_t* at = reinterpret_cast<uint64_t*>(out + ((size_t)octet * d_head + d) * 8u);
       const bool whole = octet * 8u >= first && octet * 8u + 8u <= last;
-      uint64_t held = whole ? 0u : *at;
+      uint64_t held = 0;
+      if (!whole) {
+        // (i is the dimension in the first run of them.)
+        held = i < d_head && octet == first / 8u && first % 8u != 0 ? early : *at;
+      }
       uint64_t made = 0;
 #pragma unroll
       for (uint32_t k = 0; k < 8; ++k) {
@@ -314,13 +343,12 @@ __device__ __forceinline__ void page_rows(const PagedPrologueArgs& a, bool is_va
 }
 
 // Blocks [0, page_blocks): the new rows of a page for one KV head, keys or values.
-// The rest: query heads, a wave per token and run of heads_per_wave of them.  Both
+// The rest: query heads, a wave per token and run of kHeads of them.  Both
 // walk their items in steps of their blocks, whose number is bounded.
-template <int kRows>
-__global__ __launch_bounds__(kThreads) void prologue_paged_q8_kernel(PagedPrologueArgs a,
-                                                                     uint32_t spans,
-                                                                     uint32_t page_blocks,
-                                                                     uint32_t heads_per_wave) {
+template <int kRows, int kWaves, int kHeads>
+__global__ __launch_bounds__(64 * kWaves) void prologue_paged_q8_kernel(PagedPrologueArgs a,
+                                                                        uint32_t spans,
+                                                                        uint32_t page_blocks) {
   extern __shared__ __attribute__((aligned(16))) int8_t codes[];
   __shared__ uint32_t wave_largest[kWaves];
   if (blockIdx.x < page_blocks) {
@@ -344,20 +372,19 @@ __global__ __launch_bounds__(kThreads) void prologue_paged_q8_kernel(PagedProlog
         continue;
       }
       __syncthreads();  // the last item's codes have left LDS
-      page_rows<kRows>(a, kind & 1u, (uint32_t)page, kind >> 1, first - (uint32_t)page_begin,
+      page_rows<kRows, kWaves>(a, kind & 1u, (uint32_t)page, kind >> 1, first - (uint32_t)page_begin,
                        last - (uint32_t)page_begin, s.start + (first - begin), first, codes,
                        wave_largest);
     }
     return;
   }
-  const uint32_t groups = (a.heads + heads_per_wave - 1u) / heads_per_wave;
+  const uint32_t groups = (a.heads + kHeads - 1u) / kHeads;
   const uint64_t items = (uint64_t)a.batch.tokens * groups;
   const uint64_t stride = (uint64_t)(gridDim.x - page_blocks) * kWaves;
   for (uint64_t item = (uint64_t)(blockIdx.x - page_blocks) * kWaves + (threadIdx.x >> 6);
        item < items; item += stride) {
-    const uint32_t first = (uint32_t)(item % groups) * heads_per_wave;
-    query_heads(a, (uint32_t)(item / groups), first, min(first + heads_per_wave, a.heads),
-                threadIdx.x & 63);
+    query_heads<kHeads>(a, (uint32_t)(item / groups), (uint32_t)(item % groups) * kHeads,
+                        threadIdx.x & 63);
   }
 }
 
@@ -401,29 +428,41 @@ __global__ __launch_bounds__(256) void dequantize_pages_q8_kernel(PagedQ8Args c,
 
 }  // namespace
 
-hipError_t launch_prologue_paged_q8(const PagedPrologueArgs& a, hipStream_t stream) {
+namespace {
+
+template <int kRows, int kWaves, int kHeads>
+void launch_prologue(const PagedPrologueArgs& a, uint32_t rows, hipStream_t stream) {
   const uint32_t page_tokens = 1u << a.cache.page_shift;
   // Pages that max_query new tokens can reach into.
   const uint64_t spans = (a.batch.max_query + (uint64_t)page_tokens - 2u) / page_tokens + 1u;
   const uint64_t page_blocks =
     std::min<uint64_t>((uint64_t)a.batch.sequences * spans * a.cache.kv_heads * 2u, 1u << 20);
-  const uint32_t heads_per_wave = a.batch.tokens >= 256u ? 4u : 1u;
-  const uint64_t groups = (a.heads + heads_per_wave - 1u) / heads_per_wave;
+  const uint64_t groups = (a.heads + kHeads - 1u) / kHeads;
   const uint64_t blocks =
     page_blocks +
     std::min<uint64_t>((a.batch.tokens * groups + kWaves - 1u) / kWaves, 1u << 20);
-  const uint32_t rows = std::min(page_tokens, a.batch.max_query);
-  const uint32_t lds = rows * a.cache.head_dim;
-  const dim3 grid((uint32_t)blocks);
-  if (rows <= 16u) {
-    prologue_paged_q8_kernel<2><<<grid, kThreads, lds, stream>>>(
-      a, (uint32_t)spans, (uint32_t)page_blocks, heads_per_wave);
+  prologue_paged_q8_kernel<kRows, kWaves, kHeads>
+    <<<dim3((uint32_t)blocks), 64 * kWaves, rows * a.cache.head_dim, stream>>>(
+      a, (uint32_t)spans, (uint32_t)page_blocks);
+}
+
+}  // namespace
+
+hipError_t launch_prologue_paged_q8(const PagedPrologueArgs& a, hipStream_t stream) {
+  const uint32_t rows = std::min(1u << a.cache.page_shift, a.batch.max_query);
+  // A decode step: small workgroups, a wave a row and a query head.  Chunks: 16 waves on
+  // the rows of a page, whose time is theirs one after another, and four query heads a
+  // wave, which share the token's angles (us, with the pages read back: 1 token 11.0 with
+  // 8 waves, 10.7 with 4; 64 tokens 14.6 and 12.2; 1024 tokens 31.9 with 8 waves and
+  // heads one by one, 23.0 with 16 and three at once, 20.1 four).
+  if (rows <= 4u) {
+    launch_prologue<1, 4, 1>(a, rows, stream);
+  } else if (rows <= 16u) {
+    launch_prologue<1, 16, 4>(a, rows, stream);
   } else if (rows <= 64u) {
-    prologue_paged_q8_kernel<8><<<grid, kThreads, lds, stream>>>(
-      a, (uint32_t)spans, (uint32_t)page_blocks, heads_per_wave);
+    launch_prologue<4, 16, 4>(a, rows, stream);
   } else {
-    prologue_paged_q8_kernel<16><<<grid, kThreads, lds, stream>>>(
-      a, (uint32_t)spans, (uint32_t)page_blocks, heads_per_wave);
+    launch_prologue<8, 16, 2>(a, rows, stream);
   }
   return hipGetLastError();
 }
