@@ -16,8 +16,9 @@
 //   gather  the histogram says which bins a threshold can lie in (one, or a few where
 //           top-p depends on a top-k that is not resolved yet); their elements go to a
 //           list, and what lies above them is summed by chunk from the chunk's bins
-//   draw    one workgroup a row: the threshold by radix selection in the list, then the
-//           chunk in which the draw falls, and the token by a scan of that chunk alone.
+//   draw    one workgroup a row: the threshold in the list (each entry against each in a
+//           short one, by radix selection in a long one), then the chunk in which the draw falls, and the token by a scan
+//           of that chunk alone.
 // So a row is read three times, from memory once (the rest from the caches), and its
 // exponentials are formed once.
 #include <hip/hip_runtime.h>
@@ -80,25 +81,30 @@ __device__ __forceinline__ bool takes_top(const RowRule& rule, uint32_t top) {
   return rule.greedy || rule.min_p > 1.0 || top <= kMinusInfKey;
 }
 
-// A row's weights: exp((l - max) / T) 2^shift as an integer.
+// A row's weights: exp((l - max) / T) 2^shift as an integer, and the bins that they fall
+// into.
 struct Weights {
-  uint32_t top;
-  double top_logit, factor;  // of log2(e) / T
+  float top;              // the largest logit
+  double top_wide, factor;  // factor: log2(e) / T
+  float scale;            // 8 log2(e) / T
+  double one;             // 2^shift
   int shift;
 };
 
 __device__ __forceinline__ Weights weights_of(uint32_t top, const RowRule& rule, int shift) {
-  return {top, (double)logit_of(top), 1.4426950408889634074 * rule.inverse_temperature, shift};
+  const float logit = logit_of(top);
+  const double factor = 1.4426950408889634074 * rule.inverse_temperature;
+  return {logit, (double)logit, factor, (float)(8.0 * factor), ldexp(1.0, shift), shift};
 }
 
-// 2^y for y <= 0 (0 from -1000 down) times 2^shift: y = n + f with |f| <= 1/2, and the
-// Taylor series of e^(f ln 2), whose first term left out is (ln 2 / 2)^12 / 12! = 6e-15.
-__device__ __forceinline__ double exp2_scaled(double y, int shift) {
+// A logit's weight (not a NaN's), before rounding to a whole number: 2^y 2^shift with
+// y = n + f, |f| <= 1/2, by the Taylor series of e^(f ln 2), whose first term left out is
+// (ln 2 / 2)^10 / 10! = 7e-12.  Zero from y = -1000 down, and of -inf.
+__device__ __forceinline__ double weight_real(float logit, const Weights& w) {
+  const double y = ((double)logit - w.top_wide) * w.factor;
   const double n = rint(y);
   const double t = (y - n) * 0.69314718055994530942;
-  double r = 1.0 / 39916800.0;
-  r = fma(r, t, 1.0 / 3628800.0);
-  r = fma(r, t, 1.0 / 362880.0);
+  double r = 1.0 / 362880.0;
   r = fma(r, t, 1.0 / 40320.0);
   r = fma(r, t, 1.0 / 5040.0);
   r = fma(r, t, 1.0 / 720.0);
@@ -108,28 +114,25 @@ __device__ __forceinline__ double exp2_scaled(double y, int shift) {
   r = fma(r, t, 0.5);
   r = fma(r, t, 1.0);
   r = fma(r, t, 1.0);
-  return y > -1000.0 ? ldexp(r, (int)n + shift) : 0.0;
-}
-
-// In units of 2^-shift, before rounding to a whole number.
-__device__ __forceinline__ double weight_real(uint32_t key, const Weights& w) {
   // The largest logit may be infinite, and so may the factor.
-  return key == w.top ? ldexp(1.0, w.shift)
-         : key <= kMinusInfKey
-           ? 0.0
-           : exp2_scaled(((double)logit_of(key) - w.top_logit) * w.factor, w.shift);
+  return logit == w.top ? w.one : y > -1000.0 ? ldexp(r, (int)n + w.shift) : 0.0;
 }
 
-__device__ __forceinline__ uint64_t weight_fixed(uint32_t key, const Weights& w) {
+__device__ __forceinline__ uint64_t weight_fixed(float logit, const Weights& w) {
   // Up to 2^51, an addition of 2^52 leaves the rounded number in the low bits.
-  return (uint64_t)__double_as_longlong(weight_real(key, w) + 0x1p52) & ((uint64_t{1} << 52) - 1u);
+  return (uint64_t)__double_as_longlong(weight_real(logit, w) + 0x1p52) &
+         ((uint64_t{1} << 52) - 1u);
 }
 
-// The bin of a key: falling weights fall into rising bins (each step of it is
-// monotone).  `scale` is 8 log2(e) / T.
-__device__ __forceinline__ uint32_t bin_of(uint32_t key, uint32_t top, float scale) {
-  const float z = (logit_of(top) - logit_of(key)) * scale;
-  return key == top ? 0u : (uint32_t)fminf(z, (float)(kBins - 1u));  // NaN: the last
+// How many eighths of an octave a logit's weight lies below the largest, and its bin:
+// falling logits have rising bins (each step of it is monotone).  NaN only of a NaN.
+__device__ __forceinline__ float eighths_of(float logit, const Weights& w) {
+  const float z = (w.top - logit) * w.scale;
+  return logit == w.top ? 0.0f : logit != logit ? z : z >= 0.0f ? z : (float)kBins;
+}
+
+__device__ __forceinline__ uint32_t bin_of(float logit, const Weights& w) {
+  return (uint32_t)fminf(eighths_of(logit, w), (float)(kBins - 1u));
 }
 
 // Which bins a row's threshold can lie in, and the row's largest.
@@ -456,15 +459,13 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Pla
     return;
   }
   const Weights weights = weights_of(top, rule, p.shift);
-  const float scale = (float)(8.0 * weights.factor);
   const bool counted = rule.top_k != 0u;
   const uint32_t begin = chunk * p.chunk, end = min(a.size, begin + p.chunk);
   each_logit(a.logits + (size_t)row * a.row_stride, begin, end, [&](uint32_t, float x) {
-    const uint32_t key = key_of(x);
-    if (key != 0u) {
-      const uint32_t bin = bin_of(key, top, scale);
+    if (x == x) {
+      const uint32_t bin = bin_of(x, weights);
       atomicAdd((unsigned long long*)&bin_weight[bin],
-                (unsigned long long)weight_fixed(key, weights));
+                (unsigned long long)weight_fixed(x, weights));
       if (counted) {
         atomicAdd(&bin_count[bin], 1u);
       }
@@ -520,12 +521,13 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, P
   }
   const Weights weights = weights_of(top, rule, p.shift);
   if (last >= sure) {
-    const float scale = (float)(8.0 * weights.factor);
+    // Bins sure .. last, the last bin without an end.
+    const float from = (float)sure;
+    const float to = last < kBins - 1u ? (float)(last + 1u) : INFINITY;
     const uint32_t begin = chunk * p.chunk, end = min(a.size, begin + p.chunk);
     each_logit(a.logits + (size_t)row * a.row_stride, begin, end, [&](uint32_t i, float x) {
-      const uint32_t key = key_of(x);
-      const uint32_t bin = bin_of(key, top, scale);
-      if (key != 0u && bin >= sure && bin <= last) {
+      const float z = eighths_of(x, weights);
+      if (z >= from && (z < to || to == INFINITY)) {
         found[atomicAdd(&founds, 1u)] = i;
       }
     });
@@ -535,8 +537,8 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, P
   const uint32_t n = founds;
   for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
     const uint32_t index = found[i];
-    const uint32_t key = key_of(a.logits[(size_t)row * a.row_stride + index]);
-    w.list[(size_t)chunk * p.chunk + i] = {index, key, weight_fixed(key, weights)};
+    const float x = a.logits[(size_t)row * a.row_stride + index];
+    w.list[(size_t)chunk * p.chunk + i] = {index, key_of(x), weight_fixed(x, weights)};
   }
   if (threadIdx.x == 0) {
     w.chunk_listed[chunk] = n;
@@ -551,6 +553,9 @@ struct Cut {
   }
 };
 
+// A list this short is looked at entry against entry (8 rows of 32000: 29.5 us; by radix
+// selection, or up to 256 entries this way, 31.1 and 30.0 us).
+constexpr uint32_t kDirect = 128;
 constexpr uint32_t kDigits = 1024;  // of a step of the radix selection
 
 struct DrawScratch {
@@ -562,6 +567,7 @@ struct DrawScratch {
   uint32_t wave_counts[kDrawThreads / 64u];
   uint64_t found_weight;
   uint32_t found, found_count, found_here;
+  uint32_t cut_key, cut_index;
 };
 
 // The entries of the list: in LDS, or (a row whose threshold has more than kHeld logits
@@ -737,11 +743,50 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
       low = min(low, key);
     });
   }
-  e.high = (uint32_t)block_reduce<kWaves>(high, Largest{}, s.sums);
-  e.low = ~(uint32_t)block_reduce<kWaves>((uint32_t)~low, Largest{}, s.sums);
-
   Cut cut{0u, 0xffffffffu};
-  if (b.cut != 0u && all_n != 0u) {
+  if (b.cut != 0u && all_n != 0u && all_n <= kDirect) {
+    // A short list: what lies before each entry, by looking at all others.
+    constexpr uint32_t kShare = kDrawThreads / kDirect;
+    __syncthreads();
+    const uint32_t i = threadIdx.x / kShare;
+    const bool real = i < all_n;
+    const Entry own = s.held[real ? i : 0u];
+    uint64_t before = 0;
+    uint32_t place = 0;
+    for (uint32_t j = threadIdx.x % kShare; j < all_n; j += kShare) {
+      const Entry other = s.held[j];
+      const bool first =
+        other.key > own.key || (other.key == own.key && other.index < own.index);
+      before += first ? other.weight : 0u;
+      place += first ? 1u : 0u;
+    }
+#pragma unroll
+    for (uint32_t step = 1; step < kShare; step *= 2u) {
+      before += (uint64_t)__shfl_xor((long long)before, (int)step, 64);
+      place += (uint32_t)__shfl_xor((int)place, (int)step, 64);
+    }
+    before += b.above;
+    const uint64_t upto = before + own.weight;
+    // The entries that top-k leaves, and the sum that top-p is of.
+    const uint32_t left = rule.top_k != 0u ? min(rule.top_k - b.above_n, all_n) : all_n;
+    if (real && place + 1u == left) {
+      s.found_weight = upto;
+    }
+    __syncthreads();
+    const uint64_t whole = rule.top_k != 0u ? s.found_weight : b.total;
+    const double target = rule.top_p < 1.0 ? rule.top_p * (double)whole : (double)INFINITY;
+    // An entry is kept where less than the target lies before it, and the first always;
+    // the threshold is the last one kept.
+    const bool kept = place == 0u || (double)before < target;
+    if (real && place < left && kept && (place + 1u == left || !((double)upto < target))) {
+      s.cut_key = own.key;
+      s.cut_index = own.index;
+    }
+    __syncthreads();
+    cut = {s.cut_key, s.cut_index};
+  } else if (b.cut != 0u && all_n != 0u) {
+    e.high = (uint32_t)block_reduce<kWaves>(high, Largest{}, s.sums);
+    e.low = ~(uint32_t)block_reduce<kWaves>((uint32_t)~low, Largest{}, s.sums);
     // The threshold's ties: all, or the first few by index.
     auto ties = [&](uint32_t key, uint32_t keep, uint32_t here) {
       cut.key = key;
@@ -790,7 +835,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
         },
         before, before_n, here, s);
       // The i-th tie is kept where before + i w < target.
-      const uint64_t each = weight_fixed(key, weights);
+      const uint64_t each = weight_fixed(logit_of(key), weights);
       uint32_t keep = here;
       if (each != 0u) {
         const double need = ceil((target - (double)before) / (double)each);
@@ -806,7 +851,8 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
 
   // Each chunk's kept weight.
   auto above_min = [&](uint32_t key) {
-    return rule.min_p == 0.0 || weight_real(key, weights) >= ldexp(rule.min_p, p.shift);
+    return rule.min_p == 0.0 ||
+           weight_real(logit_of(key), weights) >= ldexp(rule.min_p, p.shift);
   };
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < p.chunks; i += kDrawThreads) {
@@ -859,7 +905,6 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
   }
   // The chunk's logits, kPer a thread.
   constexpr uint32_t kPer = kMaxChunk / kDrawThreads;
-  const float scale = (float)(8.0 * weights.factor);
   const uint32_t begin = chunk * p.chunk + kPer * threadIdx.x;
   const uint32_t end = min(size, (chunk + 1u) * p.chunk);
   uint64_t kept[kPer], sum = 0, rest;
@@ -867,11 +912,10 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
   for (uint32_t j = 0; j < kPer; ++j) {
     kept[j] = 0;
     const uint32_t i = begin + j;
-    if (i < end) {
-      const uint32_t key = key_of(logits[i]);
-      const uint32_t bin = bin_of(key, top, scale);
-      if (key != 0u && (bin < b.sure || (bin <= b.last && cut.keeps(key, i) && above_min(key)))) {
-        kept[j] = weight_fixed(key, weights);
+    if (i < end && logits[i] == logits[i]) {
+      const uint32_t key = key_of(logits[i]), bin = bin_of(logits[i], weights);
+      if (bin < b.sure || (bin <= b.last && cut.keeps(key, i) && above_min(key))) {
+        kept[j] = weight_fixed(logits[i], weights);
       }
     }
     sum += kept[j];
@@ -896,7 +940,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     a.tokens[row] = (int32_t)token;
     if (a.probabilities != nullptr) {
       a.probabilities[row] =
-        (float)(weight_real(key_of(logits[token]), weights) / (double)total);
+        (float)(weight_real(logits[token], weights) / (double)total);
     }
   }
 }
