@@ -382,16 +382,16 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
     o = split.tile_o;
     ml = split.tile_ml;
   }
-  // This wave's parts are part0, part0 + kParts, ..; eight at a time, whose loads go out
+  // This wave's parts are part0, part0 + kParts, ..; four at a time, whose loads go out
   // together (past the last they repeat it, with weight 0).  Each wave keeps a maximum of
   // its own.
   const uint32_t part0 = kParts > 1 ? wave : 0u;
   float m = kLowestMax, l = 0.0f, x[kRegs] = {};
-  for (uint32_t at = part0; at < parts; at += 8u * kParts) {
-    float2 here[8];
-    float sums[8][kRegs];
+  for (uint32_t at = part0; at < parts; at += 4u * kParts) {
+    float2 here[4];
+    float sums[4][kRegs];
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
+    for (uint32_t j = 0; j < 4; ++j) {
       const size_t i = first + min(at + j * kParts, parts - 1u) * stride;
       here[j] = *reinterpret_cast<const float2*>(&ml[2 * i]);
 #pragma unroll
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
     }
     float up = m;
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
+    for (uint32_t j = 0; j < 4; ++j) {
       up = fmaxf(up, here[j].x);
     }
     const float keep = fast_exp2(m - up);
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
       x[r] *= keep;
     }
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
+    for (uint32_t j = 0; j < 4; ++j) {
       const float w = at + j * kParts < parts ? fast_exp2(here[j].x - m) : 0.0f;
       l = fmaf(w, here[j].y, l);
 #pragma unroll
@@ -483,8 +483,8 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
   // The tiled kernel's keys in parts until there are as many workgroups as the CUs hold
   // (one of head_dim 256, two of less), or four times as many where sequences of several
-  // lengths share the device (17 of up to 4200 keys: 87 us with twice, 84 with four
-  // times), each of 128 keys at least, and while their results take no more than 256 MiB.
+  // lengths share the device (17 of up to 4200 keys: 78 us with twice, 58 with four
+  // times, 66 with seven), each of 128 keys at least, and while their results take no more than 256 MiB.
   const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows * a.cache.kv_heads;
   const uint64_t all_tiles =
     std::min<uint64_t>(tiles * a.batch.sequences,
@@ -535,9 +535,10 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
   const uint64_t items = (uint64_t)a.batch.tokens * a.heads;
   const uint32_t parts = std::max(split.decode_most != 0u ? split.decode_splits : 1u,
                                   rows > kDecodeRows ? split.tile_splits : 1u);
-  // Four waves a row where there are many parts (one row of 33 parts 7.3 -> 4 us), and not
-  // more rows than a grid holds of them.
-  if (parts > 8u && items <= (uint64_t{1} << 22)) {
+  // Four waves a row where there are many parts and few rows (one row of 33 parts 7.3 -> 4
+  // us), one where the rows alone fill the device (14544 rows, most of four parts or fewer:
+  // 18.6 us with four, 9.0 with one).
+  if (parts > 8u && items <= 4096u) {
     attention_paged_join_kernel<D, T, 4><<<dim3((uint32_t)items), 256, 0, stream>>>(a, split);
   } else if (parts > 1u) {
     attention_paged_join_kernel<D, T, 1><<<dim3((uint32_t)((items + 3u) / 4u)), 256, 0, stream>>>(

@@ -2,8 +2,7 @@
 // rows (chunks of prompts).  The arithmetic is described in
 // attention_paged_q8_common.hpp.
 //
-// A workgroup takes 128 or 256 rows (token x query head) of one KV head of one sequence,
-// 32 a wave, and a run of its keys, a tile of kKeys at a time.  The next tile's codes are on
+// A workgroup takes 128 rows (token x query head) of one KV head of one sequence, 32 a wave, and a run of its keys, a tile of kKeys at a time.  The next tile's codes are on
 // their way into registers while a tile is multiplied; they become f16 as they go into
 // LDS, once for all waves.  Both products are transposed, S^T = K Q^T and
 // O^T += V^T P^T (32x32x16), so that a query row is a lane: its maximum and sum are
