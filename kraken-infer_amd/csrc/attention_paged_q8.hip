@@ -361,7 +361,9 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
   const PagedSequence s = found.sequence;
   const uint32_t group = a.heads / a.cache.kv_heads;
   const bool decode = s.count * group <= split.decode_most;
-  const uint32_t per = decode ? split.decode_keys : split.tile_keys;
+  const uint32_t per = decode                  ? split.decode_keys
+                       : split.tile_step != 0u ? *split.tile_chosen
+                                               : split.tile_keys;
   if (s.count == 0 || s.length <= per) {
     return;  // of no sequence, or written by its workgroup
   }
@@ -481,10 +483,14 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   s.decode_keys = (uint32_t)keys;
   s.decode_rows = (uint32_t)std::min<uint64_t>(rows, kDecodeRows);
   s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
-  // The tiled kernel's keys in parts until there are as many workgroups as the CUs hold
-  // (one of head_dim 256, two of less), or four times as many where sequences of several
-  // lengths share the device (17 of up to 4200 keys: 78 us with twice, 58 with four
-  // times, 66 with seven), each of 128 keys at least, and while their results take no more than 256 MiB.
+  // The tiled kernel's keys in parts, of 128 keys at least, so that there is one for each
+  // workgroup that the CUs hold at a time (one of head_dim 256, two of less), while the
+  // results take no more than 256 MiB.  (One sequence, 37 rows at 6181 keys: KVTAIL.)
+  // Sequences of several lengths share the device ill in parts of one host-chosen size,
+  // since the host has only the largest length: where one more workgroup than fits makes
+  // a second round, 17 sequences took 71 us with 512 keys and 58 with 576.  So the kernel
+  // itself chooses among sizes from an eighth of a round's upward.  Of more than 64
+  // sequences, which make rounds enough, a quarter of a round's.
   const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows * a.cache.kv_heads;
   const uint64_t all_tiles =
     std::min<uint64_t>(tiles * a.batch.sequences,
@@ -493,15 +499,21 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
                          (uint64_t)a.batch.sequences * a.cache.kv_heads);
   const uint64_t row_bytes =
     (uint64_t)a.batch.tokens * a.heads * (a.cache.head_dim + 2u) * sizeof(float);
-  uint64_t splits = 1;
-  const uint64_t enough = (a.cache.head_dim == 256u ? 1u : 2u) *
-                          (a.batch.sequences > 1u ? 4u : 1u) * (uint64_t)cu_count;
-  while (rows > kDecodeRows && all_tiles * splits < enough &&
-         a.batch.max_keys / (2u * splits) >= 128u &&
-         2u * splits * row_bytes <= (uint64_t{256} << 20)) {
-    splits *= 2u;
+  const bool chooses = a.batch.sequences > 1u && a.batch.sequences <= 64u;
+  s.tile_slots = (a.cache.head_dim == 256u ? 1u : 2u) * (uint32_t)cu_count;
+  const uint64_t rounds = a.batch.sequences == 1u ? 1u : chooses ? 8u : 4u;
+  uint64_t tile_keys = (a.batch.max_keys * all_tiles + rounds * s.tile_slots - 1u) /
+                       (rounds * s.tile_slots);
+  tile_keys = rows <= kDecodeRows ? a.batch.max_keys : std::max<uint64_t>(tile_keys, 128u);
+  tile_keys = (std::min<uint64_t>(tile_keys, a.batch.max_keys) + 63u) / 64u * 64u;
+  while (tile_keys < a.batch.max_keys &&
+         (a.batch.max_keys + tile_keys - 1u) / tile_keys * row_bytes > (uint64_t{256} << 20)) {
+    tile_keys *= 2u;
   }
-  s.tile_keys = (uint32_t)((a.batch.max_keys + splits - 1u) / splits + 63u) & ~63u;
+  s.tile_keys = (uint32_t)tile_keys;
+  s.tile_step = chooses && tile_keys < a.batch.max_keys
+                  ? std::max(64u, (s.tile_keys / 4u + 63u) / 64u * 64u)
+                  : 0u;
   s.tile_splits = (uint32_t)((a.batch.max_keys + s.tile_keys - 1u) / s.tile_keys);
   s.tile_blocks = (uint32_t)(all_tiles * s.tile_splits);
   return s;
@@ -561,7 +573,8 @@ void launch_type(const PagedAttentionArgs& a, const PagedSplit& split, hipStream
 
 size_t attention_paged_q8_workspace_bytes(const PagedAttentionArgs& a, int cu_count) {
   const PagedSplit s = split_of(a, cu_count);
-  return (decode_parts(a, s) + tile_parts(a, s)) * (a.cache.head_dim + 2u) * sizeof(float);
+  return (decode_parts(a, s) + tile_parts(a, s)) * (a.cache.head_dim + 2u) * sizeof(float) +
+         sizeof(uint32_t);
 }
 
 hipError_t launch_attention_paged_q8(const PagedAttentionArgs& a, int cu_count, void* workspace,
@@ -571,6 +584,7 @@ hipError_t launch_attention_paged_q8(const PagedAttentionArgs& a, int cu_count, 
   s.tile_o = s.decode_o + decode_parts(a, s) * a.cache.head_dim;
   s.decode_ml = s.tile_o + tile_parts(a, s) * a.cache.head_dim;
   s.tile_ml = s.decode_ml + decode_parts(a, s) * 2u;
+  s.tile_chosen = reinterpret_cast<uint32_t*>(s.tile_ml + tile_parts(a, s) * 2u);
   if (a.f16) {
     launch_type<half_t>(a, s, stream);
   } else {

@@ -48,13 +48,16 @@ struct PagedSplit {
   uint32_t decode_keys;   // keys per workgroup of the decode kernel
   uint32_t decode_rows;   // rows held per (split, sequence, KV head)
   uint32_t decode_splits;
-  uint32_t tile_keys;     // keys per workgroup of the tiled kernel
+  uint32_t tile_keys;     // keys per workgroup of the tiled kernel, the least if it chooses
+  uint32_t tile_step;     // how far apart its choices are; 0: tile_keys it is
+  uint32_t tile_slots;    // its workgroups that run at once
   uint32_t tile_splits;
   uint32_t tile_blocks;   // its workgroups, as many as a batch can need
   float* decode_o;
   float* decode_ml;
   float* tile_o;
   float* tile_ml;
+  uint32_t* tile_chosen;  // the keys that it chose, for the join
 };
 
 // Four codes (one dword, two's complement) as f16.  0x64uu is 1024 + uu in f16, so a

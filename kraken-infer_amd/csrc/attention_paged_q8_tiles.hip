@@ -12,6 +12,7 @@
 // f16 parts: a second product with the same operand from LDS.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <utility>
 
 #include "attention_paged_q8_common.hpp"
@@ -33,10 +34,43 @@ __device__ __forceinline__ void static_for(F f) {
   static_for(f, std::make_integer_sequence<int, N>{});
 }
 
-// KEYS = 32 kSub keys a tile, 4 waves.
-template <int D, class T, int kSub, int kWavesPerSimd>
-__global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_kernel(
-  PagedAttentionArgs a, PagedSplit split) {
+// The keys of a workgroup, for up to 64 sequences: of sixteen sizes the one whose rounds
+// of `tile_slots` workgroups are soonest over, each round taking its keys and what a
+// workgroup spends besides (about 128 keys' time).  Every wave comes to the same.
+__device__ __forceinline__ uint32_t chosen_keys(const PagedAttentionArgs& a,
+                                                const PagedSplit& split, uint32_t group) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t tiles = 0, length = 0;
+  if (lane < a.batch.sequences) {
+    const PagedSequence s = paged_sequence(a.batch, lane, a.cache.page_shift);
+    const uint32_t rows = s.count * group;
+    tiles = rows > split.decode_most ? (rows + kTileRows - 1u) / kTileRows : 0u;
+    length = s.length;
+  }
+  uint32_t best = split.tile_keys;
+  float least = INFINITY;
+#pragma unroll
+  for (uint32_t i = 0; i < 16; ++i) {
+    const uint32_t keys = split.tile_keys + i * split.tile_step;
+    const uint32_t parts = (uint32_t)((float)(length + keys - 1u) / (float)keys);
+    const uint32_t all =
+      (uint32_t)__builtin_amdgcn_readlane((int)wave_prefix(tiles * parts), 63) *
+      a.cache.kv_heads;
+    const float rounds = ceilf((float)all / (float)split.tile_slots);
+    const float time = rounds * (float)(keys + 128u);
+    best = time < least ? keys : best;
+    least = fminf(time, least);
+  }
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)best);
+}
+
+// One part of `part_keys` keys of one tile of rows.  `again`: the workgroup has done
+// another before.
+template <int D, class T, int kSub>
+__device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a,
+                                                     const PagedSplit& split,
+                                                     const PagedItem& found, uint32_t kv_head,
+                                                     uint32_t part_keys, bool again) {
   constexpr bool kTwo = std::is_same<T, float>::value;
   constexpr int kKeys = 32 * kSub;
   constexpr int kStride = D + 8;                      // of a key row in LDS, in halves
@@ -53,31 +87,17 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   const uint32_t n = lane & 31u, h = lane >> 5;
   const uint32_t shift = a.cache.page_shift, kv_heads = a.cache.kv_heads;
   const uint32_t group = a.heads / kv_heads;
-  // The sequences' (tile, part) pairs one after another, so that no workgroup without
-  // work stands between two with; the parts of a tile side by side, so that an XCD, which
-  // gets every eighth workgroup, reads few parts of a sequence's keys.
-  const uint32_t kv_head = blockIdx.x % kv_heads;
-  const PagedItem found =
-    paged_item(a.batch, blockIdx.x / kv_heads, shift, [&](const PagedSequence& q) {
-      const uint32_t r = q.count * group;
-      return r > split.decode_most ? (r + kTileRows - 1u) / kTileRows *
-                                       ((q.length + split.tile_keys - 1u) / split.tile_keys)
-                                   : 0u;
-    });
   const PagedSequence s = found.sequence;
   const uint32_t sequence = found.index;
-  if (s.count == 0) {
-    return;
-  }
-  const uint32_t parts = (s.length + split.tile_keys - 1u) / split.tile_keys;
+  const uint32_t parts = (s.length + part_keys - 1u) / part_keys;
   const uint32_t tile = found.item / parts, part = found.item % parts;
   const uint32_t rows = s.count * group;
   const uint32_t first_row = tile * kTileRows;
   // The keys that the tile's last row sees, of this part.
   const uint32_t before = s.length - s.count;
   const uint32_t last_row = min(first_row + kTileRows, rows) - 1u;
-  const uint32_t begin = part * split.tile_keys;
-  const uint32_t end = min(before + last_row / group + 1u, begin + split.tile_keys);
+  const uint32_t begin = part * part_keys;
+  const uint32_t end = min(before + last_row / group + 1u, begin + part_keys);
   if (begin >= end) {
     return;
   }
@@ -202,6 +222,9 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
         }
       }
     }
+  }
+  if (again) {
+    __syncthreads();  // the tiles of the item before are read
   }
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
@@ -468,7 +491,7 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   }
   sum = xor32_sum(sum);
   // The key count of the sequence decides for all of its rows, as in the join.
-  const bool whole = s.length <= split.tile_keys;
+  const bool whole = s.length <= part_keys;
   const float inverse = inverse_sum(sum);
   const size_t item = (size_t)part * a.batch.tokens * a.heads + at / D;
 #pragma unroll
@@ -494,6 +517,37 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
   }
 }
 
+// A workgroup (4 waves, 32 kSub keys a tile) takes every gridDim.x-th of the sequences'
+// (tile, part) pairs, which stand one after another, so that no place without work stands
+// between two with; the parts of a tile side by side, so that an XCD, which gets every
+// eighth workgroup, reads few parts of a sequence's keys.
+template <int D, class T, int kSub, int kWavesPerSimd>
+__global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_kernel(
+  PagedAttentionArgs a, PagedSplit split) {
+  const uint32_t kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
+  uint32_t part_keys = split.tile_keys;
+  if (split.tile_step != 0u) {
+    part_keys = chosen_keys(a, split, group);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      *split.tile_chosen = part_keys;
+    }
+  }
+  for (uint32_t block = blockIdx.x;; block += gridDim.x) {
+    const PagedItem found =
+      paged_item(a.batch, block / kv_heads, a.cache.page_shift, [&](const PagedSequence& q) {
+        const uint32_t r = q.count * group;
+        return r > split.decode_most
+                 ? (r + kTileRows - 1u) / kTileRows * ((q.length + part_keys - 1u) / part_keys)
+                 : 0u;
+      });
+    if (found.sequence.count == 0) {
+      return;
+    }
+    attention_paged_tile<D, T, kSub>(a, split, found, block % kv_heads, part_keys,
+                                     block != blockIdx.x);
+  }
+}
+
 template <int D, class T>
 void launch_tiles(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
   // One wave a SIMD for head_dim 256, whose operands take its 512 registers.  64 keys a
@@ -502,8 +556,12 @@ void launch_tiles(const PagedAttentionArgs& a, const PagedSplit& split, hipStrea
   // head_dim 128: 119 us with 64 keys, 104 with 32).
   constexpr int kWavesPerSimd = D == 256 ? 1 : 2;
   constexpr int kSub = D == 64 || (D == 256 && !std::is_same<T, float>::value) ? 2 : 1;
+  // Two rounds of workgroups, which go on to further parts: of one for each part that a
+  // batch could have most find none (17 sequences, 4096 workgroups for 512 parts: 77 us,
+  // with 1024 61).  The loop costs 1 % where there is one part for each.
+  const uint32_t blocks = std::min(split.tile_blocks, 2u * split.tile_slots);
   attention_paged_tile_kernel<D, T, kSub, kWavesPerSimd>
-    <<<dim3(split.tile_blocks), kThreads, 0, stream>>>(a, split);
+    <<<dim3(blocks), kThreads, 0, stream>>>(a, split);
 }
 
 template <class T>
