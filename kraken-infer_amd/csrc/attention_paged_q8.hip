@@ -16,6 +16,11 @@
 //  - The f32 operands need two f16 parts.  Up to 8 rows fill only half of the 16
 //    columns, so the high parts take columns 0..7 and the low parts 8..15 of the same
 //    product (kStacked) and the halves are added; up to 16 rows take two products.
+//
+// 64 sequences of up to 32768 keys, 2 KV heads of 256 (1.07 GB): 191 us, 5.6 TB/s, of the
+// 6.95 that a read of as much reaches; the parts are of one size, so the last ones end
+// alone.  One of 4096 keys: 8.6 us and 3.9 for the join, launch and latency (lengths, table,
+// codes, exchange, one after another); its 4.2 MB would take 1.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -329,7 +334,8 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
       x = fmaf(keep, lds_o[(w * kRows + r) * kStride + d], x);
     }
     if (whole) {
-      const size_t out = ((size_t)(s.start + r / group) * a.heads + kv_head * group + r % group) * D;
+      const size_t out =
+        ((size_t)(s.start + r / group) * a.heads + kv_head * group + r % group) * D;
       store_output<T>(a, out + d, x, inverse_sum(l));
     } else {
       const size_t i = (((size_t)part * a.batch.sequences + sequence) * kv_heads + kv_head) *
@@ -478,19 +484,21 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   while (parts(keys) > lanes && parts(keys) * part_bytes > (uint64_t{256} << 20)) {
     keys *= 2u;
   }
+  // (A part of more keys than there are would only bring the sums of the two past 32 bits.)
+  keys = std::min(keys, (a.batch.max_keys + 127u) / 128u * uint64_t{128});
   // A single sequence with many rows needs no second kernel beside the tiled one.
   s.decode_most = rows <= kDecodeRows || a.batch.sequences > 1u ? kDecodeRows : 0u;
   s.decode_keys = (uint32_t)keys;
   s.decode_rows = (uint32_t)std::min<uint64_t>(rows, kDecodeRows);
   s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
-  // The tiled kernel's keys in parts, of 128 keys at least, so that there is one for each
+  // The tiled kernel's keys in parts of 128 at least, so that there is one for each
   // workgroup that the CUs hold at a time (one of head_dim 256, two of less), while the
-  // results take no more than 256 MiB.  (One sequence, 37 rows at 6181 keys: KVTAIL.)
-  // Sequences of several lengths share the device ill in parts of one host-chosen size,
-  // since the host has only the largest length: where one more workgroup than fits makes
-  // a second round, 17 sequences took 71 us with 512 keys and 58 with 576.  So the kernel
-  // itself chooses among sizes from an eighth of a round's upward.  Of more than 64
-  // sequences, which make rounds enough, a quarter of a round's.
+  // results take no more than 256 MiB (one sequence, 37 rows at 6181 keys: 33.7 us in 100
+  // parts, 31.7 in 196).  Sequences of several lengths are cut ill by the largest of them,
+  // which is all that the host has: where a few parts more than fit made a second round, 17
+  // sequences took 71 us in parts of 512 keys and 58 of 576.  So the kernel chooses among
+  // sizes from an eighth of a round's on; of more than 64 sequences, which make rounds
+  // enough, a quarter of a round's is taken.
   const uint64_t tiles = (rows + kTileRows - 1u) / kTileRows * a.cache.kv_heads;
   const uint64_t all_tiles =
     std::min<uint64_t>(tiles * a.batch.sequences,
@@ -505,14 +513,17 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   uint64_t tile_keys = (a.batch.max_keys * all_tiles + rounds * s.tile_slots - 1u) /
                        (rounds * s.tile_slots);
   tile_keys = rows <= kDecodeRows ? a.batch.max_keys : std::max<uint64_t>(tile_keys, 128u);
-  tile_keys = (std::min<uint64_t>(tile_keys, a.batch.max_keys) + 63u) / 64u * 64u;
+  tile_keys = (tile_keys + 63u) / 64u * 64u;
   while (tile_keys < a.batch.max_keys &&
          (a.batch.max_keys + tile_keys - 1u) / tile_keys * row_bytes > (uint64_t{256} << 20)) {
     tile_keys *= 2u;
   }
+  tile_keys = std::min(tile_keys, (a.batch.max_keys + 63u) / 64u * uint64_t{64});
   s.tile_keys = (uint32_t)tile_keys;
+  // (The largest choice, 15 steps on, stays below 2^31.)
   s.tile_step = chooses && tile_keys < a.batch.max_keys
-                  ? std::max(64u, (s.tile_keys / 4u + 63u) / 64u * 64u)
+                  ? std::min((s.tile_keys / 4u + 63u) / 64u * 64u,
+                             (0x7fffffffu - s.tile_keys) / 15u / 64u * 64u)
                   : 0u;
   s.tile_splits = (uint32_t)((a.batch.max_keys + s.tile_keys - 1u) / s.tile_keys);
   s.tile_blocks = (uint32_t)(all_tiles * s.tile_splits);

@@ -20,15 +20,16 @@ constexpr size_t kInt32Max = 0x7fffffffu;
 constexpr size_t kMaxPairs = size_t{1} << 20;
 constexpr size_t kMaxRows = size_t{1} << 26;
 
+int refuse(const char* w, const char* what) { return invalid(std::string("HIP ") + w + what); }
+
 // The cache's checks; `w` begins the messages.
 int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c) {
-  const std::string at(w);
   if (cache == nullptr) {
-    return invalid("HIP " + at + " cache must not be null");
+    return refuse(w, " cache must not be null");
   }
   if (cache->pages == 0 || cache->page_tokens == 0 || cache->kv_heads == 0 ||
       cache->head_dim == 0) {
-    return invalid("HIP " + at + " dimensions must be positive");
+    return refuse(w, " dimensions must be positive");
   }
   uint32_t shift = 0;
   switch (cache->page_tokens) {
@@ -36,29 +37,29 @@ int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c
     case 32: shift = 5; break;
     case 64: shift = 6; break;
     case 128: shift = 7; break;
-    default: return invalid("HIP " + at + " supports pages of 16/32/64/128 tokens");
+    default: return refuse(w, " supports pages of 16/32/64/128 tokens");
   }
   if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256) {
-    return invalid("HIP " + at + " supports head_dim 64/128/256");
+    return refuse(w, " supports head_dim 64/128/256");
   }
   if (cache->pages > kInt32Max) {
-    return invalid("HIP " + at + " page count exceeds int32 range");
+    return refuse(w, " page count exceeds int32 range");
   }
   size_t scales = 0, tokens = 0, bytes = 0;
   if (!checked_mul(cache->pages, cache->kv_heads, scales) ||
       !checked_mul(scales, cache->page_tokens, tokens) ||
       !checked_mul(tokens, cache->head_dim, bytes)) {
-    return invalid("HIP " + at + " value count overflow");
+    return refuse(w, " value count overflow");
   }
   KRAKEN_TRY(validate_buffer(cache->key_pages, bytes, 1u, w, " key pages"));
   KRAKEN_TRY(validate_buffer(cache->value_pages, bytes, 1u, w, " value pages"));
   KRAKEN_TRY(validate_f32(cache->key_scales, scales, w, " key scales"));
   KRAKEN_TRY(validate_f32(cache->value_scales, scales, w, " value scales"));
   if (((uintptr_t)cache->key_pages.data | (uintptr_t)cache->value_pages.data) & 15u) {
-    return invalid("HIP " + at + " pages must be 16-byte aligned");
+    return refuse(w, " pages must be 16-byte aligned");
   }
   if (cache->kv_heads > kMaxPairs) {
-    return invalid("HIP " + at + " takes up to 1048576 kv_heads");
+    return refuse(w, " takes up to 1048576 kv_heads");
   }
   c.keys = static_cast<int8_t*>(cache->key_pages.data);
   c.values = static_cast<int8_t*>(cache->value_pages.data);
@@ -73,23 +74,22 @@ int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c
 
 int batch_args(const kraken_paged_batch* batch, size_t kv_heads, const char* w,
                PagedBatchArgs& b) {
-  const std::string at(w);
   if (batch == nullptr) {
-    return invalid("HIP " + at + " batch must not be null");
+    return refuse(w, " batch must not be null");
   }
   if (batch->sequences == 0 || batch->table_width == 0 || batch->tokens == 0 ||
       batch->max_query == 0 || batch->max_keys == 0) {
-    return invalid("HIP " + at + " batch dimensions must be positive");
+    return refuse(w, " batch dimensions must be positive");
   }
   if (batch->tokens > kInt32Max || batch->max_keys > kInt32Max) {
-    return invalid("HIP " + at + " batch exceeds int32 range");
+    return refuse(w, " batch exceeds int32 range");
   }
   if (batch->sequences > kMaxPairs / kv_heads) {
-    return invalid("HIP " + at + " takes up to 1048576 pairs of a sequence and a KV head");
+    return refuse(w, " takes up to 1048576 pairs of a sequence and a KV head");
   }
   size_t entries = 0;
   if (!checked_mul(batch->sequences, batch->table_width, entries)) {
-    return invalid("HIP " + at + " value count overflow");
+    return refuse(w, " value count overflow");
   }
   KRAKEN_TRY(validate_buffer(batch->page_table, entries, sizeof(int32_t), w, " page table"));
   KRAKEN_TRY(validate_buffer(batch->query_starts, batch->sequences + 1u, sizeof(uint32_t), w,

@@ -12,10 +12,15 @@
 // One workgroup owns the new rows of one (sequence, page, KV head, keys or values):
 // it needs the largest magnitude of all of them before it can write the first code,
 // so it holds them in registers (up to 8 rows a wave of 16), and no second pass or launch
-// is needed.  The codes go through LDS, from
-// which they leave in the layout of the pages: rows for keys, runs of eight tokens a
-// dimension for values.  The query heads are further workgroups of the same launch,
-// a wave per token and run of heads.
+// is needed.  The codes go through LDS, from which they leave in the layout of the pages:
+// rows for keys, runs of eight tokens a dimension for values.  The query heads are further
+// workgroups of the same launch, a wave per token and run of heads.
+//
+// 1024 tokens of 8 query and 2 KV heads of 256 (35 MB with what is read and written, 5 us
+// at the rate of a stream) take 14.8 us: the page rows' chain of loads, norm, largest
+// magnitude and codes is as long for one page as for all, and 32 pages of 2 heads are 64
+// long workgroups.  One token takes 4.9 us, of which a launch is 2 to 3.  Reading the pages
+// back as F16 takes 5.9 us for 17 pages, 4.9 for one.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -372,9 +377,9 @@ __global__ __launch_bounds__(64 * kWaves) void prologue_paged_q8_kernel(PagedPro
         continue;
       }
       __syncthreads();  // the last item's codes have left LDS
-      page_rows<kRows, kWaves>(a, kind & 1u, (uint32_t)page, kind >> 1, first - (uint32_t)page_begin,
-                       last - (uint32_t)page_begin, s.start + (first - begin), first, codes,
-                       wave_largest);
+      page_rows<kRows, kWaves>(a, kind & 1u, (uint32_t)page, kind >> 1,
+                               first - (uint32_t)page_begin, last - (uint32_t)page_begin,
+                               s.start + (first - begin), first, codes, wave_largest);
     }
     return;
   }

@@ -6,8 +6,8 @@
 // Nothing is sorted.  Logits are ordered by 32-bit keys.  A weight w = exp((l - max) / T)
 // is formed in 64 bits and held as an integer of 2^-shift, with room for `size` of the
 // largest: the sums are exact whatever their order, so that atomics give one result, and
-// close enough to the real numbers (6e-11 of the largest weight over 250000 tokens) that
-// a cut or a draw falls on their side of a border.
+// close enough to the real numbers (for 250000 tokens each weight is within 2^-45 of the
+// largest and 7e-12 of itself) that a cut or a draw falls on their side of a border.
 //
 // Four launches, the first three with a workgroup for each chunk of a row:
 //   top     the largest key of the chunk and its first index
@@ -17,10 +17,20 @@
 //           top-p depends on a top-k that is not resolved yet); their elements go to a
 //           list, and what lies above them is summed by chunk from the chunk's bins
 //   draw    one workgroup a row: the threshold in the list (each entry against each in a
-//           short one, by radix selection in a long one), then the chunk in which the draw falls, and the token by a scan
-//           of that chunk alone.
-// So a row is read three times, from memory once (the rest from the caches), and its
-// exponentials are formed once.
+//           short one, by radix selection in a long one), then the chunk in which the
+//           draw falls, and the token by a scan of that chunk alone.
+// So a row is read three times, from memory once (the rest from the caches), and each
+// exponential is formed once but for those of the list and of the drawn chunk.
+//
+// 64 rows of 248320 take 12 + 31 + 17 + 23 us in the four, 78 us together, 8.5 times the
+// logits' way from memory.  top runs at 5.2 TB/s.  Of bins, the sums of all workgroups in
+// memory are 5 us, counts 3, the exponentials 5, and 18 reading and adding in LDS.
+// gather repeats the scan of the row's histogram in each workgroup.  draw is a chain of
+// some thirty barriers in one workgroup a row, and most of a small call's time (8 rows of
+// 32000: 20 of 28 us).  A launch costs 2 to 3 us, a release to the device within one
+// more (31 us instead of 6), so that no launch ends with its last workgroup's join.
+// Several chunks a workgroup, logits asked for ahead of the bounds, and short lists put
+// in order by a network were no faster.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -818,7 +828,9 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
       ties(key, rule.top_k - before_n, here);
       if (rule.top_p < 1.0) {
         uint64_t sum = 0;
-        e.each([&](uint32_t k, uint32_t index, uint64_t x) { sum += cut.keeps(k, index) ? x : 0u; });
+        e.each([&](uint32_t k, uint32_t index, uint64_t x) {
+          sum += cut.keeps(k, index) ? x : 0u;
+        });
         whole = b.above + block_reduce<kWaves>(sum, Sum{}, s.sums);
       }
     }
