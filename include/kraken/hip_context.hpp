@@ -835,6 +835,54 @@ class HipContext {
       ctx_, values.raw(), size, token_output.raw(), probability_output.raw()));
   }
 
+  // Batched serving over a paged 8-bit KV cache, and sampling (no MpsContext
+  // counterpart; see kraken_hip.h).  The cache and the batch are the C structs, filled
+  // with the buffers' raw() views.  positions, gate, the rules of sampling and
+  // probability_output may be invalid (default) buffers.
+  [[nodiscard]] Status qwen35_attention_prologue_paged_q8_kv(
+    const HipBuffer& q_gate, const HipBuffer& key, const HipBuffer& value,
+    const HipBuffer& q_norm, const HipBuffer& k_norm, const HipBuffer& positions,
+    const kraken_paged_q8_cache& cache, const kraken_paged_batch& batch, std::size_t heads,
+    std::size_t n_dims, std::size_t section_0, std::size_t section_1, std::size_t section_2,
+    std::size_t section_3, float theta, float eps, HipBuffer& query_out,
+    HipBuffer& gate_out) const {
+    return Status::from_code(kraken_hip_qwen35_attention_prologue_paged_q8_kv(
+      ctx_, q_gate.raw(), key.raw(), value.raw(), q_norm.raw(), k_norm.raw(), positions.raw(),
+      &cache, &batch, heads, n_dims, section_0, section_1, section_2, section_3, theta, eps,
+      query_out.raw(), gate_out.raw()));
+  }
+  [[nodiscard]] Status attention_f32_paged_q8_kv(const HipBuffer& query, const HipBuffer& gate,
+                                                 const kraken_paged_q8_cache& cache,
+                                                 const kraken_paged_batch& batch,
+                                                 std::size_t heads, HipBuffer& output) const {
+    return Status::from_code(kraken_hip_attention_f32_paged_q8_kv(
+      ctx_, query.raw(), gate.raw(), &cache, &batch, heads, output.raw()));
+  }
+  [[nodiscard]] Status attention_f16q_paged_q8_kv(const HipBuffer& query,
+                                                  const kraken_paged_q8_cache& cache,
+                                                  const kraken_paged_batch& batch,
+                                                  std::size_t heads, HipBuffer& output) const {
+    return Status::from_code(kraken_hip_attention_f16q_paged_q8_kv(
+      ctx_, query.raw(), &cache, &batch, heads, output.raw()));
+  }
+  [[nodiscard]] Status dequantize_kv_pages_q8_f16(const kraken_paged_q8_cache& cache,
+                                                  const HipBuffer& page_ids, std::size_t count,
+                                                  HipBuffer& key_rows,
+                                                  HipBuffer& value_rows) const {
+    return Status::from_code(kraken_hip_dequantize_kv_pages_q8_f16(
+      ctx_, &cache, page_ids.raw(), count, key_rows.raw(), value_rows.raw()));
+  }
+  [[nodiscard]] Status sample_f32_i32(const HipBuffer& logits, std::size_t rows,
+                                      std::size_t size, std::size_t row_stride,
+                                      const HipBuffer& temperature, const HipBuffer& top_k,
+                                      const HipBuffer& top_p, const HipBuffer& min_p,
+                                      const HipBuffer& uniforms, HipBuffer& token_output,
+                                      HipBuffer& probability_output) const {
+    return Status::from_code(kraken_hip_sample_f32_i32(
+      ctx_, logits.raw(), rows, size, row_stride, temperature.raw(), top_k.raw(), top_p.raw(),
+      min_p.raw(), uniforms.raw(), token_output.raw(), probability_output.raw()));
+  }
+
  private:
   explicit HipContext(kraken_hip_context* raw) : ctx_(raw) {}
 

@@ -749,7 +749,8 @@ KRAKEN_API int kraken_hip_argmax_prob_f32_i32(kraken_hip_context* context, krake
  * Rows of no sequence stay as they were.  A page id outside [0, pages) is a
  * page without tokens: its keys are not attended and nothing is appended to it.
  * A page that a call appends to must stand once in the batch's tables; pages that
- * are only read may be shared. */
+ * are only read may be shared.  Refused are more than 2^31 - 1 pages, tokens or keys of
+ * a sequence and more than 1048576 pairs of a sequence and a KV head. */
 typedef struct kraken_paged_q8_cache {
   kraken_buffer key_pages;
   kraken_buffer value_pages;
@@ -803,9 +804,11 @@ KRAKEN_API int kraken_hip_qwen35_attention_prologue_paged_q8_kv(
  * 1 / sqrt(head_dim).  gate.data == NULL: none; else out *= sigmoid(gate).
  * heads is a multiple of kv_heads.  Products keep f32 accuracy: the codes are
  * exact in the matrix cores' f16 and the f32 operands go in as two f16 parts.  A
- * row without any key to attend (all its pages outside the pool) gets zeros.
- * query, gate and output are 16-byte aligned; output overlaps neither.  Uses
- * context workspace where the keys are split over workgroups. */
+ * row without any key to attend (all its pages outside the pool) gets zeros.  A NaN
+ * or an infinity in a query or in a scale reaches only the rows that use it.
+ * query, gate and output are 16-byte aligned; output overlaps neither; up to 67108864
+ * rows (tokens * heads).  Uses context workspace where the keys are split over
+ * workgroups (at most about 512 MiB). */
 KRAKEN_API int kraken_hip_attention_f32_paged_q8_kv(
   kraken_hip_context* context, kraken_buffer query, kraken_buffer gate,
   const kraken_paged_q8_cache* cache, const kraken_paged_batch* batch, size_t heads,
@@ -844,7 +847,8 @@ KRAKEN_API int kraken_hip_dequantize_kv_pages_q8_f16(
  * temperature draws greedily, NaN top_p and min_p keep all, a uniform outside
  * [0, 1) or NaN is taken as the nearest end (NaN as 0).  Weights are formed in 64
  * bits and summed as integers (2^-44 of the largest up to 262144 tokens), so a
- * result does not depend on the order of the sums.  Uses context workspace. */
+ * result does not depend on the order of the sums.  Up to 65535 rows of up to 4194304
+ * logits; context workspace of up to 1 GiB (or one row's need). */
 KRAKEN_API int kraken_hip_sample_f32_i32(
   kraken_hip_context* context, kraken_buffer logits, size_t rows, size_t size,
   size_t row_stride, kraken_buffer temperature, kraken_buffer top_k, kraken_buffer top_p,
