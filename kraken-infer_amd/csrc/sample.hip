@@ -22,9 +22,9 @@
 // So a row is read three times, from memory once (the rest from the caches), and each
 // exponential is formed once but for those of the list and of the drawn chunk.
 //
-// 64 rows of 248320 take 12 + 31 + 17 + 23 us in the four, 78 us together, 8.5 times the
+// 64 rows of 248320 take 12 + 27 + 18 + 24 us in the four, 75 us together, 8 times the
 // logits' way from memory.  top runs at 5.2 TB/s.  Of bins, the sums of all workgroups in
-// memory are 5 us, counts 3, the exponentials 5, and 18 reading and adding in LDS.
+// memory are 2 us, counts 3, the exponentials 5, and 18 reading and adding in LDS.
 // gather repeats the scan of the row's histogram in each workgroup.  draw is a chain of
 // some thirty barriers in one workgroup a row, and most of a small call's time (8 rows of
 // 32000: 20 of 28 us).  A launch costs 2 to 3 us, a release to the device within one
@@ -47,6 +47,10 @@ constexpr uint32_t kDrawThreads = 512;  // of the draw
 constexpr uint32_t kBins = 512;         // 1/8 octave each; the last takes all below 2^-63
 constexpr uint32_t kMaxChunk = 4096;    // logits of a chunk
 constexpr uint32_t kMaxChunks = 1024;   // of a row
+// Histograms of a row that its chunks add to in turn, joined by who reads them: with one,
+// 243 workgroups wait for each other (us, 1 row of 248320 / 64 of them: 30.4 / 81.7; two
+// 27.9 / 80.1, four 27.0 / 77.9, eight 26.6 / 80.0).
+constexpr uint32_t kCopies = 4;
 constexpr uint32_t kHeld = 8192;        // entries of the list that the draw holds in LDS
 constexpr uint32_t kMinusInfKey = 0x007fffffu;
 
@@ -164,8 +168,8 @@ struct Entry {
 // A row's place in the workspace.
 struct RowWork {
   RowMeta* meta;
-  uint64_t* bin_weight;    // [kBins]
-  uint32_t* bin_count;     // [kBins]
+  uint64_t* bin_weight;    // [kCopies][kBins]: chunk c adds to copy c % kCopies
+  uint32_t* bin_count;     // [kCopies][kBins]
   uint64_t* chunk_weight;  // [chunks]: of what is kept whatever the threshold
   uint64_t* chunk_top;     // [chunks]: key << 32 | ~index
   uint32_t* chunk_listed;  // [chunks]: entries of the chunk's part of the list
@@ -183,7 +187,7 @@ struct Plan {
 constexpr size_t kMetaWords = 8;
 
 size_t words_per_row(const Plan& p) {
-  return kMetaWords + kBins + kBins / 2u + (size_t)p.chunks * (2u + kBins) +
+  return kMetaWords + kCopies * (kBins + kBins / 2u) + (size_t)p.chunks * (2u + kBins) +
          ((size_t)p.chunks / 2u + 1u) / 2u * 2u + 2u + 2u * (size_t)p.chunks * p.chunk;
 }
 
@@ -193,8 +197,8 @@ __device__ __forceinline__ RowWork row_work(const Plan& p, uint32_t row) {
   uint64_t* at = p.work + (size_t)row * p.row_words;
   w.meta = reinterpret_cast<RowMeta*>(at);
   w.bin_weight = at + kMetaWords;
-  w.bin_count = reinterpret_cast<uint32_t*>(w.bin_weight + kBins);
-  w.chunk_weight = w.bin_weight + kBins + kBins / 2u;
+  w.bin_count = reinterpret_cast<uint32_t*>(w.bin_weight + kCopies * kBins);
+  w.chunk_weight = w.bin_weight + kCopies * (kBins + kBins / 2u);
   w.chunk_top = w.chunk_weight + p.chunks;
   w.chunk_bins = w.chunk_top + p.chunks;
   // The list is 16-byte aligned: an even number of words before it.
@@ -334,10 +338,10 @@ __global__ __launch_bounds__(kThreads) void sample_top_kernel(SampleArgs a, Plan
   if (threadIdx.x == 0) {
     w.chunk_top[chunk] = top;
   }
-  if (chunk == 0) {
+  for (uint32_t copy = chunk; copy < kCopies; copy += p.chunks) {
     for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
-      w.bin_weight[i] = 0;
-      w.bin_count[i] = 0;
+      w.bin_weight[copy * kBins + i] = 0;
+      w.bin_count[copy * kBins + i] = 0;
     }
   }
 }
@@ -364,8 +368,13 @@ __device__ RowMeta row_bounds(const RowRule& rule, const RowWork& w, uint64_t* s
 #pragma unroll
   for (uint32_t i = 0; i < kPer; ++i) {
     const uint32_t bin = threadIdx.x * kPer + i;
-    weight[i] = w.bin_weight[bin];
-    count[i] = w.bin_count[bin];
+    weight[i] = 0;
+    count[i] = 0;
+#pragma unroll
+    for (uint32_t copy = 0; copy < kCopies; ++copy) {
+      weight[i] += w.bin_weight[copy * kBins + bin];
+      count[i] += w.bin_count[copy * kBins + bin];
+    }
     x += weight[i];
     n += count[i];
   }
@@ -482,14 +491,15 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Pla
     }
   });
   __syncthreads();
+  const uint32_t copy = chunk % kCopies * kBins;
   for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
     const uint64_t weight = bin_weight[i];
     w.chunk_bins[(size_t)chunk * kBins + i] = weight;
     if (weight != 0u) {
-      atomicAdd((unsigned long long*)&w.bin_weight[i], (unsigned long long)weight);
+      atomicAdd((unsigned long long*)&w.bin_weight[copy + i], (unsigned long long)weight);
     }
     if (bin_count[i] != 0u) {
-      atomicAdd(&w.bin_count[i], bin_count[i]);
+      atomicAdd(&w.bin_count[copy + i], bin_count[i]);
     }
   }
 }
