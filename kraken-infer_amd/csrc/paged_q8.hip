@@ -11,13 +11,13 @@
 //
 // One workgroup owns the new rows of one (sequence, page, KV head, keys or values):
 // it needs the largest magnitude of all of them before it can write the first code,
-// so it holds them in registers (up to 8 rows a wave of 16), and no second pass or launch
-// is needed.  The codes go through LDS, from which they leave in the layout of the pages:
+// so it holds them in registers (up to 8 rows a wave), and no second pass or launch is
+// needed.  The codes go through LDS, from which they leave in the layout of the pages:
 // rows for keys, runs of eight tokens a dimension for values.  The query heads are further
 // workgroups of the same launch, a wave per token and run of heads.
 //
 // 1024 tokens of 8 query and 2 KV heads of 256 (35 MB with what is read and written, 5 us
-// at the rate of a stream) take 14.8 us: the page rows' chain of loads, norm, largest
+// at the rate of a stream) take about 15 us: the page rows' chain of loads, norm, largest
 // magnitude and codes is as long for one page as for all, and 32 pages of 2 heads are 64
 // long workgroups.  One token takes 4.9 us, of which a launch is 2 to 3.  Reading the pages
 // back as F16 takes 5.9 us for 17 pages, 4.9 for one.
@@ -455,19 +455,24 @@ void launch_prologue(const PagedPrologueArgs& a, uint32_t rows, hipStream_t stre
 
 hipError_t launch_prologue_paged_q8(const PagedPrologueArgs& a, hipStream_t stream) {
   const uint32_t rows = std::min(1u << a.cache.page_shift, a.batch.max_query);
-  // A decode step: small workgroups, a wave a row and a query head.  Chunks: 16 waves on
-  // the rows of a page, whose time is theirs one after another, and four query heads a
-  // wave, which share the token's angles (us, with the pages read back: 1 token 11.0 with
-  // 8 waves, 10.7 with 4; 64 tokens 14.6 and 12.2; 1024 tokens 31.9 with 8 waves and
-  // heads one by one, 23.0 with 16 and three at once, 20.1 four).
+  // A decode step: a wave a row and a query head, four waves.  Chunks: as few waves on a
+  // page's rows as eight rows each take, since a page's chain of loads, norms, the largest
+  // magnitude and codes is as long for one row as for all, and many short workgroups share
+  // a CU; four query heads a wave, which share the token's angles.  (us, with the pages
+  // read back.  1 token 11.0 with 8 waves, 10.7 with 4; 64 tokens 14.6 and 12.2.  16
+  // sequences, 2000 tokens, 8 heads of 128, pages of 16: 16 waves 178, 4 waves 56; 24
+  // sequences, 1600 tokens, pages of 32: 70 and 39.  Pages of 64: 1024 tokens 20.1 with 16
+  // waves, 20.4 with 8, 24 sequences 72 and 65; one query head a wave 22.9.)
   if (rows <= 4u) {
     launch_prologue<1, 4, 1>(a, rows, stream);
   } else if (rows <= 16u) {
-    launch_prologue<1, 16, 4>(a, rows, stream);
+    launch_prologue<4, 4, 4>(a, rows, stream);
+  } else if (rows <= 32u) {
+    launch_prologue<8, 4, 4>(a, rows, stream);
   } else if (rows <= 64u) {
-    launch_prologue<4, 16, 4>(a, rows, stream);
+    launch_prologue<8, 8, 4>(a, rows, stream);
   } else {
-    launch_prologue<8, 16, 2>(a, rows, stream);
+    launch_prologue<8, 16, 4>(a, rows, stream);
   }
   return hipGetLastError();
 }
