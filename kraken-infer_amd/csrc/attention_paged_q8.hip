@@ -352,8 +352,8 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
 // Joins split results: kParts waves per (row, head), which take its parts in turn, D / 64
 // values a lane.
 template <int D, class T, int kParts>
-__global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentionArgs a,
-                                                                   PagedSplit split) {
+__global__ __launch_bounds__(kParts > 4 ? 64 * kParts : 256) void attention_paged_join_kernel(
+  PagedAttentionArgs a, PagedSplit split) {
   constexpr int kRegs = D / 64;
   __shared__ float lds[kParts > 1 ? kParts : 1][64 * kRegs];
   const uint32_t lane = threadIdx.x & 63u;
@@ -457,11 +457,9 @@ __global__ __launch_bounds__(256) void attention_paged_join_kernel(PagedAttentio
     }
     store_output<T>(a, item * D + threadIdx.x, value, inverse_sum(sum));
   } else {
-    const float inverse = inverse_sum(l);
-#pragma unroll
-    for (int r = 0; r < kRegs; ++r) {
-      store_output<T>(a, item * D + lane * kRegs + r, x[r], inverse);
-    }
+    float factor[kRegs];
+    gate_factors<T>(a, item * D + lane * kRegs, factor);
+    store_outputs<T>(a, item * D + lane * kRegs, x, inverse_sum(l), factor);
   }
 }
 
@@ -471,15 +469,18 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   const uint64_t rows = group * a.batch.max_query;
   // Keys per workgroup: 128 (a 32-key step for each wave) while all sequences at the
   // longest length make no more than eleven workgroups a CU, else as many as make so few,
-  // up to 4096; more where the partial results would take over 256 MiB.  (64 sequences of
-  // up to 32768 keys, 2 KV heads: 512 keys 226 us, 1024 205, 1280 197, 1536 194, 2048 205.
-  // One of 4096, 32 workgroups of 128: 12.8 us.)
+  // up to 4096, but no more than 128 parts of a sequence, which one workgroup joins (one
+  // sequence of 131072 keys: 34 us with 128 parts, 40 with 512, 56 with 1025); more where the
+  // partial results would take over 256 MiB.  (64 sequences of up to 32768 keys, 2 KV heads:
+  // 512 keys 226 us, 1024 205, 1280 197, 1536 194, 2048 205.  One of 4096, 32 workgroups of
+  // 128: 12.4 us.)
   const uint64_t lanes = (uint64_t)a.batch.sequences * a.cache.kv_heads;
   const uint64_t part_bytes =
     std::min<uint64_t>(rows, kDecodeRows) * (a.cache.head_dim + 2u) * sizeof(float);
   const uint64_t most = 11u * (uint64_t)cu_count;
   auto parts = [&](uint64_t k) { return lanes * ((a.batch.max_keys + k - 1u) / k); };
   uint64_t keys = (lanes * a.batch.max_keys + most - 1u) / most;
+  keys = std::max<uint64_t>(keys, (a.batch.max_keys + 127u) / 128u);
   keys = std::min<uint64_t>((keys + 127u) / 128u * 128u, 4096u);
   while (parts(keys) > lanes && parts(keys) * part_bytes > (uint64_t{256} << 20)) {
     keys *= 2u;
@@ -558,10 +559,13 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
   const uint64_t items = (uint64_t)a.batch.tokens * a.heads;
   const uint32_t parts = std::max(split.decode_most != 0u ? split.decode_splits : 1u,
                                   rows > kDecodeRows ? split.tile_splits : 1u);
-  // Four waves a row where there are many parts and few rows (one row of 33 parts 7.3 -> 4
-  // us), one where the rows alone fill the device (14544 rows, most of four parts or fewer:
+  // Sixteen waves a row, or four, where there are many parts and few rows (one row of 33
+  // parts: 7.3 us with one, 4 with four; a call with 129 parts of 8 rows 17.9 us with four,
+  // 15.8 with sixteen), one where the rows alone fill the device (14544 rows, most of four parts or fewer:
   // 18.6 us with four, 9.0 with one).
-  if (parts > 8u && items <= 4096u) {
+  if (parts > 32u && items <= 1024u) {
+    attention_paged_join_kernel<D, T, 16><<<dim3((uint32_t)items), 1024, 0, stream>>>(a, split);
+  } else if (parts > 8u && items <= 4096u) {
     attention_paged_join_kernel<D, T, 4><<<dim3((uint32_t)items), 256, 0, stream>>>(a, split);
   } else if (parts > 1u) {
     attention_paged_join_kernel<D, T, 1><<<dim3((uint32_t)((items + 3u) / 4u)), 256, 0, stream>>>(

@@ -502,21 +502,25 @@ __device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a
   const bool whole = s.length <= part_keys;
   const float inverse = inverse_sum(sum);
   const size_t item = (size_t)part * a.batch.tokens * a.heads + at / D;
+  // Registers 4 j .. + 3 of product i are dimensions 32 i + 8 j + 4 h .. + 3.
+  if (whole) {
+    float factor[D / 8][4];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
+    for (int i = 0; i < D / 8; ++i) {
+      gate_factors<T>(a, at + 8 * i + 4 * h, factor[i]);
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // Registers 4 j .. + 3 are dimensions 32 i + 8 j + 4 h .. + 3.
-      const uint32_t d = 32 * i + 8 * j + 4 * h;
-      const float4_t x = {o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
-      if (whole) {
+    for (int i = 0; i < D / 8; ++i) {
+      const float x[4] = {o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1],
+                          o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+      store_outputs<T>(a, at + 8 * i + 4 * h, x, inverse, factor[i]);
+    }
+  } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          store_output<T>(a, at + d + r, x[r], inverse);
-        }
-      } else {
-        *reinterpret_cast<float4_t*>(split.tile_o + item * D + d) = x;
-      }
+    for (int i = 0; i < D / 8; ++i) {
+      const float4_t x = {o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1],
+                          o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+      *reinterpret_cast<float4_t*>(split.tile_o + item * D + 8 * i + 4 * h) = x;
     }
   }
   if (!whole && h == 0) {
