@@ -15,7 +15,7 @@
 //    by side, the operand of V is eight bytes as they lie.
 //  - The f32 operands need two f16 parts.  Up to 8 rows fill only half of the 16
 //    columns, so the high parts take columns 0..7 and the low parts 8..15 of the same
-//    product (kStacked) and the halves are added; up to 16 rows take two products.
+//    product (kStacked) and the halves are added; a block of 16 rows takes two products.
 //
 // 64 sequences of up to 32768 keys, 2 KV heads of 256 (1.07 GB): 191 us, 5.6 TB/s, of the
 // 6.95 that a read of as much reaches; the parts are of one size, so the last ones end
@@ -42,7 +42,7 @@ __device__ __forceinline__ u32x4_t load_once(const int8_t* p) {
 template <int D, class T, bool kStacked>
 __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAttentionArgs a,
                                                                         PagedSplit split) {
-  constexpr uint32_t kRows = kStacked ? 8 : 16;
+  constexpr uint32_t kRows = kStacked ? 8 : kDecodeBlock;
   constexpr bool kTwo = !kStacked && std::is_same<T, float>::value;
   constexpr int kLoads = D / 64;  // 16-byte loads of a key row per lane and row tile
   constexpr int kStride = D + 4;  // of an output row in LDS, in floats
@@ -54,19 +54,27 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   const uint32_t shift = a.cache.page_shift, kv_heads = a.cache.kv_heads;
   const uint32_t group = a.heads / kv_heads;
   const uint32_t kv_head = blockIdx.x % kv_heads;
-  uint32_t part = blockIdx.x / kv_heads, sequence = 0;
+  uint32_t item = blockIdx.x / kv_heads, sequence = 0;
   PagedSequence s;
   if (a.batch.sequences > 1u) {
     // The sequences' parts one after another: no workgroup without keys stands between
     // two with, and the XCDs, which take workgroups in turn, get as many each.
-    const PagedItem found = paged_item(a.batch, part, shift, [&](const PagedSequence& q) {
-      return q.count * group <= kRows ? (q.length + split.decode_keys - 1u) / split.decode_keys
-                                      : 0u;
+    const PagedItem found = paged_item(a.batch, item, shift, [&](const PagedSequence& q) {
+      const uint32_t r = q.count * group;
+      return r <= split.decode_rows ? (r + kRows - 1u) / kRows *
+                                        ((q.length + split.decode_keys - 1u) / split.decode_keys)
+                                    : 0u;
     });
     s = found.sequence;
     sequence = found.index;
-    part = found.item;
+    item = found.item;
+  } else {
+    s.count = a.batch.max_query;
   }
+  // The row blocks of a part stand side by side.  (A single sequence's are those of
+  // max_query, which it may fall short of.)
+  const uint32_t blocks = max(1u, (s.count * group + kRows - 1u) / kRows);
+  const uint32_t part = item / blocks, first_row = item % blocks * kRows;
   const uint32_t begin = part * split.decode_keys;
   // The first pages' ids are asked for together with a single sequence's length (in the
   // bounds of the table whatever that is): K and V wait for two loads in a row, not three.
@@ -79,20 +87,21 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   if (a.batch.sequences == 1u) {
     s = paged_sequence(a.batch, 0, shift);
   }
-  const uint32_t rows = s.count * group;
-  if (s.count == 0 || rows > kRows || begin >= s.length) {
+  if (s.count == 0 || s.count * group > split.decode_rows || first_row >= s.count * group ||
+      begin >= s.length) {
     return;
   }
+  const uint32_t rows = min(kRows, s.count * group - first_row);
   const uint32_t end = min(s.length, begin + split.decode_keys);
   const uint32_t steps = (end - begin + 31u) / 32u;
 
   // This lane's query row and the keys that it sees.
   const uint32_t row = kStacked ? n & 7u : n;
   const bool real = row < rows;
-  const uint32_t token = real ? row / group : 0u;
+  const uint32_t token = real ? (first_row + row) / group : 0u;
   const uint32_t visible = s.length - s.count + token + 1u;
   const size_t at = ((size_t)(s.start + token) * a.heads + kv_head * group +
-                     (real ? row % group : 0u)) * D;
+                     (real ? (first_row + row) % group : 0u)) * D;
 
   u32x4_t k[2][kLoads], v[2 * kLoads];
   float key_scale, val_scale;
@@ -184,7 +193,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   }
   float top = kLowestMax, sum = 0.0f;
   // Keys that every row sees need no mask.
-  const uint32_t open = s.length - s.count + 1u;
+  const uint32_t open = s.length - s.count + first_row / group + 1u;
 
   for (uint32_t step = wave; step < steps; step += kWaves) {
     const uint32_t next = step + kWaves;
@@ -335,11 +344,12 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
     }
     if (whole) {
       const size_t out =
-        ((size_t)(s.start + r / group) * a.heads + kv_head * group + r % group) * D;
+        ((size_t)(s.start + (first_row + r) / group) * a.heads + kv_head * group +
+         (first_row + r) % group) * D;
       store_output<T>(a, out + d, x, inverse_sum(l));
     } else {
       const size_t i = (((size_t)part * a.batch.sequences + sequence) * kv_heads + kv_head) *
-                         split.decode_rows + r;
+                         split.decode_rows + first_row + r;
       split.decode_o[i * D + d] = x;
       if (d == 0) {
         split.decode_ml[2 * i] = m;
@@ -488,9 +498,11 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   // (A part of more keys than there are would only bring the sums of the two past 32 bits.)
   keys = std::min(keys, (a.batch.max_keys + 127u) / 128u * uint64_t{128});
   // A single sequence with many rows needs no second kernel beside the tiled one.
-  s.decode_most = rows <= kDecodeRows || a.batch.sequences > 1u ? kDecodeRows : 0u;
+  s.decode_most = rows <= kDecodeRows       ? kDecodeRows
+                  : a.batch.sequences > 1u ? kDecodeBlock
+                                           : 0u;
   s.decode_keys = (uint32_t)keys;
-  s.decode_rows = (uint32_t)std::min<uint64_t>(rows, kDecodeRows);
+  s.decode_rows = rows <= kDecodeRows ? (uint32_t)rows : kDecodeBlock;
   s.decode_splits = (uint32_t)((a.batch.max_keys + keys - 1u) / keys);
   // The tiled kernel's keys in parts of 128 at least, so that there is one for each
   // workgroup that the CUs hold at a time (one of head_dim 256, two of less), while the
@@ -546,7 +558,8 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
   const uint32_t group = a.heads / a.cache.kv_heads;
   const uint64_t rows = (uint64_t)a.batch.max_query * group;
   if (group <= split.decode_most) {
-    const dim3 grid(split.decode_splits * a.cache.kv_heads * a.batch.sequences);
+    const uint32_t blocks = (split.decode_rows + kDecodeBlock - 1u) / kDecodeBlock;
+    const dim3 grid(split.decode_splits * blocks * a.cache.kv_heads * a.batch.sequences);
     if (rows <= 8u) {
       attention_paged_decode_kernel<D, T, true><<<grid, 256, 0, stream>>>(a, split);
     } else {
@@ -561,8 +574,8 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
                                   rows > kDecodeRows ? split.tile_splits : 1u);
   // Sixteen waves a row, or four, where there are many parts and few rows (one row of 33
   // parts: 7.3 us with one, 4 with four; a call with 129 parts of 8 rows 17.9 us with four,
-  // 15.8 with sixteen), one where the rows alone fill the device (14544 rows, most of four parts or fewer:
-  // 18.6 us with four, 9.0 with one).
+  // 15.8 with sixteen), one where the rows alone fill the device (14544 rows, most of four
+  // parts or fewer: 18.6 us with four, 9.0 with one).
   if (parts > 32u && items <= 1024u) {
     attention_paged_join_kernel<D, T, 16><<<dim3((uint32_t)items), 1024, 0, stream>>>(a, split);
   } else if (parts > 8u && items <= 4096u) {

@@ -34,9 +34,13 @@ constexpr float kLowestMax = -1e30f;
 constexpr float kWeightShift = 11.0f;
 constexpr float kMaxLead = 4.0f;
 
-// Sequences of at most this many rows (new tokens x query heads per KV head) take the
-// split decode kernel, longer ones the tiled one.
-constexpr uint32_t kDecodeRows = 16;
+// Rows (new tokens x query heads per KV head) of a batch's largest sequence up to which the
+// decode kernel takes all of it, in blocks of 16 that read the keys again (32 rows, 64
+// sequences of up to 4096 keys: 99 us, by tiles 120; 48 rows 135 and 122).  In a batch with
+// larger ones it takes the sequences of one block, the tiled kernel the others (32 rows
+// there: 51 us instead of 46 for 24 sequences of up to 80 rows).
+constexpr uint32_t kDecodeRows = 32;
+constexpr uint32_t kDecodeBlock = 16;
 // Rows of the tiled kernel's workgroups: 32 a wave.
 constexpr uint32_t kTileRows = 128;
 

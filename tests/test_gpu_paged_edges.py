@@ -230,3 +230,16 @@ def test_pages_read_back_twice(hip_ctx):
             want = (cache.values_of(n, page).astype(np.float32).astype(np.float16)
                     if 0 <= page < 5 else np.zeros((32, 3, 64), np.float16))
             np.testing.assert_array_equal(got[i], want)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new,before", [([4, 1, 2, 0, 3], [9, 300, 1000, 5, 0]), ([4], [700]),
+                                        ([3], [40]), ([2, 9, 4], [129, 64, 500])])
+def test_blocks_of_rows(hip_ctx, new, before, f16):
+    """17 to 32 rows of a sequence and KV head, more than one block of the decode kernel,
+    alone and beside shorter and longer ones."""
+    rng = np.random.default_rng(48)
+    batch = Batch(rng, 32, new, before, gap=1)
+    for heads, kv, d in ((14, 2, 64), (8, 1, 128), (24, 3, 256)):
+        cache = po.Pages(rng, batch.pages, 32, kv, d)
+        check_attention(hip_ctx, rng, cache, batch, heads, f16, gated=not f16)
