@@ -591,7 +591,7 @@ struct DrawScratch {
 };
 
 // The entries of the list: in LDS, or (a row whose threshold has more than kHeld logits
-// in its bins) in memory, chunk by chunk.
+// in its bins) in memory, a chunk a wave.
 struct Entries {
   const RowWork* work;
   const Plan* plan;
@@ -608,9 +608,10 @@ struct Entries {
         f(e.key, e.index, e.weight);
       }
     } else {
-      for (uint32_t c = 0; c < plan->chunks; ++c) {
+      for (uint32_t c = threadIdx.x / 64u; c < plan->chunks; c += kDrawThreads / 64u) {
         const uint32_t n = work->chunk_listed[c];
-        for (uint32_t i = threadIdx.x; i < n; i += kDrawThreads) {
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x & 63u; i < n; i += 64u) {
           const Entry e = work->list[(size_t)c * plan->chunk + i];
           f(e.key, e.index, e.weight);
         }
@@ -746,6 +747,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
   __syncthreads();
   uint32_t high = 0, low = 0xffffffffu;
   if (all_n <= kHeld) {
+#pragma unroll 4
     for (uint32_t i = threadIdx.x; i < all_n; i += kDrawThreads) {
       // The last chunk whose place is not behind i.
       uint32_t c = 0;
@@ -881,11 +883,34 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     s.chunk_weight[i] = w.chunk_weight[i];
   }
   __syncthreads();
-  e.each([&](uint32_t key, uint32_t i, uint64_t x) {
+  // A thread takes neighbours in the list, which are of one chunk mostly, and adds what it
+  // has of a chunk at once (an entry at a time, the 64 of a wave wait for each other).
+  uint32_t own_chunk = 0;
+  uint64_t own = 0;
+  auto add = [&](uint32_t key, uint32_t i, uint64_t x) {
     if (x != 0u && cut.keeps(key, i) && above_min(key)) {
-      atomicAdd((unsigned long long*)&s.chunk_weight[i / p.chunk], (unsigned long long)x);
+      const uint32_t c = i / p.chunk;
+      if (c != own_chunk && own != 0u) {
+        atomicAdd((unsigned long long*)&s.chunk_weight[own_chunk], (unsigned long long)own);
+        own = 0;
+      }
+      own_chunk = c;
+      own += x;
     }
-  });
+  };
+  if (all_n <= kHeld) {
+    const uint32_t each = (all_n + kDrawThreads - 1u) / kDrawThreads;
+    const uint32_t to = min(all_n, (threadIdx.x + 1u) * each);
+    for (uint32_t i = threadIdx.x * each; i < to; ++i) {
+      const Entry held = s.held[i];
+      add(held.key, held.index, held.weight);
+    }
+  } else {
+    e.each(add);
+  }
+  if (own != 0u) {
+    atomicAdd((unsigned long long*)&s.chunk_weight[own_chunk], (unsigned long long)own);
+  }
   // One running sum passes the target first; where none does (a uniform of 1), the last
   // kept token is drawn.
   if (threadIdx.x == 0) {
