@@ -576,6 +576,9 @@ struct Cut {
 // A list this short is looked at entry against entry (8 rows of 32000: 29.5 us; by radix
 // selection, or up to 256 entries this way, 31.1 and 30.0 us).
 constexpr uint32_t kDirect = 128;
+// So few left of a longer one end its radix selection (64 rows of 152000 alike: 88.5 us, 95
+// without; up to 256 95, whose comparisons take what the steps did).
+constexpr uint32_t kFew = 64;
 constexpr uint32_t kDigits = 1024;  // of a step of the radix selection
 
 struct DrawScratch {
@@ -588,6 +591,8 @@ struct DrawScratch {
   uint64_t found_weight;
   uint32_t found, found_count, found_here;
   uint32_t cut_key, cut_index;
+  uint64_t few_weights[kFew];
+  uint32_t few_values[kFew], few;
 };
 
 // The entries of the list: in LDS, or (a row whose threshold has more than kHeld logits
@@ -620,7 +625,7 @@ struct Entries {
   }
 };
 
-// Radix selection in the list, ten bits of a field at a time.  field(key, index, value)
+// Radix selection in the list, ten bits of a field at a time until few are left.  field(key, index, value)
 // says whether an entry counts, and its value, low <= value <= high.  Walking from the
 // largest value down, the last one before which less than `target` (by weight; at least
 // the first value) or fewer than `count` lie.  Returns the value; `before`, `before_n`
@@ -706,6 +711,52 @@ __device__ __forceinline__ uint32_t select_value(const Entries& e, double target
     before_n = s.found_count;
     here = s.found_here;
     at = next;
+    if (at > 0 && here <= kFew) {
+      // The few that are left, each against each.
+      if (threadIdx.x == 0) {
+        s.few = 0;
+        s.found = 0xffffffffu;
+      }
+      __syncthreads();
+      e.each([&](uint32_t key, uint32_t index, uint64_t weight) {
+        uint32_t v;
+        if (field(key, index, v) && v >> at == prefix >> at) {
+          const uint32_t i = atomicAdd(&s.few, 1u);
+          s.few_values[i] = v;
+          s.few_weights[i] = weight;
+        }
+      });
+      __syncthreads();
+      bool reached = false;
+      uint32_t own = 0, larger = 0, equal = 0;
+      uint64_t heavier = 0;
+      if (threadIdx.x < here) {
+        own = s.few_values[threadIdx.x];
+        for (uint32_t i = 0; i < here; ++i) {
+          const uint32_t v = s.few_values[i];
+          larger += v > own ? 1u : 0u;
+          equal += v == own ? 1u : 0u;
+          heavier += v > own ? s.few_weights[i] : 0u;
+        }
+        reached = larger == 0u || (kByWeight ? (double)(before + heavier) < target
+                                             : before_n + larger < count);
+        if (reached) {
+          atomicMin(&s.found, own);
+        }
+      }
+      __syncthreads();
+      prefix = s.found;
+      if (reached && own == prefix) {
+        s.found_weight = before + heavier;
+        s.found_count = before_n + larger;
+        s.found_here = equal;
+      }
+      __syncthreads();
+      before = s.found_weight;
+      before_n = s.found_count;
+      here = s.found_here;
+      break;
+    }
   }
   return prefix;
 }

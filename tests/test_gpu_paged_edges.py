@@ -243,3 +243,22 @@ def test_blocks_of_rows(hip_ctx, new, before, f16):
     for heads, kv, d in ((14, 2, 64), (8, 1, 128), (24, 3, 256)):
         cache = po.Pages(rng, batch.pages, 32, kv, d)
         check_attention(hip_ctx, rng, cache, batch, heads, f16, gated=not f16)
+
+
+@pytest.mark.parametrize("cluster", [2, 63, 64, 65, 129, 700])
+def test_cuts_inside_clusters(hip_ctx, cluster):
+    """Logits within a few steps of each other, many of them equal, and cuts among them:
+    a threshold's last digits hold one, few and many entries."""
+    rng = np.random.default_rng(cluster)
+    rows, size = 12, 9000
+    x = (rng.standard_normal((rows, size)) - 4).astype(np.float32)
+    for r in range(rows):
+        at = rng.permutation(size)[:cluster]
+        x[r, at] = np.float32(2.0) + rng.integers(0, 1 + r * cluster // 8, cluster).astype(
+            np.float32) * np.float32(2.0 ** -22)
+        x[r, rng.permutation(size)[:3]] = 3.0
+    u = rng.random(rows).astype(np.float32)
+    k = np.clip(rng.integers(1, cluster + 8, rows), 1, size).astype(np.int32)
+    check_sample(hip_ctx, x, u, top_k=k.tolist())
+    check_sample(hip_ctx, x, u, top_p=rng.uniform(0.05, 0.6, rows).astype(np.float32).tolist())
+    check_sample(hip_ctx, x, u, top_k=k.tolist(), top_p=[0.5] * rows)
