@@ -9,7 +9,8 @@ import pytest
 
 import kraken_hip as kh
 import paged_oracle as po
-from test_gpu_paged_q8 import Batch, DevicePages, check_attention, run_attention
+from test_gpu_paged_q8 import (Batch, DevicePages, check_attention, check_pages, run_attention,
+                                run_prologue)
 from test_gpu_sample import check as check_sample
 
 pytestmark = pytest.mark.gpu
@@ -262,3 +263,31 @@ def test_cuts_inside_clusters(hip_ctx, cluster):
     check_sample(hip_ctx, x, u, top_k=k.tolist())
     check_sample(hip_ctx, x, u, top_p=rng.uniform(0.05, 0.6, rows).astype(np.float32).tolist())
     check_sample(hip_ctx, x, u, top_k=k.tolist(), top_p=[0.5] * rows)
+
+
+@pytest.mark.parametrize("page_tokens,new,before", [
+    (32, [20, 1, 90], [3, 31, 64]), (128, [200, 1, 60], [40, 127, 256]), (128, [20], [120]),
+    (64, [30, 64], [50, 0]), (16, [3, 4], [14, 31])])
+def test_prologue_rows_per_page(hip_ctx, page_tokens, new, before):
+    """Every number of waves that a page's rows are spread over."""
+    rng = np.random.default_rng(page_tokens + len(new))
+    batch = Batch(rng, page_tokens, new, before, gap=1)
+    for heads, kv, d in ((6, 3, 64), (8, 2, 256)):
+        cache = po.Pages(rng, batch.pages, page_tokens, kv, d)
+        q, gate, got_q, got_gate, pages, exact = run_prologue(hip_ctx, rng, cache, batch, heads, 64,
+                                                              (11, 11, 10, 0))
+        check_pages(cache, pages.read(), exact)
+        step = np.abs(q[:batch.rows]).max(-1, keepdims=True) * 2.0 ** -19
+        assert (np.abs(got_q - q)[:batch.rows] <= step).all()
+        np.testing.assert_array_equal(got_gate[:batch.rows], gate[:batch.rows])
+        assert (got_q[batch.rows:] == -77).all()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new,before", [([1], [300]), ([1, 1, 3], [40, 900, 0])])
+def test_more_query_heads_than_a_block(hip_ctx, new, before, f16):
+    """40 query heads of one KV head: one token is more than 32 rows."""
+    rng = np.random.default_rng(49)
+    batch = Batch(rng, 64, new, before)
+    cache = po.Pages(rng, batch.pages, 64, 1, 64)
+    check_attention(hip_ctx, rng, cache, batch, 40, f16)
