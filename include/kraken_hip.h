@@ -729,8 +729,10 @@ KRAKEN_API int kraken_hip_argmax_prob_f32_i32(kraken_hip_context* context, krake
  *   value_pages  [pages][kv_heads][page_tokens / 8][head_dim][8]: the eight
  *                tokens of a run lie side by side for each dimension
  *   key_scales, value_scales  f32 [pages][kv_heads], not negative (a value scale
- *                below 2^-100, zero too, is attended as 2^-100: the prologue makes
- *                none, and under a zero scale its codes are zeros)
+ *                below 2^-70, zero too, is attended as 2^-70: the prologue makes
+ *                none, and under a zero scale its codes are zeros; above 2^30, keys of
+ *                such pages that score far below the top one, more than 67 octaves of
+ *                weight less the scale's, drop out of the softmax's sum)
  * page_tokens is 16, 32, 64 or 128; head_dim 64, 128 or 256; the page pools are
  * 16-byte aligned.  Nothing needs initialising: a page's scale and codes are
  * written when its first token is.
@@ -789,7 +791,7 @@ typedef struct kraken_paged_batch {
  * codes are the rows over the scale, rounded to even.  Codes behind a page's
  * last token stay as they were.  A new row with a NaN or an infinity makes its
  * page's scale NaN for that head (its values then read as NaN) until the page is
- * begun again; rows whose largest magnitude is below 127 * 2^-100 (1e-28) are held
+ * begun again; rows whose largest magnitude is below 127 * 2^-70 (1e-19) are held
  * as zeros.  One launch, no workspace. */
 KRAKEN_API int kraken_hip_qwen35_attention_prologue_paged_q8_kv(
   kraken_hip_context* context, kraken_buffer q_gate, kraken_buffer key, kraken_buffer value,

@@ -88,10 +88,10 @@ struct ValueScale {
   float inverse;   // 2^-b, for the softmax's sum
 };
 
-// Not below 2^-100, so that the sum of quotients stays finite; the prologue holds rows
-// that would need less as zeros.  (A NaN stays one.)
+// Not below the least that the prologue makes, so that the sum of quotients stays finite.
+// (A NaN stays one.)
 __device__ __forceinline__ ValueScale value_scale(float s) {
-  const float held = s < 0x1p-100f ? 0x1p-100f : s;
+  const float held = s < kLeastScale ? kLeastScale : s;
   return {log2f(held), 1.0f / held};
 }
 

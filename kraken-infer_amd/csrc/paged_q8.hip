@@ -178,7 +178,7 @@ __device__ __forceinline__ void grow_scale(uint32_t largest_bits, float old_scal
   }
   if (begun || old_scale == 0.0f) {
     const float s = largest / 127.0f;
-    scale = s < 0x1p-100f ? 0.0f : s;  // the least that the attention takes
+    scale = s < kLeastScale ? 0.0f : s;
     factor = 0.0f;  // older codes under a zero scale are zeros
     return;
   }

@@ -8,6 +8,13 @@
 
 namespace kraken {
 
+// The least scale of a page that is not all zeros: the prologue holds rows that need less
+// as zeros, and the attention takes a lesser value scale, zero too, as this one.  A key
+// then adds up to 2^(11 + 4 + 70) to a softmax's sum (attention_paged_q8_common.hpp), 2^31
+// of them 2^116, below f32's largest; and beside values whose scale is up to 2^30, a key of
+// such a page is lost to f32's least normal number only 37 octaves below the top score.
+constexpr float kLeastScale = 0x1p-70f;
+
 // kraken_paged_q8_cache with device pointers; page_tokens = 1 << page_shift.
 struct PagedQ8Args {
   int8_t* keys;         // [pages][kv_heads][page_tokens][head_dim]
