@@ -100,7 +100,6 @@ __device__ __forceinline__ bool takes_top(const RowRule& rule, uint32_t top) {
 struct Weights {
   float top;              // the largest logit
   double top_wide, factor;  // factor: log2(e) / T
-  float scale;            // 8 log2(e) / T
   double one;             // 2^shift
   int shift;
 };
@@ -108,7 +107,7 @@ struct Weights {
 __device__ __forceinline__ Weights weights_of(uint32_t top, const RowRule& rule, int shift) {
   const float logit = logit_of(top);
   const double factor = 1.4426950408889634074 * rule.inverse_temperature;
-  return {logit, (double)logit, factor, (float)(8.0 * factor), ldexp(1.0, shift), shift};
+  return {logit, (double)logit, factor, ldexp(1.0, shift), shift};
 }
 
 // A logit's weight (not a NaN's), before rounding to a whole number: 2^y 2^shift with
@@ -139,9 +138,10 @@ __device__ __forceinline__ uint64_t weight_fixed(float logit, const Weights& w) 
 }
 
 // How many eighths of an octave a logit's weight lies below the largest, and its bin:
-// falling logits have rising bins (each step of it is monotone).  NaN only of a NaN.
+// falling logits have rising bins (each step of it is monotone).  NaN only of a NaN.  In 64
+// bits, as the weight: two logits' difference, or 1 / T, may be beyond f32's largest.
 __device__ __forceinline__ float eighths_of(float logit, const Weights& w) {
-  const float z = (w.top - logit) * w.scale;
+  const float z = (float)(((double)logit - w.top_wide) * w.factor * -8.0);
   return logit == w.top ? 0.0f : logit != logit ? z : z >= 0.0f ? z : (float)kBins;
 }
 
