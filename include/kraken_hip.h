@@ -730,9 +730,10 @@ KRAKEN_API int kraken_hip_argmax_prob_f32_i32(kraken_hip_context* context, krake
  *                tokens of a run lie side by side for each dimension
  *   key_scales, value_scales  f32 [pages][kv_heads], not negative (a value scale
  *                below 2^-70, zero too, is attended as 2^-70: the prologue makes
- *                none, and under a zero scale its codes are zeros; above 2^30, keys of
- *                such pages that score far below the top one, more than 67 octaves of
- *                weight less the scale's, drop out of the softmax's sum)
+ *                none, and under a zero scale its codes are zeros.  Beside pages of a
+ *                scale 2^b, keys of such a page drop out of the softmax's sum where their
+ *                weight is below 2^(b - 67) of the largest: less than f32's rounding of it
+ *                for values of up to 10^11, b = 30)
  * page_tokens is 16, 32, 64 or 128; head_dim 64, 128 or 256; the page pools are
  * 16-byte aligned.  Nothing needs initialising: a page's scale and codes are
  * written when its first token is.
@@ -743,12 +744,17 @@ KRAKEN_API int kraken_hip_argmax_prob_f32_i32(kraken_hip_context* context, krake
  * position lengths[b] - count + i.  page_table[b][p] is the page that holds
  * positions p * page_tokens on; entries past the length have no effect.
  * max_query and max_keys bound every sequence's new tokens and length; they size
- * the launches and need not be tight.  The arrays are device memory, read when
- * the kernels run, so a captured graph replays with new ones in their place.
+ * the launches.  Loose ones change results by rounding only, but cost time: the
+ * attention splits keys by max_keys and picks its kernels by max_query (a bound of twice
+ * the longest length costs a prompt chunk up to 1.6 times the time and a batch of single
+ * tokens 1.1; far looser ones 2 to 7 times), so a program that captures steps keeps one
+ * graph for each power of two of them.  The arrays are device memory, read when the
+ * kernels run, so a captured graph replays with new ones in their place.
  * A sequence that breaks a bound (query_starts that decrease or pass `tokens`,
  * more new tokens than max_query or its length, a length above max_keys or
- * table_width * page_tokens) is left out: nothing of it is read or written.
- * Rows of no sequence stay as they were.  A page id outside [0, pages) is a
+ * table_width * page_tokens) is left out: nothing of it is read or written.  (Outputs
+ * of rows that two others then claim, behind query_starts that fell back, are not
+ * defined.)  Rows of no sequence stay as they were.  A page id outside [0, pages) is a
  * page without tokens: its keys are not attended and nothing is appended to it.
  * A page that a call appends to must stand once in the batch's tables; pages that
  * are only read may be shared.  Refused are more than 2^31 - 1 pages, tokens or keys of
@@ -792,7 +798,7 @@ typedef struct kraken_paged_batch {
  * last token stay as they were.  A new row with a NaN or an infinity makes its
  * page's scale NaN for that head (its values then read as NaN) until the page is
  * begun again; rows whose largest magnitude is below 127 * 2^-70 (1e-19) are held
- * as zeros.  One launch, no workspace. */
+ * as zeros.  The outputs and the pages overlap no input.  One launch, no workspace. */
 KRAKEN_API int kraken_hip_qwen35_attention_prologue_paged_q8_kv(
   kraken_hip_context* context, kraken_buffer q_gate, kraken_buffer key, kraken_buffer value,
   kraken_buffer q_norm, kraken_buffer k_norm, kraken_buffer positions,
@@ -805,7 +811,9 @@ KRAKEN_API int kraken_hip_qwen35_attention_prologue_paged_q8_kv(
  * 0..p, its own among them (appended before this call), with scale
  * 1 / sqrt(head_dim).  gate.data == NULL: none; else out *= sigmoid(gate).
  * heads is a multiple of kv_heads.  Products keep f32 accuracy: the codes are
- * exact in the matrix cores' f16 and the f32 operands go in as two f16 parts.  A
+ * exact in the matrix cores' f16 and the f32 operands go in as two f16 parts.  That
+ * holds for scores (products times 1 / sqrt(head_dim)) of magnitudes up to 2^20; f32
+ * resolves no weights far beyond, and a row with larger ones is not defined.  A
  * row without any key to attend (all its pages outside the pool) gets zeros.  A NaN
  * or an infinity in a query or in a scale reaches only the rows that use it.
  * query, gate and output are 16-byte aligned; output overlaps neither; up to 67108864
@@ -848,8 +856,9 @@ KRAKEN_API int kraken_hip_dequantize_kv_pages_q8_f16(
  * argmax_f32_i32 does; equal +inf logits share the whole weight.  A NaN
  * temperature draws greedily, NaN top_p and min_p keep all, a uniform outside
  * [0, 1) or NaN is taken as the nearest end (NaN as 0).  Weights are formed in 64
- * bits and summed as integers (2^-44 of the largest up to 262144 tokens), so a
- * result does not depend on the order of the sums.  Up to 65535 rows of up to 4194304
+ * bits and summed as integers (2^-44 of the largest up to 262144 tokens; a token of
+ * less than half of that is not drawn), so a result does not depend on the order of
+ * the sums.  Up to 65535 rows of up to 4194304
  * logits; context workspace of up to 1 GiB (or one row's need). */
 KRAKEN_API int kraken_hip_sample_f32_i32(
   kraken_hip_context* context, kraken_buffer logits, size_t rows, size_t size,

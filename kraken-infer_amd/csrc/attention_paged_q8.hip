@@ -17,7 +17,7 @@
 //    columns, so the high parts take columns 0..7 and the low parts 8..15 of the same
 //    product (kStacked) and the halves are added; a block of 16 rows takes two products.
 //
-// 64 sequences of up to 32768 keys, 2 KV heads of 256 (1.07 GB): 191 us, 5.6 TB/s, of the
+// 64 sequences of up to 32768 keys, 2 KV heads of 256 (1.07 GB): 194 us, 5.5 TB/s, of the
 // 6.95 that a read of as much reaches; the parts are of one size, so the last ones end
 // alone.  One of 4096 keys: 8.6 us and 3.9 for the join, launch and latency (lengths, table,
 // codes, exchange, one after another); its 4.2 MB would take 1.
@@ -34,7 +34,11 @@ namespace {
 
 constexpr uint32_t kWaves = 4;
 
-// Codes of a decode step are read by one workgroup, once.
+// Of sequences with pages of their own and one block of rows each code is read once, which
+// the hint is for (64 of up to 32768 keys: 194 us, 204 without it).  It costs where codes are
+// read again: by further blocks (64 sequences of 8 tokens: 97 us, 87 without) and of a prefix
+// in shared pages (three quarters of the 64 in common: 176 us, 117 without).  The host cannot
+// tell them apart: tables and row counts are the device's.
 __device__ __forceinline__ u32x4_t load_once(const int8_t* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
 }
@@ -479,9 +483,11 @@ PagedSplit split_of(const PagedAttentionArgs& a, int cu_count) {
   const uint64_t rows = group * a.batch.max_query;
   // Keys per workgroup: 128 (a 32-key step for each wave) while all sequences at the
   // longest length make no more than eleven workgroups a CU, else as many as make so few,
-  // up to 4096, but no more than 128 parts of a sequence, which one workgroup joins (one
-  // sequence of 131072 keys: 34 us with 128 parts, 40 with 512, 56 with 1025); more where the
-  // partial results would take over 256 MiB.  (64 sequences of up to 32768 keys, 2 KV heads:
+  // up to 4096; enough for 128 parts of a sequence of up to 524288 keys, which one workgroup
+  // joins (one sequence of 131072 keys: 34 us with 128 parts, 40 with 512, 56 with 1025),
+  // beyond that 4096 all the same; more where the partial results would take over 256 MiB.
+  // All of it goes by max_keys, so that a loose one makes parts too long (1 row, 4096 keys:
+  // 12.8 us, with a bound of 262144 33).  (64 sequences of up to 32768 keys, 2 KV heads:
   // 512 keys 226 us, 1024 205, 1280 197, 1536 194, 2048 205.  One of 4096, 32 workgroups of
   // 128: 12.4 us.)
   const uint64_t lanes = (uint64_t)a.batch.sequences * a.cache.kv_heads;

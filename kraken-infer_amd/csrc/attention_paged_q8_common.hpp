@@ -15,7 +15,11 @@
 // A query row is multiplied by the power of two that takes its largest value to
 // [2^13, 2^14) and goes in as two f16 parts (hi, and what hi leaves), which holds 22
 // bits of each value down to 2^-16 of the row's largest; the weights likewise.  f16
-// queries are exact in the one part, and their weights are rounded once.
+// queries are exact in the one part (what lies below 2^-38 of the row's largest aside).
+// Their weights take one part too where it saves a product (tiles, blocks of 16 rows), in
+// which each is off by at most 2^-12 of itself: the f16 output is then 2.23e-4 of itself off,
+// by its own rounding alone 2.07e-4.  Two parts bring the latter and cost 1024 rows at 8192
+// keys 118 us instead of 100, a batch of 17 sequences 65.6 instead of 61.3.
 #pragma once
 
 #include <hip/hip_runtime.h>

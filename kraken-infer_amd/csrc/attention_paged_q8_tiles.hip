@@ -12,8 +12,8 @@
 // be, and the order in which the pages keep the values.  f32 queries and weights are two
 // f16 parts: a second product with the same operand from LDS.
 //
-// 1024 rows of 8 heads of 256 at 7169 to 8192 keys: f16 99 us (650 TFLOP/s), f32 145 us
-// (890 TFLOP/s of f16 products, two for each).  Of f16's time the vector units are busy for
+// 1024 rows of 8 heads of 256 at 7169 to 8192 keys: f16 100 us (640 TFLOP/s), f32 144 us
+// (900 TFLOP/s of f16 products, two for each).  Of f16's time the vector units are busy for
 // 40 % (the softmax, and codes to f16), the matrix cores for 29 %, and waves wait for 26 %
 // (one wave a SIMD, so that nothing else runs while it does); the clock falls to 1.9 GHz.
 // A workgroup spends 9 us on its query rows and its first tile, and 3 on its results,

@@ -16,11 +16,12 @@
 // rows for keys, runs of eight tokens a dimension for values.  The query heads are further
 // workgroups of the same launch, a wave per token and run of heads.
 //
-// 1024 tokens of 8 query and 2 KV heads of 256 (35 MB with what is read and written, 5 us
-// at the rate of a stream) take about 15 us: the page rows' chain of loads, norm, largest
-// magnitude and codes is as long for one page as for all, and 32 pages of 2 heads are 64
-// long workgroups.  One token takes 4.9 us, of which a launch is 2 to 3.  Reading the pages
-// back as F16 takes 5.9 us for 17 pages, 4.9 for one.
+// 1024 tokens of 8 query and 2 KV heads of 256 (39 MB read and written, 8 us at the rate of
+// a copy) take 13.4 us, the query heads alone (34 MB; page numbers outside the pool) 10.8:
+// the 68 workgroups of pages (17 pages, 2 heads, keys and values) run beside those.  Rows
+// are loaded and stored a dword a lane.  4096 tokens 38.7 us, queries alone 30.  One token
+// takes 6.2 us in a row of calls, 4.8 traced, of which a launch is 2 to 3.  Reading pages
+// of 64 tokens back as F16: one 4.8 us, 17 5.2, 512 18.1 (5.6 TB/s), 2048 84 (4.8).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -61,6 +62,10 @@ __device__ __forceinline__ Rotation rotation_of(const PagedPrologueArgs& a, int 
   return r;
 }
 
+// The angle is reduced to a part of a half turn in 64 bits and rounded to f32 there, which
+// moves it by up to pi 2^-25, three of the sine's own roundings: a rotated query is 6.3e-8
+// of itself off, with 64-bit sines 5.5e-8, and a few key codes in a million take the
+// neighbour.  64-bit sines would be most of a short call's arithmetic.
 __device__ __forceinline__ void sin_cos_of(const PagedPrologueArgs& a, const Rotation& rot,
                                            uint32_t token, uint32_t position, int lane,
                                            float sn[4], float cs[4]) {

@@ -22,12 +22,13 @@
 // So a row is read three times, from memory once (the rest from the caches), and each
 // exponential is formed once but for those of the list and of the drawn chunk.
 //
-// 64 rows of 248320 take 12 + 27 + 18 + 22 us in the four, 72 us together, 8 times the
-// logits' way from memory.  top runs at 5.2 TB/s.  Of bins, the sums of all workgroups in
-// memory are 2 us, counts 3, the exponentials 5, and 18 reading and adding in LDS.
-// gather repeats the scan of the row's histogram in each workgroup.  draw is a chain of
-// some thirty barriers in one workgroup a row, and most of a small call's time (8 rows of
-// 32000: 17 of 26 us).  A launch costs 2 to 3 us, a release to the device within one
+// 64 rows of 248320 take 72 to 76 us by their rules, 6 times the logits' way from memory;
+// traced, which keeps dispatches apart, 12, 27, 18 and 22.  top runs at 5.2 TB/s.  Of bins,
+// the sums of all workgroups in memory are 2 us, counts 3, the exponentials 5, and 18
+// reading and adding in LDS.  gather repeats the scan of the row's histogram in each
+// workgroup.  draw is a chain of some thirty barriers in one workgroup a row, and most of a
+// small call's time (8 rows of 32000: 26 us, draw traced 17; one row of 248320: 28 and
+// 14).  A launch costs 2 to 3 us, a release to the device within one
 // more (31 us instead of 6), so that no launch ends with its last workgroup's join.
 // Several chunks a workgroup, logits asked for ahead of the bounds, and short lists put
 // in order by a network were no faster.

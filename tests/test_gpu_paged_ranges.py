@@ -93,3 +93,29 @@ def test_rows_at_the_least_scale(hip_ctx):
         else:
             assert (got.scales["value"][page] == 0).all()
             assert (got.codes["value"][page] == 0).all()
+
+
+@pytest.mark.parametrize("size", [-1e6, 1e6])
+@pytest.mark.parametrize("new,before", [([1], [0]), ([1, 1, 1], [5, 300, 0]), ([33], [0]),
+                                        ([40, 1, 50], [70, 200, 0])])
+def test_scores_at_the_end_of_their_range(hip_ctx, new, before, size):
+    """Every key the same, with a score near size: a row's output is the mean of the
+    values that it sees (to the f32 roundings of up to 300 equal weights, their codes' two
+    f16 parts and the page scales' exponents beside a maximum of 2^20: its step is 1/8, but
+    the same for all of them, 2^-17)."""
+    rng = np.random.default_rng(63)
+    d, pt = 64, 16
+    batch = Batch(rng, pt, new, before)
+    cache = po.Pages(rng, batch.pages, pt, 1, d)
+    cache.codes["key"][:] = 100
+    cache.scales["key"][:] = 3.0
+    cache.scales["value"][:] = 0.03
+    level = size / (d * 100.0 * 3.0) * math.sqrt(d)
+    query = np.full((batch.tokens, 1, d), level, np.float32)
+    got = run_attention(hip_ctx, cache, batch, 1, query)
+    for b, count in enumerate(new):
+        v = np.concatenate([cache.values_of("value", p) for p in batch.table[b] if p >= 0])[:, 0]
+        for i in range(count):
+            seen = v[:before[b] + i + 1]
+            off = np.abs(got[int(batch.starts[b]) + i, 0] - seen.mean(0))
+            assert (off <= 2.0 ** -17 * np.abs(seen).mean(0)).all(), (b, i)
