@@ -33,6 +33,7 @@ namespace kraken {
 namespace {
 
 constexpr uint32_t kWaves = 4;
+constexpr uint32_t kJoinAcross = 1u << 20;  // workgroups of the join along x
 
 // Of sequences with pages of their own and one block of rows each code is read once, which
 // the hint is for (64 of up to 32768 keys: 194 us, 204 without it).  It costs where codes are
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
 }
 
 // Joins split results: kParts waves per (row, head), which take its parts in turn, D / 64
-// values a lane.
+// values a lane.  (One wave each: four of them a workgroup, along x and then y.)
 template <int D, class T, int kParts>
 __global__ __launch_bounds__(kParts > 4 ? 64 * kParts : 256) void attention_paged_join_kernel(
   PagedAttentionArgs a, PagedSplit split) {
@@ -372,7 +373,9 @@ __global__ __launch_bounds__(kParts > 4 ? 64 * kParts : 256) void attention_page
   __shared__ float lds[kParts > 1 ? kParts : 1][64 * kRegs];
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint64_t item = kParts > 1 ? blockIdx.x : (uint64_t)blockIdx.x * 4u + wave;
+  const uint64_t item =
+    kParts > 1 ? blockIdx.x
+               : ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4u + wave;
   if (item >= (uint64_t)a.batch.tokens * a.heads) {
     return;
   }
@@ -587,8 +590,11 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
   } else if (parts > 8u && items <= 4096u) {
     attention_paged_join_kernel<D, T, 4><<<dim3((uint32_t)items), 256, 0, stream>>>(a, split);
   } else if (parts > 1u) {
-    attention_paged_join_kernel<D, T, 1><<<dim3((uint32_t)((items + 3u) / 4u)), 256, 0, stream>>>(
-      a, split);
+    // A dimension of the grid holds less than 2^32 threads, which 2^26 rows' waves are.
+    const uint32_t blocks = (uint32_t)((items + 3u) / 4u);
+    const uint32_t across = std::min(blocks, kJoinAcross);
+    attention_paged_join_kernel<D, T, 1>
+      <<<dim3(across, (blocks + across - 1u) / across), 256, 0, stream>>>(a, split);
   }
 }
 

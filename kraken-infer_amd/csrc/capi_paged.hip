@@ -16,7 +16,7 @@ namespace {
 
 constexpr size_t kInt32Max = 0x7fffffffu;
 // Limits that keep a launch's workgroups of 256 threads within a grid: pairs of a sequence
-// and a KV head, and rows (tokens x heads), four of which share a workgroup.
+// and a KV head, and rows (tokens x heads), four of which share a workgroup of the join.
 constexpr size_t kMaxPairs = size_t{1} << 20;
 constexpr size_t kMaxRows = size_t{1} << 26;
 

@@ -7,7 +7,8 @@ import pytest
 
 import kraken_hip as kh
 import paged_oracle as po
-from test_gpu_paged_q8 import (EPS, THETA, Batch, check_attention, check_pages, run_prologue)
+from test_gpu_paged_q8 import (EPS, THETA, Batch, DevicePages, check_attention, check_pages,
+                                run_prologue)
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +117,29 @@ def test_sampled_rows_beyond_32_bits(hip_ctx):
         got.append((token, share))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
     assert (got[0][0] >= 0).all()
+
+
+def test_the_most_rows(hip_ctx):
+    """67108864 query rows, the most that the attention takes: two tokens of 1024 heads and
+    65534 rows of no sequence, in a batch that has its results joined.  The rows of no
+    sequence stay as they were."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(83)
+    heads, d, pt, kv = 1024, 64, 16, 256
+    tokens = 65536
+    batch = Batch(rng, pt, [1, 1], [200, 299])
+    cache = po.Pages(rng, batch.pages, pt, kv, d)
+    query = torch.zeros(tokens, heads, d, device="cuda", dtype=torch.float16)
+    query[:2] = torch.from_numpy(rng.standard_normal((2, heads, d)).astype(np.float16)).cuda()
+    out = torch.full((tokens, heads, d), -77.0, device="cuda", dtype=torch.float16)
+    batch.tokens = tokens
+    pages, tables = DevicePages(hip_ctx, cache), batch.device(hip_ctx)
+    torch.cuda.synchronize()
+    hip_ctx.attention_f16q_paged_q8_kv(query, pages.struct, tables, heads, out)
+    torch.cuda.synchronize()
+    got, held = out[:2].cpu().numpy().astype(np.float64), query[:2].cpu().numpy()
+    assert bool((out[2:] == -77).all())
+    batch.tokens = 2
+    want, size, score = po.attention(cache, held, batch.plain(), heads)
+    tol = po.attention_tolerance(size, want, score, d, True)
+    assert (np.abs(got - want) <= tol).all()
