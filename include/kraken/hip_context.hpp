@@ -883,6 +883,80 @@ class HipContext {
       min_p.raw(), uniforms.raw(), token_output.raw(), probability_output.raw()));
   }
 
+  // Shared prefixes, eviction and log probabilities (no MpsContext counterpart; see
+  // kraken_hip.h).  gate, the weights of gather_kv_pages_q8, temperature, tokens and the
+  // outputs of token_logprobs_f32 may be invalid (default) buffers.
+  [[nodiscard]] Status attention_f32_shared_paged_q8_kv(
+    const HipBuffer& query, const HipBuffer& gate, const kraken_paged_q8_cache& cache,
+    const kraken_paged_batch& batch, const kraken_shared_prefixes& prefixes, std::size_t heads,
+    HipBuffer& output) const {
+    return Status::from_code(kraken_hip_attention_f32_shared_paged_q8_kv(
+      ctx_, query.raw(), gate.raw(), &cache, &batch, &prefixes, heads, output.raw()));
+  }
+  [[nodiscard]] Status attention_f16q_shared_paged_q8_kv(
+    const HipBuffer& query, const kraken_paged_q8_cache& cache, const kraken_paged_batch& batch,
+    const kraken_shared_prefixes& prefixes, std::size_t heads, HipBuffer& output) const {
+    return Status::from_code(kraken_hip_attention_f16q_shared_paged_q8_kv(
+      ctx_, query.raw(), &cache, &batch, &prefixes, heads, output.raw()));
+  }
+  [[nodiscard]] Status key_weights_f32_paged_q8_kv(const HipBuffer& query,
+                                                   const kraken_paged_q8_cache& cache,
+                                                   const kraken_paged_batch& batch,
+                                                   std::size_t heads, std::size_t window,
+                                                   float decay, HipBuffer& key_weights,
+                                                   std::size_t weight_stride) const {
+    return Status::from_code(kraken_hip_key_weights_f32_paged_q8_kv(
+      ctx_, query.raw(), &cache, &batch, heads, window, decay, key_weights.raw(),
+      weight_stride));
+  }
+  [[nodiscard]] Status key_weights_f16q_paged_q8_kv(const HipBuffer& query,
+                                                    const kraken_paged_q8_cache& cache,
+                                                    const kraken_paged_batch& batch,
+                                                    std::size_t heads, std::size_t window,
+                                                    float decay, HipBuffer& key_weights,
+                                                    std::size_t weight_stride) const {
+    return Status::from_code(kraken_hip_key_weights_f16q_paged_q8_kv(
+      ctx_, query.raw(), &cache, &batch, heads, window, decay, key_weights.raw(),
+      weight_stride));
+  }
+  [[nodiscard]] Status select_keys_f32_i32(const HipBuffer& key_weights,
+                                           std::size_t weight_stride, const HipBuffer& lengths,
+                                           const HipBuffer& keep, std::size_t sequences,
+                                           std::size_t kv_heads, std::size_t max_keys,
+                                           std::size_t first, std::size_t last,
+                                           HipBuffer& kept_output, std::size_t kept_stride,
+                                           HipBuffer& kept_lengths) const {
+    return Status::from_code(kraken_hip_select_keys_f32_i32(
+      ctx_, key_weights.raw(), weight_stride, lengths.raw(), keep.raw(), sequences, kv_heads,
+      max_keys, first, last, kept_output.raw(), kept_stride, kept_lengths.raw()));
+  }
+  [[nodiscard]] Status gather_kv_pages_q8(const kraken_paged_q8_cache& cache,
+                                          const HipBuffer& page_table, std::size_t table_width,
+                                          const HipBuffer& kept, const HipBuffer& kept_lengths,
+                                          std::size_t kept_stride, std::size_t sequences,
+                                          const HipBuffer& target_table,
+                                          std::size_t target_width,
+                                          const HipBuffer& key_weights,
+                                          std::size_t weight_stride,
+                                          HipBuffer& weights_output) const {
+    return Status::from_code(kraken_hip_gather_kv_pages_q8(
+      ctx_, &cache, page_table.raw(), table_width, kept.raw(), kept_lengths.raw(), kept_stride,
+      sequences, target_table.raw(), target_width, key_weights.raw(), weight_stride,
+      weights_output.raw()));
+  }
+  [[nodiscard]] Status token_logprobs_f32(const HipBuffer& logits, std::size_t rows,
+                                          std::size_t size, std::size_t row_stride,
+                                          const HipBuffer& temperature, const HipBuffer& tokens,
+                                          std::size_t top, HipBuffer& logprob_output,
+                                          HipBuffer& rank_output, HipBuffer& entropy_output,
+                                          HipBuffer& top_token_output,
+                                          HipBuffer& top_logprob_output) const {
+    return Status::from_code(kraken_hip_token_logprobs_f32(
+      ctx_, logits.raw(), rows, size, row_stride, temperature.raw(), tokens.raw(), top,
+      logprob_output.raw(), rank_output.raw(), entropy_output.raw(), top_token_output.raw(),
+      top_logprob_output.raw()));
+  }
+
  private:
   explicit HipContext(kraken_hip_context* raw) : ctx_(raw) {}
 

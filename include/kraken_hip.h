@@ -866,6 +866,128 @@ KRAKEN_API int kraken_hip_sample_f32_i32(
   kraken_buffer min_p, kraken_buffer uniforms, kraken_buffer token_output,
   kraken_buffer probability_output);
 
+/* Sequences of a batch that begin alike: group g is its sequences group_starts[g] ..
+ * group_starts[g + 1] - 1, the first prefix_lengths[g] tokens of each stand in the same
+ * pages, and what is read of them is the first such sequence's row of page_table.  Of a
+ * prefix count whole pages, and of these what lies before the new tokens of every
+ * sequence of the group that brings any.  max_rows bounds a group's new tokens, all its
+ * sequences' together, max_prefix its prefix; groups are at most the batch's sequences.
+ * A group that breaks a bound (group_starts that decrease or pass `sequences`, more new
+ * tokens than max_rows, a prefix above max_prefix, a sequence's rows outside those from
+ * the group's first to its last) shares nothing: its sequences are attended each by
+ * itself, as those of no group are.  (Outputs of a sequence that two groups claim are not
+ * defined.)  The arrays are device memory, read when the kernels run. */
+typedef struct kraken_shared_prefixes {
+  kraken_buffer group_starts;   /* uint32 [groups + 1] */
+  kraken_buffer prefix_lengths; /* uint32 [groups] */
+  size_t groups;
+  size_t max_rows;
+  size_t max_prefix;
+} kraken_shared_prefixes;
+
+/* kraken_hip_attention_f32_paged_q8_kv and kraken_hip_attention_f16q_paged_q8_kv of a
+ * batch whose sequences share prefixes: the same outputs to rounding, with each shared
+ * page read for all rows of its group at once instead of once for each sequence.  Up to
+ * 1048576 rows (tokens * heads); what the plain entries require holds here too.  Uses
+ * context workspace (at most about 512 MiB beside the rows' own partial results,
+ * 8 * head_dim + 64 bytes for each). */
+KRAKEN_API int kraken_hip_attention_f32_shared_paged_q8_kv(
+  kraken_hip_context* context, kraken_buffer query, kraken_buffer gate,
+  const kraken_paged_q8_cache* cache, const kraken_paged_batch* batch,
+  const kraken_shared_prefixes* prefixes, size_t heads, kraken_buffer output);
+KRAKEN_API int kraken_hip_attention_f16q_shared_paged_q8_kv(
+  kraken_hip_context* context, kraken_buffer query, const kraken_paged_q8_cache* cache,
+  const kraken_paged_batch* batch, const kraken_shared_prefixes* prefixes, size_t heads,
+  kraken_buffer output);
+
+/* The attention weight that cached keys receive: for each sequence b of the batch that
+ * brings tokens, each KV head h and each position j below its length,
+ *   key_weights[b][h][j] = decay * key_weights[b][h][j] + sum of p(r, g, j)
+ * over the last `window` (0: all) of its new rows r and the query heads g of h, where p
+ * is the weight that kraken_hip_attention_f32_paged_q8_kv gives key j in row r (its own
+ * and all before it are attended).  Positions of this batch's new tokens have no earlier
+ * weight, and with decay 0 no earlier weight is read: nothing needs initialising.
+ * key_weights is f32 [sequences][kv_heads][weight_stride]; positions from the length on
+ * stay as they were, as do sequences that bring no tokens, break a bound of the batch or
+ * are longer than weight_stride.  A key outside the pool receives nothing.  query is as
+ * for the attention, f32 or f16; the weights keep f32 accuracy in both, by the same
+ * limits, and their sums have one order whatever else the batch holds.  A NaN or an
+ * infinity in a query or a scale reaches all weights of its sequence and KV head.  decay
+ * is finite and not negative.  query is 16-byte aligned; key_weights overlaps no input.
+ * Up to 67108864 rows (tokens * heads).  Uses context workspace. */
+KRAKEN_API int kraken_hip_key_weights_f32_paged_q8_kv(
+  kraken_hip_context* context, kraken_buffer query, const kraken_paged_q8_cache* cache,
+  const kraken_paged_batch* batch, size_t heads, size_t window, float decay,
+  kraken_buffer key_weights, size_t weight_stride);
+KRAKEN_API int kraken_hip_key_weights_f16q_paged_q8_kv(
+  kraken_hip_context* context, kraken_buffer query, const kraken_paged_q8_cache* cache,
+  const kraken_paged_batch* batch, size_t heads, size_t window, float decay,
+  kraken_buffer key_weights, size_t weight_stride);
+
+/* The positions that a cache keeps: for each sequence b, n = lengths[b] tokens long, and
+ * each KV head, k = min(keep[b], n) of them: the newest min(last, k), then the first up
+ * to `first`, then the largest key_weights of those between (equal ones: the lower
+ * position first; NaN below all others).  kept_output int32
+ * [sequences][kv_heads][kept_stride] receives them in rising order and kept_lengths uint32
+ * [sequences] receives k; entries from k on stay as they were.  A sequence longer than
+ * max_keys, or with k above kept_stride, is left out: neither output of it is written.
+ * lengths and keep are uint32 [sequences] in device memory, key_weights f32
+ * [sequences][kv_heads][weight_stride] with weight_stride >= max_keys.  Up to 1048576
+ * pairs of a sequence and a KV head, and 2^31 - 1 positions. */
+KRAKEN_API int kraken_hip_select_keys_f32_i32(
+  kraken_hip_context* context, kraken_buffer key_weights, size_t weight_stride,
+  kraken_buffer lengths, kraken_buffer keep, size_t sequences, size_t kv_heads,
+  size_t max_keys, size_t first, size_t last, kraken_buffer kept_output, size_t kept_stride,
+  kraken_buffer kept_lengths);
+
+/* Moves tokens of paged sequences into other pages of the pool, each KV head its own:
+ * slot i of sequence b and KV head h, in the page target_table[b][i / page_tokens],
+ * becomes a copy of position kept[b][h][i] of page_table[b], for i below
+ * kept_lengths[b].  A target page's scale becomes the largest of its sources' (of keys and
+ * values apart) and a code that came with scale s becomes code * (s / scale), rounded to
+ * even: equal scales move bits, and no value moves by more than half a step of its new
+ * page.  A source whose scale is not finite makes its target page's scale NaN for that
+ * head and keeps its codes.  A position outside the table's pages or a page outside the
+ * pool gives zeros; codes behind the last kept token of its page become zeros.  A target
+ * page outside the pool is not written.  page_table is int32 [sequences][table_width],
+ * target_table int32 [sequences][target_width], kept int32
+ * [sequences][kv_heads][kept_stride], kept_lengths uint32 [sequences]; a sequence whose
+ * kept_lengths[b] passes kept_stride or target_width * page_tokens is left out.
+ * A target page stands once in target_table and is no source page: shared pages stay as
+ * they are, and the sequence's old ones are free once this has run.
+ * With key_weights given (f32 [sequences][kv_heads][weight_stride]), weights_output, laid
+ * out alike, receives their values at the kept positions in its first kept_lengths[b]
+ * entries (a position from weight_stride on: zero); a sequence with kept_lengths[b] above
+ * weight_stride is then left out.  Both are empty otherwise.  Outputs overlap no input. */
+KRAKEN_API int kraken_hip_gather_kv_pages_q8(
+  kraken_hip_context* context, const kraken_paged_q8_cache* cache, kraken_buffer page_table,
+  size_t table_width, kraken_buffer kept, kraken_buffer kept_lengths, size_t kept_stride,
+  size_t sequences, kraken_buffer target_table, size_t target_width,
+  kraken_buffer key_weights, size_t weight_stride, kraken_buffer weights_output);
+
+/* Log probabilities of `rows` rows of logits f32 [rows][row_stride], the first `size` of a
+ * row, under softmax(logits / temperature); temperature f32 [rows], an empty buffer or
+ * one that is not above zero (or NaN) stands for 1.  In order of falling logit (equal
+ * ones: the lower index first):
+ *   logprob_output f32 and rank_output int32 [rows]: of the token tokens[row] (int32),
+ *     and its place in that order, the likeliest being 0; a token outside [0, size) gets
+ *     -inf and `size`
+ *   entropy_output f32 [rows]: of the row, in nats
+ *   top_token_output int32 and top_logprob_output f32 [rows][top]: the first `top` tokens
+ *     of that order, up to 32; entries past the last token get `size` and -inf
+ * Any output may be empty, but not all; tokens is given with logprob_output or
+ * rank_output, and top is 0 exactly where both of its outputs are empty.  NaN logits
+ * count as no token (-inf; they stand last, behind -inf, by index, and are never among
+ * the top), equal +inf logits share the whole weight, and a row without a logit above -inf
+ * has entropy 0 and -inf throughout.  Sums leave the largest logit out, so that values
+ * near zero keep f32's relative accuracy.  Up to 65535 rows of up to 4194304 logits.
+ * Uses context workspace. */
+KRAKEN_API int kraken_hip_token_logprobs_f32(
+  kraken_hip_context* context, kraken_buffer logits, size_t rows, size_t size,
+  size_t row_stride, kraken_buffer temperature, kraken_buffer tokens, size_t top,
+  kraken_buffer logprob_output, kraken_buffer rank_output, kraken_buffer entropy_output,
+  kraken_buffer top_token_output, kraken_buffer top_logprob_output);
+
 #ifdef __cplusplus
 }
 #endif

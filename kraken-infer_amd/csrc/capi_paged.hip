@@ -1,4 +1,4 @@
-// C entry points over a paged 8-bit KV cache, and sampling: argument checks in the
+// C entry points over a paged 8-bit KV cache, sampling and log probabilities: argument checks in the
 // order of the other entries (dimensions, bounds, overflow, buffers, uint32 ranges),
 // then one launch function each.
 #include <hip/hip_runtime.h>
@@ -19,6 +19,8 @@ constexpr size_t kInt32Max = 0x7fffffffu;
 // and a KV head, and rows (tokens x heads), four of which share a workgroup of the join.
 constexpr size_t kMaxPairs = size_t{1} << 20;
 constexpr size_t kMaxRows = size_t{1} << 26;
+// Each row of a shared prefix has partial results of its own.
+constexpr size_t kMaxSharedRows = size_t{1} << 20;
 
 int refuse(const char* w, const char* what) { return invalid(std::string("HIP ") + w + what); }
 
@@ -115,6 +117,48 @@ int finish(kraken_hip_context* ctx, hipError_t e, const char* w) {
   return finish_launch(ctx, "HIP ", w, " command failed: ");
 }
 
+// The checks of an attention's rows over a batch: query, gate and output.
+int attention_args(const kraken_buffer& query, const kraken_buffer& gate,
+                   const kraken_paged_q8_cache* cache, const kraken_paged_batch* batch,
+                   size_t heads, const kraken_buffer* output, bool f16, size_t max_rows,
+                   const char* w, PagedAttentionArgs& a) {
+  if (heads == 0) {
+    return refuse(w, " dimensions must be positive");
+  }
+  KRAKEN_TRY(cache_args(cache, w, a.cache));
+  if (heads % cache->kv_heads != 0) {
+    return refuse(w, " heads must be divisible by kv_heads");
+  }
+  KRAKEN_TRY(batch_args(batch, cache->kv_heads, w, a.batch));
+  size_t rows = 0, values = 0;
+  if (!checked_mul(batch->tokens, heads, rows) || !checked_mul(rows, cache->head_dim, values)) {
+    return refuse(w, " value count overflow");
+  }
+  if (rows > max_rows) {
+    return invalid(std::string("HIP ") + w + " takes up to " + std::to_string(max_rows) +
+                   " query rows");
+  }
+  const size_t element = f16 ? sizeof(uint16_t) : sizeof(float);
+  KRAKEN_TRY(validate_buffer(query, values, element, w, " query"));
+  if (gate.data != nullptr) {
+    KRAKEN_TRY(validate_f32(gate, values, w, " gate"));
+  }
+  uintptr_t places = (uintptr_t)query.data | (uintptr_t)gate.data;
+  if (output != nullptr) {
+    KRAKEN_TRY(validate_buffer(*output, values, element, w, " output"));
+    places |= (uintptr_t)output->data;
+    a.output = output->data;
+  }
+  if (places & 15u) {
+    return refuse(w, " buffers must be 16-byte aligned");
+  }
+  a.query = query.data;
+  a.gate = static_cast<const float*>(gate.data);
+  a.heads = (uint32_t)heads;
+  a.f16 = f16;
+  return KRAKEN_OK;
+}
+
 int paged_attention_entry(kraken_hip_context* ctx, const kraken_buffer& query,
                           const kraken_buffer& gate, const kraken_paged_q8_cache* cache,
                           const kraken_paged_batch* batch, size_t heads,
@@ -122,38 +166,83 @@ int paged_attention_entry(kraken_hip_context* ctx, const kraken_buffer& query,
   const char* w = "paged attention";
   KRAKEN_TRY(check_context(ctx));
   PagedAttentionArgs a{};
-  if (heads == 0) {
-    return invalid("HIP paged attention dimensions must be positive");
-  }
-  KRAKEN_TRY(cache_args(cache, w, a.cache));
-  if (heads % cache->kv_heads != 0) {
-    return invalid("HIP paged attention heads must be divisible by kv_heads");
-  }
-  KRAKEN_TRY(batch_args(batch, cache->kv_heads, w, a.batch));
-  size_t rows = 0, values = 0;
-  if (!checked_mul(batch->tokens, heads, rows) || !checked_mul(rows, cache->head_dim, values)) {
-    return invalid("HIP paged attention value count overflow");
-  }
-  if (rows > kMaxRows) {
-    return invalid("HIP paged attention takes up to 67108864 query rows");
-  }
-  const size_t element = f16 ? sizeof(uint16_t) : sizeof(float);
-  KRAKEN_TRY(validate_buffer(query, values, element, w, " query"));
-  if (gate.data != nullptr) {
-    KRAKEN_TRY(validate_f32(gate, values, w, " gate"));
-  }
-  KRAKEN_TRY(validate_buffer(output, values, element, w, " output"));
-  if (((uintptr_t)query.data | (uintptr_t)gate.data | (uintptr_t)output.data) & 15u) {
-    return invalid("HIP paged attention buffers must be 16-byte aligned");
-  }
-  a.query = query.data;
-  a.gate = static_cast<const float*>(gate.data);
-  a.output = output.data;
-  a.heads = (uint32_t)heads;
-  a.f16 = f16;
+  KRAKEN_TRY(attention_args(query, gate, cache, batch, heads, &output, f16, kMaxRows, w, a));
   KRAKEN_TRY(begin_launch(ctx));
   KRAKEN_TRY(ensure_workspace(ctx, attention_paged_q8_workspace_bytes(a, ctx->cu_count)));
   return finish(ctx, launch_attention_paged_q8(a, ctx->cu_count, ctx->workspace, ctx->stream), w);
+}
+
+int shared_attention_entry(kraken_hip_context* ctx, const kraken_buffer& query,
+                           const kraken_buffer& gate, const kraken_paged_q8_cache* cache,
+                           const kraken_paged_batch* batch,
+                           const kraken_shared_prefixes* prefixes, size_t heads,
+                           const kraken_buffer& output, bool f16) {
+  const char* w = "shared paged attention";
+  KRAKEN_TRY(check_context(ctx));
+  PagedAttentionArgs a{};
+  KRAKEN_TRY(
+    attention_args(query, gate, cache, batch, heads, &output, f16, kMaxSharedRows, w, a));
+  if (prefixes == nullptr) {
+    return refuse(w, " prefixes must not be null");
+  }
+  if (prefixes->groups == 0 || prefixes->max_rows == 0 || prefixes->max_prefix == 0) {
+    return refuse(w, " prefix dimensions must be positive");
+  }
+  if (prefixes->groups > batch->sequences) {
+    return refuse(w, " takes no more groups than sequences");
+  }
+  KRAKEN_TRY(validate_buffer(prefixes->group_starts, prefixes->groups + 1u, sizeof(uint32_t), w,
+                             " group starts"));
+  KRAKEN_TRY(validate_buffer(prefixes->prefix_lengths, prefixes->groups, sizeof(uint32_t), w,
+                             " prefix lengths"));
+  SharedPrefixArgs p{};
+  p.starts = static_cast<const uint32_t*>(prefixes->group_starts.data);
+  p.lengths = static_cast<const uint32_t*>(prefixes->prefix_lengths.data);
+  p.groups = (uint32_t)prefixes->groups;
+  // No group can have more than either.
+  p.max_rows = (uint32_t)std::min(prefixes->max_rows, batch->tokens);
+  p.max_prefix = (uint32_t)std::min(prefixes->max_prefix, batch->max_keys);
+  KRAKEN_TRY(begin_launch(ctx));
+  KRAKEN_TRY(ensure_workspace(ctx, attention_shared_q8_workspace_bytes(a, p, ctx->cu_count)));
+  return finish(
+    ctx, launch_attention_shared_q8(a, p, ctx->cu_count, ctx->workspace, ctx->stream), w);
+}
+
+int key_weights_entry(kraken_hip_context* ctx, const kraken_buffer& query,
+                      const kraken_paged_q8_cache* cache, const kraken_paged_batch* batch,
+                      size_t heads, size_t window, float decay, const kraken_buffer& weights,
+                      size_t stride, bool f16) {
+  const char* w = "key weights";
+  KRAKEN_TRY(check_context(ctx));
+  KeyWeightsArgs a{};
+  KRAKEN_TRY(attention_args(query, kraken_buffer{nullptr, 0}, cache, batch, heads, nullptr, f16,
+                            kMaxRows, w, a.rows));
+  if (!(decay >= 0.0f) || std::isinf(decay)) {
+    return refuse(w, " decay must be finite and not negative");
+  }
+  if (stride == 0) {
+    return refuse(w, " stride must be positive");
+  }
+  size_t pairs = 0, values = 0;
+  if (!checked_mul(batch->sequences, cache->kv_heads, pairs) ||
+      !checked_mul(pairs, stride, values)) {
+    return refuse(w, " value count overflow");
+  }
+  KRAKEN_TRY(validate_f32(weights, values, w, " output"));
+  a.window = (uint32_t)std::min(window == 0 ? kInt32Max : window, kInt32Max);
+  a.decay = decay;
+  a.weights = static_cast<float*>(weights.data);
+  a.stride = (uint32_t)std::min(stride, kInt32Max);
+  a.row_stride = stride;
+  KRAKEN_TRY(begin_launch(ctx));
+  KRAKEN_TRY(ensure_workspace(ctx, key_weights_workspace_bytes(a, ctx->cu_count)));
+  return finish(ctx, launch_key_weights(a, ctx->cu_count, ctx->workspace, ctx->stream), w);
+}
+
+// Whether two buffers share bytes.
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + b_bytes && y < x + a_bytes;
 }
 
 }  // namespace
@@ -331,6 +420,214 @@ KRAKEN_API int kraken_hip_sample_f32_i32(kraken_hip_context* ctx, kraken_buffer 
   KRAKEN_TRY(begin_launch(ctx));
   KRAKEN_TRY(ensure_workspace(ctx, sample_workspace_bytes(a)));
   return finish(ctx, launch_sample(a, ctx->workspace, ctx->stream), w);
+}
+
+KRAKEN_API int kraken_hip_attention_f32_shared_paged_q8_kv(
+  kraken_hip_context* ctx, kraken_buffer query, kraken_buffer gate,
+  const kraken_paged_q8_cache* cache, const kraken_paged_batch* batch,
+  const kraken_shared_prefixes* prefixes, size_t heads, kraken_buffer output) {
+  return shared_attention_entry(ctx, query, gate, cache, batch, prefixes, heads, output, false);
+}
+
+KRAKEN_API int kraken_hip_attention_f16q_shared_paged_q8_kv(
+  kraken_hip_context* ctx, kraken_buffer query, const kraken_paged_q8_cache* cache,
+  const kraken_paged_batch* batch, const kraken_shared_prefixes* prefixes, size_t heads,
+  kraken_buffer output) {
+  return shared_attention_entry(ctx, query, kraken_buffer{nullptr, 0}, cache, batch, prefixes,
+                                heads, output, true);
+}
+
+KRAKEN_API int kraken_hip_key_weights_f32_paged_q8_kv(
+  kraken_hip_context* ctx, kraken_buffer query, const kraken_paged_q8_cache* cache,
+  const kraken_paged_batch* batch, size_t heads, size_t window, float decay,
+  kraken_buffer key_weights, size_t weight_stride) {
+  return key_weights_entry(ctx, query, cache, batch, heads, window, decay, key_weights,
+                           weight_stride, false);
+}
+
+KRAKEN_API int kraken_hip_key_weights_f16q_paged_q8_kv(
+  kraken_hip_context* ctx, kraken_buffer query, const kraken_paged_q8_cache* cache,
+  const kraken_paged_batch* batch, size_t heads, size_t window, float decay,
+  kraken_buffer key_weights, size_t weight_stride) {
+  return key_weights_entry(ctx, query, cache, batch, heads, window, decay, key_weights,
+                           weight_stride, true);
+}
+
+KRAKEN_API int kraken_hip_select_keys_f32_i32(
+  kraken_hip_context* ctx, kraken_buffer key_weights, size_t weight_stride,
+  kraken_buffer lengths, kraken_buffer keep, size_t sequences, size_t kv_heads,
+  size_t max_keys, size_t first, size_t last, kraken_buffer kept_output, size_t kept_stride,
+  kraken_buffer kept_lengths) {
+  const char* w = "select keys";
+  KRAKEN_TRY(check_context(ctx));
+  if (sequences == 0 || kv_heads == 0 || max_keys == 0 || kept_stride == 0) {
+    return refuse(w, " dimensions must be positive");
+  }
+  if (max_keys > kInt32Max) {
+    return refuse(w, " keys exceed int32 range");
+  }
+  if (kv_heads > kMaxPairs || sequences > kMaxPairs / kv_heads) {
+    return refuse(w, " takes up to 1048576 pairs of a sequence and a KV head");
+  }
+  if (weight_stride < max_keys) {
+    return refuse(w, " weight stride must be at least max_keys");
+  }
+  const size_t pairs = sequences * kv_heads;
+  size_t values = 0, places = 0;
+  if (!checked_mul(pairs, weight_stride, values) || !checked_mul(pairs, kept_stride, places)) {
+    return refuse(w, " value count overflow");
+  }
+  KRAKEN_TRY(validate_f32(key_weights, values, w, " weights"));
+  KRAKEN_TRY(validate_buffer(lengths, sequences, sizeof(uint32_t), w, " lengths"));
+  KRAKEN_TRY(validate_buffer(keep, sequences, sizeof(uint32_t), w, " keep"));
+  KRAKEN_TRY(validate_buffer(kept_output, places, sizeof(int32_t), w, " output"));
+  KRAKEN_TRY(validate_buffer(kept_lengths, sequences, sizeof(uint32_t), w, " output lengths"));
+  SelectKeysArgs a{};
+  a.weights = static_cast<const float*>(key_weights.data);
+  a.lengths = static_cast<const uint32_t*>(lengths.data);
+  a.keep = static_cast<const uint32_t*>(keep.data);
+  a.kept = static_cast<int32_t*>(kept_output.data);
+  a.kept_lengths = static_cast<uint32_t*>(kept_lengths.data);
+  a.weight_stride = weight_stride;
+  a.kept_stride = kept_stride;
+  a.sequences = (uint32_t)sequences;
+  a.kv_heads = (uint32_t)kv_heads;
+  a.max_keys = (uint32_t)max_keys;
+  a.first = (uint32_t)std::min(first, kInt32Max);
+  a.last = (uint32_t)std::min(last, kInt32Max);
+  KRAKEN_TRY(begin_launch(ctx));
+  return finish(ctx, launch_select_keys(a, ctx->stream), w);
+}
+
+KRAKEN_API int kraken_hip_gather_kv_pages_q8(
+  kraken_hip_context* ctx, const kraken_paged_q8_cache* cache, kraken_buffer page_table,
+  size_t table_width, kraken_buffer kept, kraken_buffer kept_lengths, size_t kept_stride,
+  size_t sequences, kraken_buffer target_table, size_t target_width,
+  kraken_buffer key_weights, size_t weight_stride, kraken_buffer weights_output) {
+  const char* w = "KV page gather";
+  KRAKEN_TRY(check_context(ctx));
+  GatherPagesArgs a{};
+  KRAKEN_TRY(cache_args(cache, w, a.cache));
+  if (table_width == 0 || kept_stride == 0 || sequences == 0 || target_width == 0) {
+    return refuse(w, " dimensions must be positive");
+  }
+  if (sequences > kMaxPairs / cache->kv_heads) {
+    return refuse(w, " takes up to 1048576 pairs of a sequence and a KV head");
+  }
+  if (table_width > kInt32Max || target_width > kInt32Max) {
+    return refuse(w, " table width exceeds int32 range");
+  }
+  const size_t pairs = sequences * cache->kv_heads;
+  size_t sources = 0, targets = 0, places = 0;
+  if (!checked_mul(sequences, table_width, sources) ||
+      !checked_mul(sequences, target_width, targets) ||
+      !checked_mul(pairs, kept_stride, places)) {
+    return refuse(w, " value count overflow");
+  }
+  KRAKEN_TRY(validate_buffer(page_table, sources, sizeof(int32_t), w, " page table"));
+  KRAKEN_TRY(validate_buffer(kept, places, sizeof(int32_t), w, " positions"));
+  KRAKEN_TRY(validate_buffer(kept_lengths, sequences, sizeof(uint32_t), w, " lengths"));
+  KRAKEN_TRY(validate_buffer(target_table, targets, sizeof(int32_t), w, " target table"));
+  if ((key_weights.data == nullptr) != (weights_output.data == nullptr)) {
+    return refuse(w, " takes weights and their output together");
+  }
+  if (key_weights.data != nullptr) {
+    size_t values = 0;
+    if (weight_stride == 0) {
+      return refuse(w, " weight stride must be positive");
+    }
+    if (!checked_mul(pairs, weight_stride, values)) {
+      return refuse(w, " value count overflow");
+    }
+    KRAKEN_TRY(validate_f32(key_weights, values, w, " weights"));
+    KRAKEN_TRY(validate_f32(weights_output, values, w, " weights output"));
+    if (overlap(key_weights.data, values * sizeof(float), weights_output.data,
+                values * sizeof(float))) {
+      return refuse(w, " weights output must not overlap the weights");
+    }
+  }
+  a.table = static_cast<const int32_t*>(page_table.data);
+  a.target_table = static_cast<const int32_t*>(target_table.data);
+  a.kept = static_cast<const int32_t*>(kept.data);
+  a.kept_lengths = static_cast<const uint32_t*>(kept_lengths.data);
+  a.weights = static_cast<const float*>(key_weights.data);
+  a.weights_output = static_cast<float*>(weights_output.data);
+  a.kept_stride = kept_stride;
+  a.weight_stride = weight_stride;
+  a.sequences = (uint32_t)sequences;
+  a.width = (uint32_t)table_width;
+  a.target_width = (uint32_t)target_width;
+  KRAKEN_TRY(begin_launch(ctx));
+  return finish(ctx, launch_gather_pages(a, ctx->stream), w);
+}
+
+KRAKEN_API int kraken_hip_token_logprobs_f32(
+  kraken_hip_context* ctx, kraken_buffer logits, size_t rows, size_t size, size_t row_stride,
+  kraken_buffer temperature, kraken_buffer tokens, size_t top, kraken_buffer logprob_output,
+  kraken_buffer rank_output, kraken_buffer entropy_output, kraken_buffer top_token_output,
+  kraken_buffer top_logprob_output) {
+  const char* w = "token logprobs";
+  KRAKEN_TRY(check_context(ctx));
+  if (rows == 0 || size == 0) {
+    return refuse(w, " dimensions must be positive");
+  }
+  if (row_stride < size) {
+    return refuse(w, " row stride must be at least the row size");
+  }
+  size_t values = 0;
+  if (!checked_mul(rows - 1u, row_stride, values) || !checked_add(values, size, values)) {
+    return refuse(w, " value count overflow");
+  }
+  if (size > (size_t{1} << 22) || rows > 65535u) {
+    return refuse(w, " takes rows of up to 4194304 logits, and 65535 of them");
+  }
+  if (top > kMaxTopLogprobs) {
+    return refuse(w, " lists up to 32 tokens");
+  }
+  KRAKEN_TRY(validate_f32(logits, values, w, " logits"));
+  const bool given = logprob_output.data != nullptr || rank_output.data != nullptr;
+  const bool listed = top_token_output.data != nullptr || top_logprob_output.data != nullptr;
+  if (!given && !listed && entropy_output.data == nullptr) {
+    return refuse(w, " has no output");
+  }
+  if (given != (tokens.data != nullptr)) {
+    return refuse(w, " takes tokens exactly with their outputs");
+  }
+  if (listed != (top != 0)) {
+    return refuse(w, " takes a number of top tokens exactly with their outputs");
+  }
+  const struct {
+    const kraken_buffer& buffer;
+    size_t values;
+    const char* name;
+  } optional[] = {{temperature, rows, " temperature"},
+                  {tokens, rows, " tokens"},
+                  {logprob_output, rows, " logprob output"},
+                  {rank_output, rows, " rank output"},
+                  {entropy_output, rows, " entropy output"},
+                  {top_token_output, rows * top, " top token output"},
+                  {top_logprob_output, rows * top, " top logprob output"}};
+  for (const auto& o : optional) {
+    if (o.buffer.data != nullptr) {
+      KRAKEN_TRY(validate_buffer(o.buffer, o.values, 4u, w, o.name));
+    }
+  }
+  LogprobsArgs a{};
+  a.logits = static_cast<const float*>(logits.data);
+  a.temperature = static_cast<const float*>(temperature.data);
+  a.tokens = static_cast<const int32_t*>(tokens.data);
+  a.logprobs = static_cast<float*>(logprob_output.data);
+  a.ranks = static_cast<int32_t*>(rank_output.data);
+  a.entropies = static_cast<float*>(entropy_output.data);
+  a.top_tokens = static_cast<int32_t*>(top_token_output.data);
+  a.top_logprobs = static_cast<float*>(top_logprob_output.data);
+  a.row_stride = row_stride;
+  a.rows = (uint32_t)rows;
+  a.size = (uint32_t)size;
+  a.top = (uint32_t)top;
+  KRAKEN_TRY(begin_launch(ctx));
+  KRAKEN_TRY(ensure_workspace(ctx, token_logprobs_workspace_bytes(a)));
+  return finish(ctx, launch_token_logprobs(a, ctx->workspace, ctx->stream), w);
 }
 
 }  // extern "C"

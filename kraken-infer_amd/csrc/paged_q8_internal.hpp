@@ -71,12 +71,76 @@ struct SampleArgs {
   uint32_t rows, size;
 };
 
+// kraken_shared_prefixes with device pointers.
+struct SharedPrefixArgs {
+  const uint32_t* starts;   // [groups + 1]
+  const uint32_t* lengths;  // [groups]
+  uint32_t groups, max_rows, max_prefix;
+};
+
+struct KeyWeightsArgs {
+  PagedAttentionArgs rows;  // without gate and output
+  uint32_t window;          // rows of a sequence that count
+  float decay;
+  float* weights;     // [sequences][kv_heads][row_stride]
+  size_t row_stride;
+  uint32_t stride;    // row_stride, as far as a length goes
+};
+
+struct SelectKeysArgs {
+  const float* weights;  // [sequences][kv_heads][weight_stride]
+  const uint32_t* lengths;
+  const uint32_t* keep;
+  int32_t* kept;  // [sequences][kv_heads][kept_stride]
+  uint32_t* kept_lengths;
+  size_t weight_stride, kept_stride;
+  uint32_t sequences, kv_heads, max_keys, first, last;
+};
+
+struct GatherPagesArgs {
+  PagedQ8Args cache;
+  const int32_t* table;         // [sequences][width]
+  const int32_t* target_table;  // [sequences][target_width]
+  const int32_t* kept;          // [sequences][kv_heads][kept_stride]
+  const uint32_t* kept_lengths;
+  const float* weights;   // [sequences][kv_heads][weight_stride] or null
+  float* weights_output;  // alike
+  size_t kept_stride, weight_stride;
+  uint32_t sequences, width, target_width;
+};
+
+constexpr uint32_t kMaxTopLogprobs = 32;
+
+struct LogprobsArgs {
+  const float* logits;
+  const float* temperature;  // nullable, as the next and the outputs
+  const int32_t* tokens;
+  float* logprobs;
+  int32_t* ranks;
+  float* entropies;
+  int32_t* top_tokens;
+  float* top_logprobs;
+  size_t row_stride;
+  uint32_t rows, size, top;
+};
+
 hipError_t launch_prologue_paged_q8(const PagedPrologueArgs& a, hipStream_t stream);
 hipError_t launch_dequantize_pages_q8(const PagedQ8Args& c, const int32_t* ids, uint32_t count,
                                       void* key_rows, void* value_rows, hipStream_t stream);
 size_t attention_paged_q8_workspace_bytes(const PagedAttentionArgs& a, int cu_count);
 hipError_t launch_attention_paged_q8(const PagedAttentionArgs& a, int cu_count, void* workspace,
                                      hipStream_t stream);
+size_t attention_shared_q8_workspace_bytes(const PagedAttentionArgs& a, const SharedPrefixArgs& p,
+                                           int cu_count);
+hipError_t launch_attention_shared_q8(const PagedAttentionArgs& a, const SharedPrefixArgs& p,
+                                      int cu_count, void* workspace, hipStream_t stream);
+size_t key_weights_workspace_bytes(const KeyWeightsArgs& a, int cu_count);
+hipError_t launch_key_weights(const KeyWeightsArgs& a, int cu_count, void* workspace,
+                              hipStream_t stream);
+hipError_t launch_select_keys(const SelectKeysArgs& a, hipStream_t stream);
+hipError_t launch_gather_pages(const GatherPagesArgs& a, hipStream_t stream);
+size_t token_logprobs_workspace_bytes(const LogprobsArgs& a);
+hipError_t launch_token_logprobs(const LogprobsArgs& a, void* workspace, hipStream_t stream);
 size_t sample_workspace_bytes(const SampleArgs& a);
 hipError_t launch_sample(const SampleArgs& a, void* workspace, hipStream_t stream);
 

@@ -55,10 +55,18 @@ class PagedBatch(ctypes.Structure):
                 ("max_query", ctypes.c_size_t), ("max_keys", ctypes.c_size_t)]
 
 
+class SharedPrefixes(ctypes.Structure):
+    """kraken_shared_prefixes: groups of a batch's sequences that begin alike."""
+    _fields_ = [("group_starts", KrakenBuffer), ("prefix_lengths", KrakenBuffer),
+                ("groups", ctypes.c_size_t), ("max_rows", ctypes.c_size_t),
+                ("max_prefix", ctypes.c_size_t)]
+
+
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
 _pages = ctypes.POINTER(PagedQ8Cache)
 _batch = ctypes.POINTER(PagedBatch)
+_prefixes = ctypes.POINTER(SharedPrefixes)
 _B = KrakenBuffer
 _ctx = ctypes.c_void_p
 
@@ -146,6 +154,13 @@ SIGNATURES = {
     "kraken_hip_attention_f16q_paged_q8_kv": [_B, _pages, _batch, _sz, _B],
     "kraken_hip_dequantize_kv_pages_q8_f16": [_pages, _B, _sz, _B, _B],
     "kraken_hip_sample_f32_i32": [_B, _sz, _sz, _sz] + [_B] * 7,
+    "kraken_hip_attention_f32_shared_paged_q8_kv": [_B, _B, _pages, _batch, _prefixes, _sz, _B],
+    "kraken_hip_attention_f16q_shared_paged_q8_kv": [_B, _pages, _batch, _prefixes, _sz, _B],
+    "kraken_hip_key_weights_f32_paged_q8_kv": [_B, _pages, _batch, _sz, _sz, _f, _B, _sz],
+    "kraken_hip_key_weights_f16q_paged_q8_kv": [_B, _pages, _batch, _sz, _sz, _f, _B, _sz],
+    "kraken_hip_select_keys_f32_i32": [_B, _sz, _B, _B] + [_sz] * 5 + [_B, _sz, _B],
+    "kraken_hip_gather_kv_pages_q8": [_pages, _B, _sz, _B, _B, _sz, _sz, _B, _sz, _B, _sz, _B],
+    "kraken_hip_token_logprobs_f32": [_B, _sz, _sz, _sz, _B, _B, _sz] + [_B] * 5,
     "kraken_hip_begin_graph": [],
     "kraken_hip_commit_graph": [],
     "kraken_hip_make_buffer": [_sz, ctypes.POINTER(_B)],
