@@ -911,8 +911,9 @@ KRAKEN_API int kraken_hip_attention_f16q_shared_paged_q8_kv(
  * stay as they were, as do sequences that bring no tokens, break a bound of the batch or
  * are longer than weight_stride.  A key outside the pool receives nothing.  query is as
  * for the attention, f32 or f16; the weights keep f32 accuracy in both, by the same
- * limits, and their sums have one order whatever else the batch holds.  A NaN or an
- * infinity in a query or a scale reaches all weights of its sequence and KV head.  decay
+ * limits.  Sums go in one order, so that the same call gives the same bits; loose bounds
+ * of the batch change it.  A NaN or an infinity in a query that counts or in the scale of
+ * a key that it sees reaches all weights of its sequence and KV head.  decay
  * is finite and not negative.  query is 16-byte aligned; key_weights overlaps no input.
  * Up to 67108864 rows (tokens * heads).  Uses context workspace. */
 KRAKEN_API int kraken_hip_key_weights_f32_paged_q8_kv(
