@@ -44,9 +44,13 @@ __device__ __forceinline__ u32x4_t load_once(const int8_t* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
 }
 
-template <int D, class T, bool kStacked>
-__global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAttentionArgs a,
-                                                                        PagedSplit split) {
+// Workgroup `block`'s work; false where there is none.  `again`: the workgroup has done other
+// before.
+template <int D, class T, bool kStacked, class Work>
+__device__ __forceinline__ bool attention_paged_decode(const PagedAttentionArgs& a,
+                                                       const PagedSplit& split, const Work& work,
+                                                       uint32_t block, bool again) {
+  constexpr bool kShared = std::is_same<Work, SharedWork>::value;
   constexpr uint32_t kRows = kStacked ? 8 : kDecodeBlock;
   constexpr bool kTwo = !kStacked && std::is_same<T, float>::value;
   constexpr int kLoads = D / 64;  // 16-byte loads of a key row per lane and row tile
@@ -58,10 +62,24 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   const uint32_t n = lane & 15u, g = lane >> 4;
   const uint32_t shift = a.cache.page_shift, kv_heads = a.cache.kv_heads;
   const uint32_t group = a.heads / kv_heads;
-  const uint32_t kv_head = blockIdx.x % kv_heads;
-  uint32_t item = blockIdx.x / kv_heads, sequence = 0;
+  const uint32_t kv_head = block % kv_heads;
+  uint32_t item = block / kv_heads, sequence = 0;
   PagedSequence s;
-  if (a.batch.sequences > 1u) {
+  // Of a shared call's item: its first key, and what it is.
+  uint32_t first = 0, shared_group = kNoGroup;
+  uint32_t part_keys = split.decode_keys;
+  if constexpr (kShared) {
+    const SharedFound found = shared_item(work, 0, item);
+    if (found.item.count == 0) {
+      return false;
+    }
+    s = {found.item.start, found.item.count, found.item.length};
+    sequence = found.item.sequence;
+    first = found.item.first;
+    shared_group = found.item.group;
+    item = found.work;
+    part_keys = work.keys[0];
+  } else if (a.batch.sequences > 1u) {
     // The sequences' parts one after another: no workgroup without keys stands between
     // two with, and the XCDs, which take workgroups in turn, get as many each.
     const PagedItem found = paged_item(a.batch, item, shift, [&](const PagedSequence& q) {
@@ -80,7 +98,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   // max_query, which it may fall short of.)
   const uint32_t blocks = max(1u, (s.count * group + kRows - 1u) / kRows);
   const uint32_t part = item / blocks, first_row = item % blocks * kRows;
-  const uint32_t begin = part * split.decode_keys;
+  const uint32_t begin = first + part * part_keys;
   // The first pages' ids are asked for together with a single sequence's length (in the
   // bounds of the table whatever that is): K and V wait for two loads in a row, not three.
   const int32_t* table = a.batch.table + (size_t)sequence * a.batch.width;
@@ -89,22 +107,26 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   // Of the lane's key rows (run n / 4 of the step's four) and of its own run g.
   int32_t page_k = page_of(first_key(wave) + 8u * (n >> 2));
   int32_t page_v = page_of(first_key(wave) + 8u * g);
-  if (a.batch.sequences == 1u) {
-    s = paged_sequence(a.batch, 0, shift);
-  }
-  if (s.count == 0 || s.count * group > split.decode_rows || first_row >= s.count * group ||
-      begin >= s.length) {
-    return;
+  if constexpr (!kShared) {
+    if (a.batch.sequences == 1u) {
+      s = paged_sequence(a.batch, 0, shift);
+    }
+    if (s.count == 0 || s.count * group > split.decode_rows || first_row >= s.count * group ||
+        begin >= s.length) {
+      return false;
+    }
   }
   const uint32_t rows = min(kRows, s.count * group - first_row);
-  const uint32_t end = min(s.length, begin + split.decode_keys);
+  const uint32_t end = min(s.length, begin + part_keys);
   const uint32_t steps = (end - begin + 31u) / 32u;
 
   // This lane's query row and the keys that it sees.
   const uint32_t row = kStacked ? n & 7u : n;
   const bool real = row < rows;
   const uint32_t token = real ? (first_row + row) / group : 0u;
-  const uint32_t visible = s.length - s.count + token + 1u;
+  // Keys before the row's own position and it; of a group's, all.
+  const uint32_t before = shared_group == kIsGroup ? s.length - 1u : s.length - s.count;
+  const uint32_t visible = shared_group == kIsGroup ? s.length : before + token + 1u;
   const size_t at = ((size_t)(s.start + token) * a.heads + kv_head * group +
                      (real ? (first_row + row) % group : 0u)) * D;
 
@@ -198,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
   }
   float top = kLowestMax, sum = 0.0f;
   // Keys that every row sees need no mask.
-  const uint32_t open = s.length - s.count + first_row / group + 1u;
+  const uint32_t open = shared_group == kIsGroup ? s.length : before + first_row / group + 1u;
 
   for (uint32_t step = wave; step < steps; step += kWaves) {
     const uint32_t next = step + kWaves;
@@ -315,6 +337,9 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
       }
     }
   }
+  if (again) {
+    __syncthreads();  // the results before are read
+  }
   if (n < kRows) {
     if (g == 0) {
       lds_m[wave][n] = top;
@@ -332,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
     }
   }
   __syncthreads();
-  const bool whole = s.length <= split.decode_keys;
+  const bool whole = shared_group == kNoGroup && s.length <= part_keys;
   for (uint32_t e = threadIdx.x; e < rows * D; e += 256u) {
     const uint32_t r = e / D, d = e % D;
     float m = lds_m[0][r];
@@ -347,11 +372,18 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
       l = fmaf(keep, lds_l[w][r], l);
       x = fmaf(keep, lds_o[(w * kRows + r) * kStride + d], x);
     }
+    const size_t out = ((size_t)(s.start + (first_row + r) / group) * a.heads +
+                        kv_head * group + (first_row + r) % group);
     if (whole) {
-      const size_t out =
-        ((size_t)(s.start + (first_row + r) / group) * a.heads + kv_head * group +
-         (first_row + r) % group) * D;
-      store_output<T>(a, out + d, x, inverse_sum(l));
+      store_output<T>(a, out * D + d, x, inverse_sum(l));
+    } else if constexpr (kShared) {
+      const uint32_t kind = shared_group == kIsGroup ? 1u : 0u;
+      const size_t i = (size_t)part * a.batch.tokens * a.heads + out;
+      work.o[kind][i * D + d] = x;
+      if (d == 0) {
+        work.ml[kind][2 * i] = m;
+        work.ml[kind][2 * i + 1] = l;
+      }
     } else {
       const size_t i = (((size_t)part * a.batch.sequences + sequence) * kv_heads + kv_head) *
                          split.decode_rows + first_row + r;
@@ -361,6 +393,22 @@ __global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAtt
         split.decode_ml[2 * i + 1] = l;
       }
     }
+  }
+  return true;
+}
+
+template <int D, class T, bool kStacked, class Work>
+__global__ __launch_bounds__(256, 2) void attention_paged_decode_kernel(PagedAttentionArgs a,
+                                                                        PagedSplit split,
+                                                                        Work work) {
+  if constexpr (std::is_same<Work, SharedWork>::value) {
+    // Those of a shared call go on to further work: the host does not know how much there is.
+    for (uint32_t block = blockIdx.x;
+         attention_paged_decode<D, T, kStacked>(a, split, work, block, block != blockIdx.x);
+         block += gridDim.x) {
+    }
+  } else {
+    attention_paged_decode<D, T, kStacked>(a, split, work, blockIdx.x, false);
   }
 }
 
@@ -570,9 +618,9 @@ void launch_for(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_
     const uint32_t blocks = (split.decode_rows + kDecodeBlock - 1u) / kDecodeBlock;
     const dim3 grid(split.decode_splits * blocks * a.cache.kv_heads * a.batch.sequences);
     if (rows <= 8u) {
-      attention_paged_decode_kernel<D, T, true><<<grid, 256, 0, stream>>>(a, split);
+      attention_paged_decode_kernel<D, T, true><<<grid, 256, 0, stream>>>(a, split, PlainWork{});
     } else {
-      attention_paged_decode_kernel<D, T, false><<<grid, 256, 0, stream>>>(a, split);
+      attention_paged_decode_kernel<D, T, false><<<grid, 256, 0, stream>>>(a, split, PlainWork{});
     }
   }
   if (rows > kDecodeRows) {
@@ -610,6 +658,43 @@ void launch_type(const PagedAttentionArgs& a, const PagedSplit& split, hipStream
 }
 
 }  // namespace
+
+namespace {
+
+template <int D, class T>
+void launch_shared_decode_for(const PagedAttentionArgs& a, const SharedWork& work,
+                              uint32_t decode_rows, uint32_t workgroups, hipStream_t stream) {
+  if (decode_rows == 8u) {
+    attention_paged_decode_kernel<D, T, true>
+      <<<dim3(workgroups), 256, 0, stream>>>(a, PagedSplit{}, work);
+  } else {
+    attention_paged_decode_kernel<D, T, false>
+      <<<dim3(workgroups), 256, 0, stream>>>(a, PagedSplit{}, work);
+  }
+}
+
+template <class T>
+void launch_shared_decode_type(const PagedAttentionArgs& a, const SharedWork& work,
+                               uint32_t decode_rows, uint32_t workgroups, hipStream_t stream) {
+  if (a.cache.head_dim == 256u) {
+    launch_shared_decode_for<256, T>(a, work, decode_rows, workgroups, stream);
+  } else if (a.cache.head_dim == 128u) {
+    launch_shared_decode_for<128, T>(a, work, decode_rows, workgroups, stream);
+  } else {
+    launch_shared_decode_for<64, T>(a, work, decode_rows, workgroups, stream);
+  }
+}
+
+}  // namespace
+
+void launch_shared_decode(const PagedAttentionArgs& a, const SharedWork& work,
+                          uint32_t decode_rows, uint32_t workgroups, hipStream_t stream) {
+  if (a.f16) {
+    launch_shared_decode_type<half_t>(a, work, decode_rows, workgroups, stream);
+  } else {
+    launch_shared_decode_type<float>(a, work, decode_rows, workgroups, stream);
+  }
+}
 
 size_t attention_paged_q8_workspace_bytes(const PagedAttentionArgs& a, int cu_count) {
   const PagedSplit s = split_of(a, cu_count);

@@ -68,6 +68,58 @@ struct PagedSplit {
   uint32_t* tile_chosen;  // the keys that it chose, for the join
 };
 
+// What a workgroup takes beside a plain call: nothing.
+struct PlainWork {};
+
+// In a call whose sequences share prefixes the kernels take items, which a launch before
+// lists: the shared keys of a group for all its rows, and what is left of each sequence.
+struct alignas(8) SharedItem {
+  uint32_t start, count;  // rows: tokens of the batch
+  uint32_t length;        // keys [first, length)
+  uint32_t sequence;      // whose page table
+  uint32_t first;
+  uint32_t group;         // of a sequence: the group whose keys before `first` its rows see
+                          // too, kNoGroup if first is 0; of a group's item kIsGroup
+};
+constexpr uint32_t kNoGroup = 0xffffffffu, kIsGroup = 0xfffffffeu;
+
+struct SharedWork {
+  const SharedItem* items;      // of groups, then of sequences
+  const uint32_t* ends;         // [2][count]: workgroups (by KV head) of the items up to each,
+                                // of the decode kernel and of the tiled one
+  const uint32_t* keys;         // [2]: keys of a workgroup
+  uint32_t count;
+  float* o[2];                  // [part][token][head][D] of sequences, of groups
+  float* ml[2];                 // [part][token][head][2]
+};
+
+struct SharedFound {
+  SharedItem item;  // count 0: none
+  uint32_t work;    // the workgroup's number in the item
+};
+
+// The item of workgroup `want` (by KV head) of the decode kernel (kind 0) or the tiled one,
+// looked for by a wave.
+__device__ __forceinline__ SharedFound shared_item(const SharedWork& w, uint32_t kind,
+                                                   uint32_t want) {
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t* ends = w.ends + (size_t)kind * w.count;
+  uint32_t before = 0;
+  for (uint32_t at = 0; at < w.count; at += 64) {
+    const uint32_t end = ends[min(at + lane, w.count - 1u)];
+    const uint64_t past = __ballot(end > want);
+    if (past != 0) {
+      const uint32_t from = (uint32_t)__builtin_ctzll(past);
+      if (from != 0) {
+        before = (uint32_t)__builtin_amdgcn_readlane((int)end, (int)from - 1);
+      }
+      return {w.items[at + from], want - before};
+    }
+    before = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+  }
+  return {SharedItem{}, 0u};
+}
+
 // Four codes (one dword, two's complement) as f16.  0x64uu is 1024 + uu in f16, so a
 // code offset to uu = code + 128 needs one byte permute for two values and one packed
 // subtraction of 1152.
@@ -179,5 +231,12 @@ __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f 
 
 void launch_attention_paged_q8_tiles(const PagedAttentionArgs& a, const PagedSplit& split,
                                      hipStream_t stream);
+
+// The two kernels over a shared call's items.  decode_rows: of a block of the decode kernel,
+// 8 or 16.
+void launch_shared_decode(const PagedAttentionArgs& a, const SharedWork& work,
+                          uint32_t decode_rows, uint32_t workgroups, hipStream_t stream);
+void launch_shared_tiles(const PagedAttentionArgs& a, const SharedWork& work,
+                         uint32_t workgroups, hipStream_t stream);
 
 }  // namespace kraken

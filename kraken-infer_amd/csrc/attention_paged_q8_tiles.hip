@@ -72,13 +72,16 @@ __device__ __forceinline__ uint32_t chosen_keys(const PagedAttentionArgs& a,
   return (uint32_t)__builtin_amdgcn_readfirstlane((int)best);
 }
 
-// One part of `part_keys` keys of one tile of rows.  `again`: the workgroup has done
-// another before.
-template <int D, class T, int kSub>
+// One part of `part_keys` keys of one tile of rows, of a shared call's item from its key
+// `first` on (of a `shared_group` as there).  `again`: the workgroup has done another
+// before.
+template <int D, class T, int kSub, class Work>
 __device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a,
-                                                     const PagedSplit& split,
-                                                     const PagedItem& found, uint32_t kv_head,
+                                                     const PagedSplit& split, const Work& work,
+                                                     const PagedItem& found, uint32_t first,
+                                                     uint32_t shared_group, uint32_t kv_head,
                                                      uint32_t part_keys, bool again) {
+  constexpr bool kShared = std::is_same<Work, SharedWork>::value;
   constexpr bool kTwo = std::is_same<T, float>::value;
   constexpr int kKeys = 32 * kSub;
   constexpr int kStride = D + 8;                      // of a key row in LDS, in halves
@@ -97,15 +100,17 @@ __device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a
   const uint32_t group = a.heads / kv_heads;
   const PagedSequence s = found.sequence;
   const uint32_t sequence = found.index;
-  const uint32_t parts = (s.length + part_keys - 1u) / part_keys;
+  const uint32_t parts = (s.length - first + part_keys - 1u) / part_keys;
   const uint32_t tile = found.item / parts, part = found.item % parts;
   const uint32_t rows = s.count * group;
   const uint32_t first_row = tile * kTileRows;
   // The keys that the tile's last row sees, of this part.
   const uint32_t before = s.length - s.count;
   const uint32_t last_row = min(first_row + kTileRows, rows) - 1u;
-  const uint32_t begin = part * part_keys;
-  const uint32_t end = min(before + last_row / group + 1u, begin + part_keys);
+  const uint32_t begin = first + part * part_keys;
+  const bool of_group = shared_group == kIsGroup;  // whose rows see all its keys
+  const uint32_t end = min(of_group ? s.length : before + last_row / group + 1u,
+                           begin + part_keys);
   if (begin >= end) {
     return;
   }
@@ -116,11 +121,12 @@ __device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a
   const uint32_t row = wave_row + n;
   const bool real = row < rows;
   const uint32_t token = real ? row / group : 0u;
-  const uint32_t visible = real ? before + token + 1u : 0u;
+  const uint32_t visible = real ? of_group ? s.length : before + token + 1u : 0u;
   const size_t at = ((size_t)(s.start + token) * a.heads + kv_head * group +
                      (real ? row % group : 0u)) * D;
   // What every row of the wave sees (0: a row without a query sees nothing).
-  const uint32_t open = wave_row + 32u <= rows ? before + wave_row / group + 1u : 0u;
+  const uint32_t open =
+    wave_row + 32u <= rows ? of_group ? s.length : before + wave_row / group + 1u : 0u;
 
   // Lane l holds the page of granule l % kGranules of a tile; past the last tile, the
   // last one's again.
@@ -499,9 +505,14 @@ __device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a
   }
   sum = xor32_sum(sum);
   // The key count of the sequence decides for all of its rows, as in the join.
-  const bool whole = s.length <= part_keys;
+  const bool whole = shared_group == kNoGroup && s.length <= part_keys;
   const float inverse = inverse_sum(sum);
   const size_t item = (size_t)part * a.batch.tokens * a.heads + at / D;
+  float *tile_o = split.tile_o, *tile_ml = split.tile_ml;
+  if constexpr (kShared) {
+    tile_o = work.o[of_group ? 1 : 0];
+    tile_ml = work.ml[of_group ? 1 : 0];
+  }
   // Registers 4 j .. + 3 of product i are dimensions 32 i + 8 j + 4 h .. + 3.
   if (whole) {
     float factor[D / 8][4];
@@ -520,12 +531,12 @@ __device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a
     for (int i = 0; i < D / 8; ++i) {
       const float4_t x = {o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1],
                           o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
-      *reinterpret_cast<float4_t*>(split.tile_o + item * D + 8 * i + 4 * h) = x;
+      *reinterpret_cast<float4_t*>(tile_o + item * D + 8 * i + 4 * h) = x;
     }
   }
   if (!whole && h == 0) {
-    split.tile_ml[2 * item] = top;
-    split.tile_ml[2 * item + 1] = sum;
+    tile_ml[2 * item] = top;
+    tile_ml[2 * item + 1] = sum;
   }
 }
 
@@ -533,10 +544,23 @@ __device__ __forceinline__ void attention_paged_tile(const PagedAttentionArgs& a
 // (tile, part) pairs, which stand one after another, so that no place without work stands
 // between two with; the parts of a tile side by side, so that an XCD, which gets every
 // eighth workgroup, reads few parts of a sequence's keys.
-template <int D, class T, int kSub, int kWavesPerSimd>
+template <int D, class T, int kSub, int kWavesPerSimd, class Work>
 __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_kernel(
-  PagedAttentionArgs a, PagedSplit split) {
+  PagedAttentionArgs a, PagedSplit split, Work work) {
   const uint32_t kv_heads = a.cache.kv_heads, group = a.heads / kv_heads;
+  if constexpr (std::is_same<Work, SharedWork>::value) {
+    const uint32_t part_keys = work.keys[1];
+    for (uint32_t block = blockIdx.x;; block += gridDim.x) {
+      const SharedFound found = shared_item(work, 1, block / kv_heads);
+      const SharedItem& i = found.item;
+      if (i.count == 0) {
+        return;
+      }
+      attention_paged_tile<D, T, kSub>(
+        a, split, work, PagedItem{{i.start, i.count, i.length}, i.sequence, found.work}, i.first,
+        i.group, block % kv_heads, part_keys, block != blockIdx.x);
+    }
+  }
   uint32_t part_keys = split.tile_keys;
   if (split.tile_step != 0u) {
     part_keys = chosen_keys(a, split, group);
@@ -555,35 +579,41 @@ __global__ __launch_bounds__(kThreads, kWavesPerSimd) void attention_paged_tile_
     if (found.sequence.count == 0) {
       return;
     }
-    attention_paged_tile<D, T, kSub>(a, split, found, block % kv_heads, part_keys,
-                                     block != blockIdx.x);
+    attention_paged_tile<D, T, kSub>(a, split, work, found, 0, kNoGroup, block % kv_heads,
+                                     part_keys, block != blockIdx.x);
   }
 }
 
-template <int D, class T>
-void launch_tiles(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
+template <int D, class T, class Work>
+void launch_tiles(const PagedAttentionArgs& a, const PagedSplit& split, const Work& work,
+                  uint32_t blocks, hipStream_t stream) {
   // One wave a SIMD for head_dim 256, whose operands take its 512 registers.  64 keys a
   // tile; 32 where two f32 parts of 256 dimensions, or two waves of 128, leave no
   // registers for more (a spilled one waits for every load under way: 17 sequences,
   // head_dim 128: 119 us with 64 keys, 104 with 32).
   constexpr int kWavesPerSimd = D == 256 ? 1 : 2;
   constexpr int kSub = D == 64 || (D == 256 && !std::is_same<T, float>::value) ? 2 : 1;
-  // Two rounds of workgroups, which go on to further parts: of one for each part that a
-  // batch could have most find none (17 sequences, 4096 workgroups for 512 parts: 77 us,
-  // with 1024 61).  The loop costs 1 % where there is one part for each.
-  const uint32_t blocks = std::min(split.tile_blocks, 2u * split.tile_slots);
   attention_paged_tile_kernel<D, T, kSub, kWavesPerSimd>
-    <<<dim3(blocks), kThreads, 0, stream>>>(a, split);
+    <<<dim3(blocks), kThreads, 0, stream>>>(a, split, work);
 }
 
-template <class T>
-void launch_type(const PagedAttentionArgs& a, const PagedSplit& split, hipStream_t stream) {
-  if (a.cache.head_dim == 256u) {
-    launch_tiles<256, T>(a, split, stream);
-  } else if (a.cache.head_dim == 128u) {
-    launch_tiles<128, T>(a, split, stream);
+template <class Work>
+void launch_types(const PagedAttentionArgs& a, const PagedSplit& split, const Work& work,
+                  uint32_t blocks, hipStream_t stream) {
+  const auto sized = [&](auto of_type) {
+    using T = decltype(of_type);
+    if (a.cache.head_dim == 256u) {
+      launch_tiles<256, T>(a, split, work, blocks, stream);
+    } else if (a.cache.head_dim == 128u) {
+      launch_tiles<128, T>(a, split, work, blocks, stream);
+    } else {
+      launch_tiles<64, T>(a, split, work, blocks, stream);
+    }
+  };
+  if (a.f16) {
+    sized(half_t{});
   } else {
-    launch_tiles<64, T>(a, split, stream);
+    sized(float{});
   }
 }
 
@@ -591,11 +621,15 @@ void launch_type(const PagedAttentionArgs& a, const PagedSplit& split, hipStream
 
 void launch_attention_paged_q8_tiles(const PagedAttentionArgs& a, const PagedSplit& split,
                                      hipStream_t stream) {
-  if (a.f16) {
-    launch_type<half_t>(a, split, stream);
-  } else {
-    launch_type<float>(a, split, stream);
-  }
+  // Two rounds of workgroups, which go on to further parts: of one for each part that a
+  // batch could have most find none (17 sequences, 4096 workgroups for 512 parts: 77 us,
+  // with 1024 61).  The loop costs 1 % where there is one part for each.
+  launch_types(a, split, PlainWork{}, std::min(split.tile_blocks, 2u * split.tile_slots), stream);
+}
+
+void launch_shared_tiles(const PagedAttentionArgs& a, const SharedWork& work,
+                         uint32_t workgroups, hipStream_t stream) {
+  launch_types(a, PagedSplit{}, work, workgroups, stream);
 }
 
 }  // namespace kraken

@@ -199,9 +199,9 @@ int shared_attention_entry(kraken_hip_context* ctx, const kraken_buffer& query,
   p.starts = static_cast<const uint32_t*>(prefixes->group_starts.data);
   p.lengths = static_cast<const uint32_t*>(prefixes->prefix_lengths.data);
   p.groups = (uint32_t)prefixes->groups;
-  // No group can have more than either.
+  // No group can have more rows than the batch.
   p.max_rows = (uint32_t)std::min(prefixes->max_rows, batch->tokens);
-  p.max_prefix = (uint32_t)std::min(prefixes->max_prefix, batch->max_keys);
+  p.max_prefix = (uint32_t)std::min(prefixes->max_prefix, size_t{0xffffffffu});
   KRAKEN_TRY(begin_launch(ctx));
   KRAKEN_TRY(ensure_workspace(ctx, attention_shared_q8_workspace_bytes(a, p, ctx->cu_count)));
   return finish(
