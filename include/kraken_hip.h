@@ -887,7 +887,8 @@ typedef struct kraken_shared_prefixes {
 
 /* kraken_hip_attention_f32_paged_q8_kv and kraken_hip_attention_f16q_paged_q8_kv of a
  * batch whose sequences share prefixes: the same outputs to rounding, with each shared
- * page read for all rows of its group at once instead of once for each sequence.  Up to
+ * page read for all rows of its group at once instead of once for each sequence (or by
+ * the plain call, where the bounds say that it is sooner done).  Up to
  * 1048576 rows (tokens * heads); what the plain entries require holds here too.  Uses
  * context workspace (at most about 512 MiB beside the rows' own partial results,
  * 8 * head_dim + 64 bytes for each). */

@@ -20,15 +20,17 @@
 namespace kraken {
 namespace {
 
-constexpr uint32_t kPlanThreads = 1024;
+constexpr uint32_t kPlanThreads = 256;
 constexpr uint32_t kPlanWaves = kPlanThreads / 64u;
 constexpr uint32_t kHeldItems = 1024;  // listed in LDS on the way to memory
+constexpr uint32_t kChoices = 16;      // sizes of the tiled kernel's parts that are tried
 
 // What the host gives the plan.
 struct SharedLimits {
   uint32_t group;         // query heads of a KV head
   uint32_t decode_most;   // rows up to which an item goes to the decode kernel
-  uint32_t decode_rows;   // of a block of it
+  uint32_t decode_shift;  // log2 of the rows of a block of it
+  uint32_t decode_many;   // workgroups beyond which they take more keys
   uint32_t decode_slots;  // workgroups that its work is cut into
   uint32_t tile_slots;    // workgroups of the tiled kernel that run at once
   uint32_t planes[2];     // parts that there is room for, of sequences and of groups
@@ -40,19 +42,18 @@ struct SharedLists {
   uint32_t* keys;
 };
 
-__device__ __forceinline__ uint32_t rows_of(const SharedLimits& l, const SharedItem& i) {
-  return i.count * l.group;
-}
+// Rows' blocks of an item in the kernel that takes it (0: the decode kernel, 1: the tiled
+// one); 0 blocks without rows.
+struct ItemWork {
+  uint32_t kind, blocks;
+};
 
-// Workgroups (by KV head) of an item in `keys` keys each, of the kernel `kind`.
-__device__ __forceinline__ uint32_t work_of(const SharedLimits& l, const SharedItem& i,
-                                            uint32_t kind, uint32_t keys) {
-  const uint32_t rows = rows_of(l, i);
-  if (rows == 0 || (rows <= l.decode_most) != (kind == 0)) {
-    return 0u;
-  }
-  const uint32_t across = kind == 0 ? l.decode_rows : kTileRows;
-  return (rows + across - 1u) / across * ((i.length - i.first + keys - 1u) / keys);
+__device__ __forceinline__ ItemWork work_of(const SharedLimits& l, const SharedItem& i) {
+  const uint32_t rows = i.count * l.group;
+  const bool few = rows <= l.decode_most;
+  const uint32_t shift = few ? l.decode_shift : 7u;
+  static_assert(kTileRows == 1u << 7, "");
+  return {few ? 0u : 1u, (rows + (1u << shift) - 1u) >> shift};
 }
 
 // One workgroup.
@@ -61,19 +62,34 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(PagedAttentio
                                                                    SharedLimits l,
                                                                    SharedLists lists) {
   __shared__ SharedItem held[kHeldItems];
-  __shared__ uint64_t sums[kPlanWaves][2];
-  __shared__ uint32_t most[kPlanWaves][4], scans[kPlanWaves], choice[kPlanWaves];
-  __shared__ float times[kPlanWaves];
+  __shared__ uint32_t held_starts[kHeldItems + 1u];
+  __shared__ float sums[kPlanWaves][2], times[kChoices];
+  __shared__ uint32_t most[kPlanWaves][4], scans[kPlanWaves][2];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t sequences = a.batch.sequences, shift = a.cache.page_shift;
-  const uint32_t kv_heads = a.cache.kv_heads, count = p.groups + sequences;
-  SharedItem* const items = count <= kHeldItems ? held : lists.items;
+  const uint32_t count = p.groups + sequences;
+  const bool small = count <= kHeldItems;
+  SharedItem* const items = small ? held : lists.items;
+  const uint32_t* const starts = small ? held_starts : a.batch.starts;
 
+  // The arrays' loads go out together: of a wave's first group too.
+  uint32_t group_begin = 0, group_end = 0, group_prefix = 0;
+  if (wave < p.groups) {
+    group_begin = p.starts[wave];
+    group_end = p.starts[wave + 1u];
+    group_prefix = p.lengths[wave];
+  }
   for (uint32_t i = tid; i < count; i += kPlanThreads) {
     SharedItem item{0u, 0u, 0u, 0u, 0u, kIsGroup};
     if (i >= p.groups) {
       const PagedSequence q = paged_sequence(a.batch, i - p.groups, shift);
       item = {q.start, q.count, q.length, i - p.groups, 0u, kNoGroup};
+      if (small) {
+        held_starts[i - p.groups] = q.start;
+        if (i + 1u == count) {
+          held_starts[sequences] = a.batch.starts[sequences];
+        }
+      }
     }
     items[i] = item;
   }
@@ -81,17 +97,22 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(PagedAttentio
 
   // A wave a group.
   for (uint32_t g = wave; g < p.groups; g += kPlanWaves) {
-    const uint32_t begin = p.starts[g], end = p.starts[g + 1], prefix = p.lengths[g];
-    if (begin >= end || end > sequences || prefix > p.max_prefix) {
+    if (g != wave) {
+      group_begin = p.starts[g];
+      group_end = p.starts[g + 1u];
+      group_prefix = p.lengths[g];
+    }
+    const uint32_t begin = group_begin, end = group_end;
+    if (begin >= end || end > sequences || group_prefix > p.max_prefix) {
       continue;
     }
-    const uint32_t row = a.batch.starts[begin], stop = a.batch.starts[end];
+    const uint32_t row = starts[begin], stop = starts[end];
     if (row >= stop || stop > a.batch.tokens || stop - row > p.max_rows) {
       continue;
     }
     // Its sequences with rows: how many, the first, and the fewest tokens before the new
     // ones; whether all their rows lie in the group's.
-    uint32_t least = prefix, first = end, live = 0;
+    uint32_t least = group_prefix, first = end, live = 0;
     bool fits = true;
     for (uint32_t i = begin + lane; i < end; i += 64u) {
       const SharedItem q = items[p.groups + i];
@@ -102,11 +123,10 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(PagedAttentio
         fits = fits && q.start >= row && q.start + q.count <= stop;
       }
     }
-    for (int step = 1; step < 64; step *= 2) {
-      least = min(least, (uint32_t)__shfl_xor((int)least, step));
-      first = min(first, (uint32_t)__shfl_xor((int)first, step));
-      live += (uint32_t)__shfl_xor((int)live, step);
-    }
+    // (The smallest of x is what the largest of ~x leaves.)
+    least = ~(uint32_t)__builtin_amdgcn_readlane((int)wave_scan(~least, Largest{}), 63);
+    first = ~(uint32_t)__builtin_amdgcn_readlane((int)wave_scan(~first, Largest{}), 63);
+    live = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(live, Sum{}), 63);
     const uint32_t shared = least >> shift << shift;
     // (A single sequence would gain nothing.)
     if (!__all(fits) || live < 2u || shared == 0) {
@@ -128,28 +148,26 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(PagedAttentio
   __syncthreads();
 
   // Rows' blocks times keys for each kernel, and the longest of each kind of item in it.
-  uint64_t all[2] = {0, 0};
+  float all[2] = {0.0f, 0.0f};
   uint32_t longest[4] = {0, 0, 0, 0};
   for (uint32_t i = tid; i < count; i += kPlanThreads) {
     const SharedItem q = items[i];
-    const uint32_t rows = rows_of(l, q), keys = q.length - q.first;
-    const uint32_t kind = rows <= l.decode_most ? 0u : 1u;
-    const uint32_t across = kind == 0 ? l.decode_rows : kTileRows;
-    const uint32_t at = 2u * kind + (i < p.groups ? 1u : 0u);
+    const ItemWork w = work_of(l, q);
+    const uint32_t keys = w.blocks != 0 ? q.length - q.first : 0u;
+    const uint32_t at = 2u * w.kind + (i < p.groups ? 1u : 0u);
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
-      longest[k] = at == k && rows != 0 ? max(longest[k], keys) : longest[k];
+      longest[k] = at == k ? max(longest[k], keys) : longest[k];
     }
-    const uint64_t work = (uint64_t)((rows + across - 1u) / across) * keys;
-    all[0] += kind == 0 ? work : 0u;
-    all[1] += kind == 1 ? work : 0u;
+    all[0] += w.kind == 0 ? (float)w.blocks * (float)keys : 0.0f;
+    all[1] += w.kind == 1 ? (float)w.blocks * (float)keys : 0.0f;
   }
 #pragma unroll
   for (uint32_t k = 0; k < 4; ++k) {
     longest[k] = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(longest[k], Largest{}), 63);
   }
-  all[0] = last_lane(wave_scan(all[0], Sum{}));
-  all[1] = last_lane(wave_scan(all[1], Sum{}));
+  all[0] = wave_sum(all[0]);
+  all[1] = wave_sum(all[1]);
   if (lane == 0) {
     sums[wave][0] = all[0];
     sums[wave][1] = all[1];
@@ -159,74 +177,105 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(PagedAttentio
     }
   }
   __syncthreads();
-  all[0] = all[1] = 0;
-  uint32_t need[2] = {0, 0};  // keys of a part, so that the parts have room
+  all[0] = all[1] = 0.0f;
+#pragma unroll
   for (uint32_t w = 0; w < kPlanWaves; ++w) {
 #pragma unroll
     for (uint32_t k = 0; k < 2; ++k) {
-      all[k] += sums[w][k];
-      need[k] = max(need[k], (most[w][2 * k] + l.planes[0] - 1u) / l.planes[0]);
-      need[k] = max(need[k], (most[w][2 * k + 1] + l.planes[1] - 1u) / l.planes[1]);
+      all[k] += sums[w][k] * (float)a.cache.kv_heads;
+      longest[2 * k] = max(longest[2 * k], most[w][2 * k]);
+      longest[2 * k + 1] = max(longest[2 * k + 1], most[w][2 * k + 1]);
     }
   }
-  // The decode kernel's: as many workgroups as its slots, of 128 to 4096 keys.
-  uint64_t keys = (all[0] * kv_heads + l.decode_slots - 1u) / l.decode_slots;
-  keys = min(max(keys, (uint64_t)128u), (uint64_t)4096u);
-  const uint32_t decode_keys = (uint32_t)((max(keys, (uint64_t)need[0]) + 127u) / 128u * 128u);
+  // Keys of a part, so that an item's parts have room.
+  uint32_t need[2];
+#pragma unroll
+  for (uint32_t k = 0; k < 2; ++k) {
+    need[k] = max((longest[2 * k] + l.planes[0] - 1u) / l.planes[0],
+                  (longest[2 * k + 1] + l.planes[1] - 1u) / l.planes[1]);
+  }
+  // The decode kernel's: as many workgroups as its slots, of 128 to 4096 keys; 256 at least
+  // where they are more than 4 a CU all the same, as a workgroup's way to its first keys is
+  // long (64 sequences of up to 4096 own keys: the call 110 us with 128, 100 with 256, 104
+  // with 512; four of up to 256: 20.9 and 22.0).
+  const float least = all[0] > 128.0f * (float)l.decode_many ? 256.0f : 128.0f;
+  const float wanted = fminf(fmaxf(all[0] / (float)l.decode_slots, least), 4096.0f);
+  const uint32_t decode_keys = (max((uint32_t)wanted, need[0]) + 127u) / 128u * 128u;
   // The tiled kernel's: of sixteen sizes the one whose rounds of `tile_slots` workgroups are
   // soonest over, each round taking its keys and what a workgroup spends besides (about 128
-  // keys' time).  Each wave tries one: those that make one round, two .. eight if all parts
-  // were full, and an eighth more.
-  {
-    const uint64_t rounds = (uint64_t)l.tile_slots * (1u + wave / 2u);
-    keys = (all[1] * kv_heads + rounds - 1u) / rounds;
-    keys += wave % 2u != 0u ? keys / 8u : 0u;
-    keys = max(min(max(keys, (uint64_t)128u), (uint64_t)0x3fffffc0u), (uint64_t)need[1]);
-    const uint32_t mine = (uint32_t)((keys + 63u) / 64u * 64u);
-    float total = 0.0f;
-    for (uint32_t i = lane; i < count; i += 64u) {
-      total += (float)work_of(l, items[i], 1u, mine);
-    }
-    total = wave_sum(total) * (float)kv_heads;
-    if (lane == 0) {
-      choice[wave] = mine;
-      times[wave] = ceilf(total / (float)l.tile_slots) * ((float)mine + 128.0f);
-    }
-  }
-  __syncthreads();
+  // keys' time).  Tried are those that make one round, two .. eight if all parts were full,
+  // and an eighth more.
+  auto tile_keys = [&](uint32_t choice) {
+    const float rounds = (float)(1u + choice / 2u) * (float)l.tile_slots;
+    const float keys = all[1] / rounds * (choice % 2u != 0u ? 1.125f : 1.0f);
+    return (max((uint32_t)fminf(fmaxf(keys, 128.0f), 1e9f), need[1]) + 63u) / 64u * 64u;
+  };
   uint32_t best = 0;
-  for (uint32_t w = 1; w < kPlanWaves; ++w) {
-    best = times[w] < times[best] ? w : best;
+  if (all[1] > 0.0f) {
+    for (uint32_t c = wave; c < kChoices; c += kPlanWaves) {
+      const float keys = (float)tile_keys(c);
+      float total = 0.0f;
+      for (uint32_t i = lane; i < count; i += 64u) {
+        const SharedItem q = items[i];
+        const ItemWork w = work_of(l, q);
+        total += w.kind == 1 ? (float)w.blocks * ceilf((float)(q.length - q.first) / keys) : 0.0f;
+      }
+      total = wave_sum(total) * (float)a.cache.kv_heads;
+      if (lane == 0) {
+        times[c] = ceilf(total / (float)l.tile_slots) * (keys + 128.0f);
+      }
+    }
+    __syncthreads();
+    float least = times[0];
+#pragma unroll
+    for (uint32_t c = 1; c < kChoices; ++c) {
+      best = times[c] < least ? c : best;
+      least = fminf(times[c], least);
+    }
   }
-  const uint32_t part_keys[2] = {decode_keys, choice[best]};
-  if (tid < 2u) {
-    lists.keys[tid] = part_keys[tid];
+  const uint32_t part_keys[2] = {decode_keys, tile_keys(best)};
+  if (tid == 0) {
+    lists.keys[0] = part_keys[0];
+    lists.keys[1] = part_keys[1];
   }
   // The workgroups up to each item.
-#pragma unroll
-  for (uint32_t kind = 0; kind < 2; ++kind) {
-    uint32_t before = 0;
-    for (uint32_t base = 0; base < count; base += kPlanThreads) {
-      const uint32_t i = base + tid;
-      const uint32_t mine = i < count ? work_of(l, items[i], kind, part_keys[kind]) : 0u;
-      uint32_t upto = wave_scan(mine, Sum{});
-      __syncthreads();
-      if (lane == 63u) {
-        scans[wave] = upto;
-      }
-      __syncthreads();
-      upto += before;
-      for (uint32_t w = 0; w < kPlanWaves; ++w) {
-        upto += w < wave ? scans[w] : 0u;
-        before += scans[w];
-      }
-      if (i < count) {
-        lists.ends[(size_t)kind * count + i] = upto;
+  uint32_t before[2] = {0, 0};
+  for (uint32_t base = 0; base < count; base += kPlanThreads) {
+    const uint32_t i = base + tid;
+    uint32_t upto[2] = {0, 0};
+    if (i < count) {
+      const SharedItem q = items[i];
+      const ItemWork w = work_of(l, q);
+      const uint32_t keys = part_keys[w.kind];
+      const uint32_t mine = w.blocks * ((q.length - q.first + keys - 1u) / keys);
+      upto[0] = w.kind == 0 ? mine : 0u;
+      upto[1] = w.kind == 1 ? mine : 0u;
+      if (small) {
+        lists.items[i] = q;
       }
     }
-  }
-  if (items == held && tid < count) {
-    lists.items[tid] = held[tid];
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k) {
+      upto[k] = wave_scan(upto[k], Sum{});
+    }
+    __syncthreads();
+    if (lane == 63u) {
+      scans[wave][0] = upto[0];
+      scans[wave][1] = upto[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k) {
+      upto[k] += before[k];
+#pragma unroll
+      for (uint32_t w = 0; w < kPlanWaves; ++w) {
+        upto[k] += w < wave ? scans[w][k] : 0u;
+        before[k] += scans[w][k];
+      }
+      if (i < count) {
+        lists.ends[(size_t)k * count + i] = upto[k];
+      }
+    }
   }
 }
 
@@ -335,6 +384,22 @@ struct SharedPlan {
   size_t bytes;
 };
 
+// Whether reading shared keys once can make up for the launches that it takes: the bytes
+// that the plain call would read again, in every block of 16 rows of the decode kernel, as
+// far as the host's bounds say.  Measured even, plain and shared: without the tiled kernel 26
+// MB (4 sequences of 4 rows, 8192 tokens of 1 KiB: 21.4 us and 21.6; 32768: 42.6 and 26.8), with
+// it about 100 MB (64 sequences, 2048 tokens: 48.8 and 45.6, 512 tokens 21 and 41; 8 of 32
+// rows, 2048 tokens: 29 and 48, 8192: 73 and 58).
+bool worth_sharing(const PagedAttentionArgs& a, const SharedPrefixArgs& p) {
+  const uint64_t group = a.heads / a.cache.kv_heads;
+  const uint64_t own = a.batch.max_query * group, all = std::max(own, p.max_rows * group);
+  const uint64_t blocks = own <= kDecodeBlock || own > kDecodeRows ? 1u : 2u;
+  const double again = (double)(a.batch.sequences - p.groups) *
+                       (double)std::min(p.max_prefix, a.batch.max_keys) *
+                       (double)(2u * (uint64_t)a.cache.kv_heads * a.cache.head_dim * blocks);
+  return again > (all > kDecodeRows ? 100e6 : 26e6);
+}
+
 SharedPlan plan_of(const PagedAttentionArgs& a, const SharedPrefixArgs& p, int cu_count,
                    void* workspace) {
   SharedPlan s{};
@@ -345,10 +410,11 @@ SharedPlan plan_of(const PagedAttentionArgs& a, const SharedPrefixArgs& p, int c
   const uint64_t all = std::max<uint64_t>(own, (uint64_t)p.max_rows * l.group);
   // Blocks of eight rows where all items, or those of single sequences, have no more; else of
   // sixteen, of which two are still faster than a tile of 128.
-  l.decode_rows = all <= 8u || (own <= 8u && all > kDecodeRows) ? 8u : 16u;
-  l.decode_most = l.decode_rows == 8u ? 8u
-                  : all <= kDecodeRows || own <= kDecodeRows ? kDecodeRows : kDecodeBlock;
+  const bool eight = all <= 8u || (own <= 8u && all > kDecodeRows);
+  l.decode_shift = eight ? 3u : 4u;
+  l.decode_most = eight ? 8u : own <= kDecodeRows ? kDecodeRows : kDecodeBlock;
   l.decode_slots = 11u * (uint32_t)cu_count;
+  l.decode_many = 4u * (uint32_t)cu_count;
   l.tile_slots = (a.cache.head_dim == 256u ? 1u : 2u) * (uint32_t)cu_count;
   const uint64_t rows = (uint64_t)a.batch.tokens * a.heads;
   const uint64_t row_bytes = rows * (a.cache.head_dim + 2u) * sizeof(float);
@@ -359,7 +425,7 @@ SharedPlan plan_of(const PagedAttentionArgs& a, const SharedPrefixArgs& p, int c
   const uint64_t items = (uint64_t)a.batch.sequences + p.groups;
   const uint64_t pairs = items * a.cache.kv_heads;
   s.decode_workgroups = (uint32_t)std::min<uint64_t>(
-    pairs * (l.decode_most / l.decode_rows) * ((a.batch.max_keys + 127u) / 128u),
+    pairs * (l.decode_most >> l.decode_shift) * ((a.batch.max_keys + 127u) / 128u),
     l.decode_slots + std::min<uint64_t>(pairs, l.decode_slots));
   s.tile_workgroups = all > l.decode_most ? 2u * l.tile_slots : 0u;
   size_t at = 0;
@@ -388,7 +454,9 @@ template <int D, class T>
 void launch_join(const PagedAttentionArgs& a, const SharedPrefixArgs& p, const SharedPlan& s,
                  hipStream_t stream) {
   const uint32_t rows = a.batch.tokens * a.heads;
-  if (rows <= 1024u) {
+  // (Up to some seventy parts of a row.  128 rows: the call 53.7 us with four waves, 49.2 with
+  // sixteen; 512 rows 100 and 101; 3072 rows of a few parts 55.8 and 68.)
+  if (rows <= 256u) {
     shared_join_kernel<D, T, 16>
       <<<dim3(rows), 1024, 0, stream>>>(a, s.work, p.groups, s.limits.decode_most);
   } else {
@@ -413,14 +481,18 @@ void launch_join_type(const PagedAttentionArgs& a, const SharedPrefixArgs& p, co
 
 size_t attention_shared_q8_workspace_bytes(const PagedAttentionArgs& a, const SharedPrefixArgs& p,
                                            int cu_count) {
-  return plan_of(a, p, cu_count, nullptr).bytes;
+  return worth_sharing(a, p) ? plan_of(a, p, cu_count, nullptr).bytes
+                             : attention_paged_q8_workspace_bytes(a, cu_count);
 }
 
 hipError_t launch_attention_shared_q8(const PagedAttentionArgs& a, const SharedPrefixArgs& p,
                                       int cu_count, void* workspace, hipStream_t stream) {
+  if (!worth_sharing(a, p)) {
+    return launch_attention_paged_q8(a, cu_count, workspace, stream);
+  }
   const SharedPlan s = plan_of(a, p, cu_count, workspace);
   shared_plan_kernel<<<dim3(1), kPlanThreads, 0, stream>>>(a, p, s.limits, s.lists);
-  launch_shared_decode(a, s.work, s.limits.decode_rows, s.decode_workgroups, stream);
+  launch_shared_decode(a, s.work, 1u << s.limits.decode_shift, s.decode_workgroups, stream);
   if (s.tile_workgroups != 0u) {
     launch_shared_tiles(a, s.work, s.tile_workgroups, stream);
   }
