@@ -22,6 +22,7 @@
 #include "attention_paged_q8_common.hpp"
 #include "context_internal.hpp"
 #include "device_common.hpp"
+#include "key_weights_internal.hpp"
 
 namespace kraken {
 namespace {
@@ -42,6 +43,7 @@ struct WeightPlan {
   uint32_t chunks;                  // most of a sequence
   uint32_t blocks;                  // most 256-key blocks of a sequence
   uint32_t keys;                    // longest sequence
+  uint32_t least_rows;              // sequences of fewer are another launch's
   half_t* queries;    // [kv_heads][tiles][parts][head_dim / 16][64][8]
   float* factors;     // [kv_heads][tiles * 32]: of a product to log2 units
   uint32_t* visible;  // [tiles * 32]: keys that the row sees; 0: counts nowhere
@@ -60,7 +62,8 @@ struct RowRange {
 
 __device__ __forceinline__ RowRange row_range(const KeyWeightsArgs& a, const WeightPlan& p,
                                               const PagedSequence& s) {
-  if (s.count == 0 || s.length > a.stride) {
+  const uint32_t rows = counted_rows(a, s, p.group);
+  if (rows == 0 || rows < p.least_rows) {
     return {0u, 0u, false};
   }
   const uint32_t begin = s.start + s.count - min(s.count, a.window);
@@ -89,7 +92,7 @@ __device__ __forceinline__ uint32_t work_of(const KeyWeightsArgs& a, const Weigh
 // else its earlier weight, if it had one, decayed.
 __device__ __forceinline__ float earlier_weight(const KeyWeightsArgs& a, const RowRange& r,
                                                 const float* at, bool had) {
-  return !r.first ? *at : a.decay > 0.0f && had ? a.decay * *at : 0.0f;
+  return r.first ? decayed_weight(a, at, had) : *at;
 }
 
 // One workgroup a tile of 32 rows of a KV head: eight threads a row.
@@ -110,7 +113,8 @@ __global__ __launch_bounds__(kThreads) void weight_rows_kernel(KeyWeightsArgs a,
     PagedSequence s{0u, 0u, 0u};
     if (at + lane < a.rows.batch.sequences) {
       s = paged_sequence(a.rows.batch, at + lane, a.rows.cache.page_shift);
-      if (s.length > a.stride) {
+      const uint32_t rows = counted_rows(a, s, p.group);
+      if (rows == 0 || rows < p.least_rows) {
         s.count = 0;
       }
     }
@@ -466,9 +470,8 @@ size_t plan_of(const KeyWeightsArgs& a, int cu_count, void* workspace, WeightPla
   const PagedQ8Args& c = a.rows.cache;
   p = WeightPlan{};
   p.group = a.rows.heads / c.kv_heads;
-  // What a length cannot pass.
-  const uint64_t table = (uint64_t)a.rows.batch.width << c.page_shift;
-  p.keys = (uint32_t)std::min<uint64_t>({a.rows.batch.max_keys, table, a.stride});
+  p.keys = longest_length(a);
+  p.least_rows = few_weights_bytes(a, cu_count) != 0u ? kFewRows + 1u : 0u;
   p.blocks = (p.keys + kBlockKeys - 1u) / kBlockKeys;
   // Rows in groups whose statistics take no more than 256 MiB (or one token's).
   const uint64_t token_bytes =
@@ -541,14 +544,34 @@ void launch_type(const KeyWeightsArgs& a, const WeightPlan& p, uint32_t group_to
 
 }  // namespace
 
+namespace {
+
+// Whether a sequence may have more rows than a call keeps scores of.
+bool has_many(const KeyWeightsArgs& a, size_t few_bytes) {
+  const uint64_t group = a.rows.heads / a.rows.cache.kv_heads;
+  return few_bytes == 0u || std::min(a.window, a.rows.batch.max_query) * group > kFewRows;
+}
+
+}  // namespace
+
 size_t key_weights_workspace_bytes(const KeyWeightsArgs& a, int cu_count) {
   WeightPlan p;
   uint32_t group_tokens;
-  return plan_of(a, cu_count, nullptr, p, group_tokens);
+  const size_t few = few_weights_bytes(a, cu_count);
+  return std::max(few,
+                  has_many(a, few) ? plan_of(a, cu_count, nullptr, p, group_tokens) : 0u);
 }
 
 hipError_t launch_key_weights(const KeyWeightsArgs& a, int cu_count, void* workspace,
                               hipStream_t stream) {
+  // (One after the other on the stream, in the same workspace.)
+  const size_t few = few_weights_bytes(a, cu_count);
+  if (few != 0u) {
+    launch_few_weights(a, cu_count, workspace, stream);
+  }
+  if (!has_many(a, few)) {
+    return hipGetLastError();
+  }
   WeightPlan p;
   uint32_t group_tokens;
   plan_of(a, cu_count, workspace, p, group_tokens);
