@@ -6,8 +6,8 @@
 // The first launch is the score half of the attention's decode kernel
 // (attention_paged_q8.hip): a workgroup takes one KV head of one sequence and a run of its
 // keys, its four waves 32-key steps in turn, S^T = K Q^T (16x16x32), the f32 query's two
-// f16 parts in one product's columns up to 8 rows.  It leaves the scores in log2 units as
-// [step][row][32] and each row's maximum and sum.  The second joins those and adds
+// f16 parts in one product's columns up to 8 rows.  It leaves the scores in log2 units and
+// each row's maximum and sum.  The second joins those and adds
 // 2^(score - log2 of the row's sum) over the rows of each key.
 #include <hip/hip_runtime.h>
 
@@ -38,14 +38,21 @@ struct FewPlan {
 
 __device__ __forceinline__ bool takes_few(uint32_t rows) { return rows != 0 && rows <= kFewRows; }
 
+// (Whole numbers, the query as 31 bits in four columns of 8-bit products, spare the codes'
+// way to f16, and took as long: 64 sequences of up to 32768 keys, four rows, 138 us both.  The
+// call without its stores takes 111, the keys alone 97: the 34 MB of scores cost 27.)
 template <int D, class T, bool kStacked>
-__global__ __launch_bounds__(kThreads, 3) void few_scores_kernel(KeyWeightsArgs a, FewPlan p) {
+__global__ __launch_bounds__(kThreads, D == 256 && !kStacked ? 2 : 3) void few_scores_kernel(
+  KeyWeightsArgs a, FewPlan p) {
   constexpr uint32_t kRows = kStacked ? 8 : 16;
   constexpr bool kTwo = !kStacked && std::is_same<T, float>::value;
-  constexpr int kLoads = D / 64;  // 16-byte loads of a key row per lane and row tile
+  constexpr int kLoads = D / 64;        // of 16 keys: 1024 bytes each
+  constexpr uint32_t kChunks = D / 16;  // of 16 bytes in a key row
   __shared__ float2 joined[kWaves][kRows];
+  __shared__ __attribute__((aligned(16))) int8_t lds[kWaves][32 * D];
 
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t n = lane & 15u, g = lane >> 4;
   const uint32_t shift = a.rows.cache.page_shift, kv_heads = a.rows.cache.kv_heads;
   const uint32_t kv_head = blockIdx.x % kv_heads;
@@ -63,42 +70,75 @@ __global__ __launch_bounds__(kThreads, 3) void few_scores_kernel(KeyWeightsArgs 
   const uint32_t begin = part * p.part_keys, end = min(s.length, begin + p.part_keys);
   const uint32_t steps = (end - begin + 31u) / 32u;
   const size_t pair = (size_t)found.index * kv_heads + kv_head;
-  const int32_t* table = a.rows.batch.table + (size_t)found.index * a.rows.batch.width;
-  auto page_of = [&](uint32_t key) {
-    return table[min(key >> shift, a.rows.batch.width - 1u)];
-  };
   auto first_key = [&](uint32_t step) { return begin + step * 32u; };
-  // Of the lane's key rows (run n / 4 of the step's four) and of its scores' run g.
-  auto place_k = [&](uint32_t step) { return first_key(step) + 8u * (n >> 2) + (n & 3u); };
-
-  u32x4_t k[2][kLoads];
-  auto load_k = [&](uint32_t step, int32_t page) {
-    const uint32_t held = page >= 0 && (uint32_t)page < a.rows.cache.pages ? (uint32_t)page : 0u;
-    const int8_t* at = a.rows.cache.keys +
-                       ((((size_t)held * kv_heads + kv_head) << shift) +
-                        (place_k(step) & ((1u << shift) - 1u))) * D + 16u * g;
+  // Lane 2 i + h has the page (-1: none) and the scale of granule h, 16 keys, of the wave's
+  // step i: a part has up to 32 for each wave.  (Table loads between the keys' would be
+  // waited for with all keys before them.)
+  int32_t pages;
+  float scales;
+  {
+    const uint32_t key = first_key(wave + kWaves * (lane >> 1)) + 16u * (lane & 1u);
+    const int32_t page = a.rows.batch.table[(size_t)found.index * a.rows.batch.width +
+                                            min(key >> shift, a.rows.batch.width - 1u)];
+    pages = page >= 0 && (uint32_t)page < a.rows.cache.pages ? page : -1;
+    scales = a.rows.cache.key_scales[(size_t)max(pages, 0) * kv_heads + kv_head];
+  }
+  // A load of the wave is 1024 bytes of keys as they lie, 64 / kChunks rows; through LDS, a
+  // region for each wave, they get to the lanes whose operands they are.  Chunk c of key row
+  // r is held at place c ^ turn(r) of its row, so that the sixteen rows of an operand, runs
+  // of four, lie in as many places.  Two steps' keys are on their way at a time.
+  auto turn = [](uint32_t r) { return ((r >> 3 & 3u) * 4u + (r & 3u)) & (kChunks - 1u); };
+  u32x4_t k[2][2 * kLoads];
+  auto load_k = [&](auto parity, uint32_t i) {  // of the wave's step i
+    constexpr int kBuffer = decltype(parity)::value;
+    const uint32_t key = first_key(wave + kWaves * i);
 #pragma unroll
-    for (int i = 0; i < 2 * kLoads; ++i) {
-      k[i / kLoads][i % kLoads] = __builtin_nontemporal_load(
-        reinterpret_cast<const u32x4_t*>(at + i / kLoads * 4 * D + 64 * (i % kLoads)));
+    for (int half = 0; half < 2; ++half) {
+      const int32_t page = __builtin_amdgcn_readlane(pages, (int)(2u * i + half & 63u));
+      const uint32_t slot = (key + 16u * half) & ((1u << shift) - 1u);
+      const int8_t* at = a.rows.cache.keys +
+                         ((((size_t)max(page, 0) * kv_heads + kv_head) << shift) + slot) * D;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        k[kBuffer][half * kLoads + j] =
+          __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(at + 1024u * j + lane * 16u));
+      }
     }
   };
-  float key_scale = 0.0f;
-  bool inside = false;
-  auto load_scale = [&](int32_t page) {
-    inside = page >= 0 && (uint32_t)page < a.rows.cache.pages;
-    key_scale = a.rows.cache.key_scales[(size_t)(inside ? page : 0) * kv_heads + kv_head];
+  // Scores at [step][row][32] of the part.  Lanes without a row, and steps past the last, lie
+  // outside the resource.  (A store under a branch leaves the compiler not knowing how many
+  // are under way, and a wait for keys then is one for keys behind them, too: so there is one
+  // with each step's loads from the first on.)
+  const __amdgpu_buffer_rsrc_t scores = make_buffer_rsrc(
+    p.scores + (pair * p.steps + begin / 32u) * p.rows * 32u, steps * p.rows * 128u);
+  constexpr uint32_t kNowhere = 0xffffffe0u;
+  auto store4 = [&](const float* x, uint32_t at) {
+    __builtin_amdgcn_raw_buffer_store_b128(
+      u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+              __float_as_uint(x[3])}, scores, (int)at, 0, 0);
   };
-  int32_t page_k = page_of(place_k(wave)), page_s = page_of(first_key(wave) + 8u * g);
+  auto store_nothing = [&]() {
+    const float x[4] = {};
+    store4(x, kNowhere);
+    if constexpr (!kStacked) {
+      store4(x, kNowhere);
+    }
+  };
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, 1>;
 
-  // This lane's query row and the keys that it sees.
-  const uint32_t row = kStacked ? n & 7u : n;
+  // Row n of a tile's product is key 8 (n / 4) + n % 4, of the second tile 4 on, so that a
+  // lane's scores are those of run g of eight keys.
+  const uint32_t key_row = 8u * (n >> 2) + (n & 3u), key_turn = turn(key_row);
+  // This lane's query row and the keys that it sees of the part.
+  const uint32_t row = n & (kRows - 1u);
   const bool real = row < rows;
   const uint32_t token = s.count - min(s.count, a.window) + (real ? row / p.group : 0u);
-  const uint32_t visible = s.length - s.count + token + 1u;
+  const uint32_t visible = min(s.length - s.count + token + 1u, end);
   const T* query = static_cast<const T*>(a.rows.query) +
                    ((size_t)(s.start + token) * a.rows.heads + kv_head * p.group +
                     (real ? row % p.group : 0u)) * D + 16u * g;
+  // Dimensions 64 c + 16 g .. + 15 of the row.
   half8_t q_hi[2 * kLoads], q_lo[kTwo ? 2 * kLoads : 1];
   float row_factor;
   {
@@ -110,10 +150,8 @@ __global__ __launch_bounds__(kThreads, 3) void few_scores_kernel(KeyWeightsArgs 
         load4(query + 64 * c + 4 * i, &x[c][4 * i]);
       }
     }
-    if (wave < steps) {
-      load_k(wave, page_k);
-      load_scale(page_s);
-    }
+    load_k(Even{}, 0u);
+    store_nothing();
 #pragma unroll
     for (int c = 0; c < kLoads; ++c) {
 #pragma unroll
@@ -140,33 +178,43 @@ __global__ __launch_bounds__(kThreads, 3) void few_scores_kernel(KeyWeightsArgs 
           lo[i] = w[0];
           lo[i + 1] = w[1];
         }
-        if constexpr (kStacked) {
-          q_hi[2 * c + h] = n < 8u ? hi : lo;
-        } else {
-          q_hi[2 * c + h] = hi;
-          if constexpr (kTwo) {
-            q_lo[2 * c + h] = lo;
-          }
+        // Stacked: the high parts of rows n, then the low ones of rows n - 8.
+        q_hi[2 * c + h] = kStacked && n >= 8u ? lo : hi;
+        if constexpr (kTwo) {
+          q_lo[2 * c + h] = lo;
         }
       }
     }
   }
+  load_k(Odd{}, 1u);
+  store_nothing();
 
   float top = kLowestMax, sum = 0.0f;
-  for (uint32_t step = wave; step < steps; step += kWaves) {
-    const uint32_t next = step + kWaves;
-    if (next < steps) {
-      page_k = page_of(place_k(next));
-      page_s = page_of(first_key(next) + 8u * g);
+  auto take = [&](auto parity, uint32_t i) {
+    constexpr int kBuffer = decltype(parity)::value;
+    const uint32_t step = wave + kWaves * i;
+#pragma unroll
+    for (int j = 0; j < 2 * kLoads; ++j) {
+      const uint32_t r = (uint32_t)j * (64u / kChunks) + lane / kChunks;
+      *reinterpret_cast<u32x4_t*>(&lds[wave][r * D + (lane % kChunks ^ turn(r)) * 16u]) =
+        k[kBuffer][j];
     }
+    // (A wave's own LDS instructions run in order; the compiler has to keep it.)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    auto chunk = [&](int tile, int c) {
+      return *reinterpret_cast<const u32x4_t*>(
+        &lds[wave][(key_row + 4u * tile) * D + ((4u * c + g) ^ key_turn) * 16u]);
+    };
     float4_t score[2] = {float4_t{0.0f, 0.0f, 0.0f, 0.0f}, float4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
     for (int c = 0; c < kLoads; ++c) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int tile = 0; tile < 2; ++tile) {
+        const u32x4_t codes = chunk(tile, c);
 #pragma unroll
-        for (int tile = 0; tile < 2; ++tile) {
-          const half8_t x = codes_to_f16(k[tile][c][2 * h], k[tile][c][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) {
+          const half8_t x = codes_to_f16(codes[2 * h], codes[2 * h + 1]);
           score[tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q_hi[2 * c + h], score[tile],
                                                                0, 0, 0);
           if constexpr (kTwo) {
@@ -176,36 +224,52 @@ __global__ __launch_bounds__(kThreads, 3) void few_scores_kernel(KeyWeightsArgs 
         }
       }
     }
-    const float factor = inside ? row_factor * key_scale : 0.0f;
+    load_k(parity, i + 2u);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int from = (int)(2u * i & 63u);
+    const bool second = g >= 2u;  // the run's granule
+    const int32_t page0 = __builtin_amdgcn_readlane(pages, from);
+    const int32_t page1 = __builtin_amdgcn_readlane(pages, from + 1);
+    const int scale0 = __builtin_amdgcn_readlane(__float_as_int(scales), from);
+    const int scale1 = __builtin_amdgcn_readlane(__float_as_int(scales), from + 1);
+    const bool inside = (second ? page1 : page0) >= 0;
+    const float factor = inside ? row_factor * __int_as_float(second ? scale1 : scale0) : 0.0f;
     const float offset = inside ? 0.0f : -INFINITY;
-    if (next < steps) {
-      load_k(next, page_k);
-      load_scale(page_s);
-    }
-    const uint32_t key = first_key(step) + 8u * g;
-    float w[8], largest = kLowestMax;
+    const uint32_t key = first_key(step) + 8u * g, at = (step * p.rows + row) * 128u + 32u * g;
+    float w[8], up = top;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float x = score[i / 4][i % 4];
+    for (int j = 0; j < 8; ++j) {
+      w[j] = score[j / 4][j % 4];
       if constexpr (kStacked) {
-        x += dpp<kDppRowRor8>(x);
+        w[j] += dpp<kDppRowRor8>(w[j]);
       }
-      w[i] = fmaf(x, factor, offset);
-      w[i] = key + i < visible ? w[i] : -INFINITY;
-      largest = fmaxf(largest, w[i]);
+      w[j] = fmaf(w[j], factor, offset);
+      w[j] = key + j < visible ? w[j] : -INFINITY;
+      up = fmaxf(up, w[j]);
     }
-    if (real && n < kRows) {
-      float* at = p.scores + ((pair * p.steps + begin / 32u + step) * p.rows + row) * 32u + 8u * g;
-      *reinterpret_cast<float4_t*>(at) = float4_t{w[0], w[1], w[2], w[3]};
-      *reinterpret_cast<float4_t*>(at + 4) = float4_t{w[4], w[5], w[6], w[7]};
+    if constexpr (kStacked) {
+      // (The upper lanes have the lower ones' scores, and store the second half of them.)
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = n < 8u ? w[j] : w[4 + j];
+      }
+      store4(x, real ? at + (n < 8u ? 0u : 16u) : kNowhere);
+    } else {
+      store4(w, real ? at : kNowhere);
+      store4(w + 4, real ? at + 16u : kNowhere);
     }
-    const float up = fmaxf(top, largest);
     sum *= fast_exp2(top - up);
     top = up;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum += fast_exp2(w[i] - top);
+    for (int j = 0; j < 8; ++j) {
+      sum += fast_exp2(w[j] - top);
     }
+  };
+  for (uint32_t i = 0; wave + kWaves * i < steps; i += 2u) {
+    take(Even{}, i);
+    take(Odd{}, i + 1u);  // past the last step: no key counts
   }
   // The four runs of a step, then the waves.
   {
@@ -213,8 +277,8 @@ __global__ __launch_bounds__(kThreads, 3) void few_scores_kernel(KeyWeightsArgs 
     sum = xor32_sum(xor16_sum(sum * fast_exp2(top - up)));
     top = up;
   }
-  if (g == 0 && n < kRows) {
-    joined[wave][n] = make_float2(top, sum);
+  if (lane < kRows) {
+    joined[wave][lane] = make_float2(top, sum);
   }
   __syncthreads();
   if (threadIdx.x < rows) {
@@ -230,7 +294,10 @@ __global__ __launch_bounds__(kThreads, 3) void few_scores_kernel(KeyWeightsArgs 
   }
 }
 
+// Four keys a thread.
 __global__ __launch_bounds__(kThreads) void few_sums_kernel(KeyWeightsArgs a, FewPlan p) {
+  static_assert(kSumKeys == 4u * kThreads, "");
+  constexpr uint32_t kAhead = 4;  // rows whose scores are asked for before their logs are known
   __shared__ float logs[kFewRows];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t kv_heads = a.rows.cache.kv_heads, kv_head = blockIdx.x % kv_heads;
@@ -245,6 +312,25 @@ __global__ __launch_bounds__(kThreads) void few_sums_kernel(KeyWeightsArgs a, Fe
   const uint32_t rows = counted_rows(a, s, p.group);
   const size_t pair = (size_t)found.index * kv_heads + kv_head;
   const uint32_t parts = (s.length + p.part_keys - 1u) / p.part_keys;
+  const uint32_t key = found.item * kSumKeys + 4u * threadIdx.x;
+  // (Within the steps that were written: those of keys up to the length.)
+  const uint32_t step = min(key / 32u, (s.length - 1u) / 32u);
+  const float* scores = p.scores + (pair * p.steps + step) * p.rows * 32u + key % 32u;
+  auto score = [&](uint32_t row) {
+    return *reinterpret_cast<const float4_t*>(scores + min(row, rows - 1u) * 32u);
+  };
+  float4_t ahead[kAhead];
+#pragma unroll
+  for (uint32_t i = 0; i < kAhead; ++i) {
+    ahead[i] = score(i);
+  }
+  float* at = a.weights + pair * a.row_stride + key;
+  const uint32_t before = s.length - s.count;
+  float earlier[4];
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    earlier[i] = decayed_weight(a, at + i, key + i < before);
+  }
   // log2 of each row's sum; infinity, which makes its weights zero, without any key.
   for (uint32_t row = wave; row < rows; row += kWaves) {
     float top = kLowestMax, sum = 0.0f;
@@ -261,19 +347,26 @@ __global__ __launch_bounds__(kThreads) void few_sums_kernel(KeyWeightsArgs a, Fe
     }
   }
   __syncthreads();
-  const uint32_t before = s.length - s.count;
+  float sums[4] = {};
+  auto add = [&](const float4_t& x, uint32_t row) {
 #pragma unroll
-  for (uint32_t i = 0; i < kSumKeys / kThreads; ++i) {
-    const uint32_t key = found.item * kSumKeys + i * kThreads + threadIdx.x;
-    if (key < s.length) {
-      const float* scores =
-        p.scores + (pair * p.steps + key / 32u) * p.rows * 32u + key % 32u;
-      float sum = 0.0f;
-      for (uint32_t row = 0; row < rows; ++row) {
-        sum += fast_exp2(scores[row * 32u] - logs[row]);
-      }
-      float* at = a.weights + pair * a.row_stride + key;
-      *at = sum + decayed_weight(a, at, key < before);
+    for (uint32_t i = 0; i < 4; ++i) {
+      sums[i] += fast_exp2(x[i] - logs[row]);
+    }
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < kAhead; ++i) {
+    if (i < rows) {
+      add(ahead[i], i);
+    }
+  }
+  for (uint32_t row = kAhead; row < rows; ++row) {
+    add(score(row), row);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    if (key + i < s.length) {
+      at[i] = sums[i] + earlier[i];
     }
   }
 }
@@ -310,10 +403,11 @@ FewPlan plan_of(const KeyWeightsArgs& a, int cu_count, size_t& bytes, void* work
 template <int D, class T>
 void launch_for(const KeyWeightsArgs& a, const FewPlan& p, hipStream_t stream) {
   const uint32_t pairs = a.rows.batch.sequences * a.rows.cache.kv_heads;
+  const dim3 grid(pairs * p.parts);
   if (p.rows <= 8u) {
-    few_scores_kernel<D, T, true><<<dim3(pairs * p.parts), kThreads, 0, stream>>>(a, p);
+    few_scores_kernel<D, T, true><<<grid, kThreads, 0, stream>>>(a, p);
   } else {
-    few_scores_kernel<D, T, false><<<dim3(pairs * p.parts), kThreads, 0, stream>>>(a, p);
+    few_scores_kernel<D, T, false><<<grid, kThreads, 0, stream>>>(a, p);
   }
   const uint32_t blocks = (p.steps * 32u + kSumKeys - 1u) / kSumKeys;
   few_sums_kernel<<<dim3(pairs * blocks), kThreads, 0, stream>>>(a, p);
