@@ -32,6 +32,7 @@ constexpr uint32_t kWaves = kThreads / 64u;
 constexpr uint32_t kTile = 32;                       // rows of a product
 constexpr uint32_t kWaveKeys = 64;
 constexpr uint32_t kBlockKeys = kWaves * kWaveKeys;  // of a workgroup
+constexpr int kRing = 2;  // fragments of rows on their way from LDS
 
 // A call's rows [0, tokens * group) of each KV head in groups of tokens, and the
 // workspace of one.
@@ -190,12 +191,11 @@ __global__ __launch_bounds__(kThreads) void weight_rows_kernel(KeyWeightsArgs a,
 
 // A pass over a block of 256 keys and a chunk of row tiles.
 template <int D, class T, bool kSums>
-__global__ __launch_bounds__(kThreads, 1) void weight_pass_kernel(KeyWeightsArgs a, WeightPlan p) {
+__global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs a, WeightPlan p) {
   constexpr bool kTwo = std::is_same<T, float>::value;
   constexpr int kParts = kTwo ? 2 : 1, kSteps = D / 16, kSubs = kWaveKeys / 32;
   constexpr uint32_t kTileHalves = kParts * kSteps * 512u;
-  constexpr int kLoads = kTileHalves / 8 / kThreads;  // of 16 bytes a thread
-  static_assert(kLoads >= 1, "a tile has 16 bytes for every thread");
+  constexpr uint32_t kCopies = kTileHalves / 512u / kWaves;  // of 1024 bytes a wave
   __shared__ __attribute__((aligned(16))) half_t lds[2][kTileHalves];
   __shared__ float2 joined[2][kWaves][kTile];
 
@@ -225,23 +225,23 @@ __global__ __launch_bounds__(kThreads, 1) void weight_pass_kernel(KeyWeightsArgs
     };
     auto inside = [&](int32_t page) { return page >= 0 && (uint32_t)page < a.rows.cache.pages; };
 
-    // The rows' first tile on its way while the keys are fetched.
-    u32x4_t ahead[kLoads];
-    const u32x4_t* source = reinterpret_cast<const u32x4_t*>(
-      p.queries + (size_t)kv_head * p.tiles * kTileHalves);
-    auto fetch = [&](uint32_t tile) {
+    // A tile goes from memory to LDS by itself (registers on its way are what two waves a
+    // SIMD do not have); the wave waits for its copies, the workgroup for all.
+    auto copy = [&](uint32_t tile, uint32_t parity) {
+      const i32x4_t from =
+        rsrc_words(p.queries + ((size_t)kv_head * p.tiles + tile) * kTileHalves, kTileHalves * 2u);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        ahead[i] = source[(size_t)tile * (kTileHalves / 8u) + tid + kThreads * i];
+      for (uint32_t i = 0; i < kCopies; ++i) {
+        const uint32_t at = (wave * kCopies + i) * 512u;
+        copy16_to_lds(from, at * 2u + lane * 16u, lds[parity] + at);
       }
     };
-    auto publish = [&](uint32_t parity) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        reinterpret_cast<u32x4_t*>(lds[parity])[tid + kThreads * i] = ahead[i];
-      }
+    auto arrived = [&]() {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
     };
-    fetch(begin_tile);
+    __syncthreads();  // the item before has read its tiles
+    copy(begin_tile, 0);
 
     // Row r of a product is key swap(r), bits 2 and 3 in each other's place, so that a
     // lane's registers are runs of eight keys: 8 b + i of half h is key 16 b + 8 h + i.
@@ -279,78 +279,102 @@ __global__ __launch_bounds__(kThreads, 1) void weight_pass_kernel(KeyWeightsArgs
     for (int sub = 0; sub < kSubs; ++sub) {
       sums[sub] = float16_t{};
     }
-    __syncthreads();  // the item before has read its tiles
-    publish(0);
-    __syncthreads();
-
+    // The lane's row's values, a tile ahead.
+    struct Values {
+      uint32_t visible;
+      float factor, log;
+    };
+    auto values_of = [&](uint32_t tile) {
+      const uint32_t row = tile * kTile + n;
+      return Values{p.visible[row], p.factors[(size_t)kv_head * padded + row],
+                    kSums ? p.logs[(size_t)kv_head * padded + row] : 0.0f};
+    };
+    Values values = values_of(begin_tile);
+    arrived();
     for (uint32_t tile = begin_tile; tile < stop_tile; ++tile) {
       const uint32_t parity = (tile - begin_tile) & 1u;
-      if (tile + 1u < stop_tile) {
-        fetch(tile + 1u);
-      }
+      const uint32_t following = min(tile + 1u, stop_tile - 1u);
       const uint32_t row = tile * kTile + n;
-      const uint32_t seen = row >= range.begin && row < range.end ? p.visible[row] : 0u;
-      const float factor = p.factors[(size_t)kv_head * padded + row];
-      const float log = kSums ? p.logs[(size_t)kv_head * padded + row] : 0.0f;
+      const bool own = row >= range.begin && row < range.end;
+      const uint32_t seen = own ? values.visible : 0u;
+      const float factor = values.factor, log = values.log;
+      values = values_of(following);
+      if (tile + 1u < stop_tile) {
+        copy(tile + 1u, parity ^ 1u);
+      }
       float top = kLowestMax, sum = 0.0f;
-      if (__any(seen > first_key)) {
-        float16_t score[kSubs];
+      const bool any = __any(seen > first_key);  // else no row sees the wave's keys
+      float16_t score[kSubs];
+      // Fragments of the rows kRing ahead of the products that take them.
+      const half8_t* q = reinterpret_cast<const half8_t*>(lds[parity]) + lane;
+      half8_t ring[kRing];
+      if (any) {
 #pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub) {
-          score[sub] = float16_t{};
+        for (int i = 0; i < kRing; ++i) {
+          ring[i] = q[i * 64];
         }
-        const half8_t* q = reinterpret_cast<const half8_t*>(lds[parity]) + lane;
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) {
+        for (int i = 0; i < kParts * kSteps; ++i) {
 #pragma unroll
-          for (int c = 0; c < kSteps; ++c) {
-            const half8_t x = q[(part * kSteps + c) * 64];
-#pragma unroll
-            for (int sub = 0; sub < kSubs; ++sub) {
-              score[sub] =
-                __builtin_amdgcn_mfma_f32_32x32x16_f16(k[sub][c], x, score[sub], 0, 0, 0);
-            }
+          for (int sub = 0; sub < kSubs; ++sub) {
+            score[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+              k[sub][i % kSteps], ring[i % kRing], i == 0 ? float16_t{} : score[sub], 0, 0, 0);
           }
+          if (i + kRing < kParts * kSteps) {
+            ring[i % kRing] = q[(i + kRing) * 64];
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        const bool masked = __any(seen < first_key + kWaveKeys);
-        if constexpr (kSums) {
+        float scaled[2 * kSubs];
+#pragma unroll
+        for (int b = 0; b < 2 * kSubs; ++b) {
+          scaled[b] = factor * scale[b];
+        }
+        // Keys that a row does not see add nothing, whatever their scores are.
+        auto soften = [&](auto masks) {
+          constexpr bool kMasked = decltype(masks)::value;
+          auto exponent = [&](int sub, int r, float base) {
+            const int b = 2 * sub + r / 8;
+            const float y = fmaf(score[sub][r], scaled[b], base);
+            return !kMasked || first_key + 16u * b + 8u * h + r % 8 < seen ? y : -INFINITY;
+          };
+          if constexpr (!kSums) {
+            // (A scale is not negative: the largest score of a run of keys is that of its
+            // largest product.)
+#pragma unroll
+            for (int b = 0; b < 2 * kSubs; ++b) {
+              float largest = -INFINITY;
+#pragma unroll
+              for (int r = 8 * (b % 2); r < 8 * (b % 2) + 8; ++r) {
+                const bool sees = !kMasked || first_key + 16u * b + 8u * h + r % 8 < seen;
+                largest = fmaxf(largest, sees ? score[b / 2][r] : -INFINITY);
+              }
+              const float y = fmaf(largest, scaled[b], offset[b]);
+              top = largest > -INFINITY ? fmaxf(top, y) : top;
+            }
+            top = xor32_max(top);
+          }
 #pragma unroll
           for (int sub = 0; sub < kSubs; ++sub) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int b = 2 * sub + r / 8;
-              float y = fmaf(score[sub][r], factor * scale[b], offset[b] - log);
-              if (masked) {
-                const uint32_t key = first_key + 16u * b + 8u * h + r % 8;
-                y = key < seen ? y : -INFINITY;
+              const float base = offset[2 * sub + r / 8] - (kSums ? log : top);
+              const float w = fast_exp2(exponent(sub, r, base));
+              if constexpr (kSums) {
+                sums[sub][r] += w;
+              } else {
+                sum += w;
               }
-              sums[sub][r] += fast_exp2(y);
             }
           }
+          if constexpr (!kSums) {
+            sum = xor32_sum(sum);
+          }
+        };
+        if (__any(seen < first_key + kWaveKeys)) {
+          soften(std::true_type{});
         } else {
-#pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int b = 2 * sub + r / 8;
-              float y = fmaf(score[sub][r], factor * scale[b], offset[b]);
-              if (masked) {
-                const uint32_t key = first_key + 16u * b + 8u * h + r % 8;
-                y = key < seen ? y : -INFINITY;
-              }
-              score[sub][r] = y;
-              top = fmaxf(top, y);
-            }
-          }
-          top = xor32_max(top);
-#pragma unroll
-          for (int sub = 0; sub < kSubs; ++sub) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              sum += fast_exp2(score[sub][r] - top);
-            }
-          }
-          sum = xor32_sum(sum);
+          soften(std::false_type{});
         }
       }
       if constexpr (!kSums) {
@@ -358,13 +382,10 @@ __global__ __launch_bounds__(kThreads, 1) void weight_pass_kernel(KeyWeightsArgs
           joined[parity][wave][n] = make_float2(top, sum);
         }
       }
-      if (tile + 1u < stop_tile) {
-        publish(parity ^ 1u);
-      }
-      __syncthreads();
+      arrived();
       if constexpr (!kSums) {
         // (The other parity's are written meanwhile, these again behind another barrier.)
-        if (wave == 0 && h == 0 && row >= range.begin && row < range.end) {
+        if (wave == 0 && h == 0 && own) {
           float2 all = joined[parity][0][n];
 #pragma unroll
           for (uint32_t w = 1; w < kWaves; ++w) {
@@ -378,24 +399,22 @@ __global__ __launch_bounds__(kThreads, 1) void weight_pass_kernel(KeyWeightsArgs
       }
     }
     if constexpr (kSums) {
-      // Over the rows, which are the lanes of each half.
+      // Over the rows, which are the lanes of each half; lane n keeps register n.
+      static_assert(16 * kSubs == 32, "a register for each lane of a half");
+      float mine = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16 * kSubs; ++i) {
+        const float all = reduce32_sum(sums[i / 16][i % 16]);
+        mine = n == (uint32_t)i ? all : mine;
+      }
       const size_t pair = (size_t)found.index * kv_heads + kv_head;
-      const uint32_t before = s.length - s.count;
-#pragma unroll
-      for (int sub = 0; sub < kSubs; ++sub) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float all = reduce32_sum(sums[sub][r]);
-          const uint32_t key = first_key + 32u * sub + 16u * (r / 8) + 8u * h + r % 8;
-          if (n == 0 && key < s.length) {
-            if (p.chunks > 1u) {
-              p.sums[((size_t)chunk * a.rows.batch.sequences * kv_heads + pair) * p.keys + key] =
-                all;
-            } else {
-              float* at = a.weights + pair * a.row_stride + key;
-              *at = all + earlier_weight(a, range, at, key < before);
-            }
-          }
+      const uint32_t key = first_key + 16u * (n / 8u) + 8u * h + n % 8u;
+      if (key < s.length) {
+        if (p.chunks > 1u) {
+          p.sums[((size_t)chunk * a.rows.batch.sequences * kv_heads + pair) * p.keys + key] = mine;
+        } else {
+          float* at = a.weights + pair * a.row_stride + key;
+          *at = mine + earlier_weight(a, range, at, key < s.length - s.count);
         }
       }
     }
