@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "context_internal.hpp"
 #include "device_common.hpp"
@@ -14,37 +15,156 @@ namespace {
 
 constexpr uint32_t kSelectThreads = 1024;
 constexpr uint32_t kSelectWaves = kSelectThreads / 64u;
-constexpr uint32_t kGatherThreads = 256;
+constexpr uint32_t kHeld = 32;  // keys that a thread holds
+// Digits of a key, from the top: 11, 11 and 10 bits.  Softmax weights fill few values of the
+// top eight bits, their exponents, so that counts by eight bits fall on few words.
+constexpr uint32_t kDigitBits = 11, kBins = 1u << kDigitBits;
+// Counts in as many copies, by lane, so that lanes of one digit do not wait for each other.
+constexpr uint32_t kCopies = 4;
 
-// Sum over the workgroup's threads before this one, and the whole.
-__device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t& all, uint32_t* s) {
-  const uint32_t upto = wave_scan(x, Sum{});
+// Sum over the workgroup's waves before this one, and over all, of a value that each wave
+// has one of.
+__device__ __forceinline__ uint32_t waves_before(uint32_t x, uint32_t& all, uint32_t* s) {
   __syncthreads();
-  if ((threadIdx.x & 63u) == 63u) {
-    s[threadIdx.x >> 6] = upto;
+  if ((threadIdx.x & 63u) == 0) {
+    s[threadIdx.x >> 6] = x;
   }
   __syncthreads();
   uint32_t before = 0;
   all = 0;
+#pragma unroll
   for (uint32_t i = 0; i < kSelectWaves; ++i) {
     before += i < threadIdx.x >> 6 ? s[i] : 0u;
     all += s[i];
   }
-  return before + upto - x;
+  return before;
 }
 
-// One workgroup a sequence and KV head: the least key that is kept, found eight bits at a
-// time from the top by counts, then the kept positions in order, of those equal to it the
-// first few.
+struct SelectScratch {
+  uint32_t bins[kCopies][kBins];
+  uint32_t waves[kSelectWaves];
+  uint32_t digit, above;
+};
+
+// The `most` positions of the largest of `weights` [0, count), in rising order, plus `first`.
+// A wave takes a run of them, 64 at a time, a lane each: loads are of whole lines, and the
+// positions in order of wave, time and lane.  kInRegisters: up to kHeld times, each read once.
+template <bool kInRegisters>
+__device__ __forceinline__ void select_between(const float* weights, uint32_t count, uint32_t most,
+                                               uint32_t first, int32_t* kept, SelectScratch& s) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t times = (count + kSelectThreads - 1u) / kSelectThreads;  // of a wave
+  const uint32_t begin = wave * times * 64u + lane;
+  uint32_t held[kInRegisters ? kHeld : 1];
+  auto key_at = [&](uint32_t j) {
+    const uint32_t i = begin + j * 64u;
+    return i < count ? key_of(weights[i]) : 0u;
+  };
+  if constexpr (kInRegisters) {
+    float x[kHeld];
+#pragma unroll
+    for (uint32_t j = 0; j < kHeld; ++j) {
+      x[j] = j < times && begin + j * 64u < count ? weights[begin + j * 64u] : 0.0f;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kHeld; ++j) {
+      held[j] = key_of(x[j]);
+    }
+  }
+  // f(key, time) for this lane's; it has to ask whether the place is one.
+  auto each = [&](auto f) {
+    if constexpr (kInRegisters) {
+#pragma unroll
+      for (uint32_t j = 0; j < kHeld; ++j) {
+        if (j < times) {  // uniform
+          f(held[j], j);
+        }
+      }
+    } else {
+      for (uint32_t j = 0; j < times; ++j) {
+        f(key_at(j), j);
+      }
+    }
+  };
+  // The least key that is kept; `want` of those equal to it are.
+  uint32_t least = 0, known = 0, want = most;  // known: bits of `least` that are settled
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const uint32_t shift = pass == 0 ? 21u : pass == 1 ? 10u : 0u;
+    const uint32_t mask = pass == 2 ? 1023u : kBins - 1u;
+    for (uint32_t i = tid; i < kCopies * kBins; i += kSelectThreads) {
+      s.bins[0][i] = 0;
+    }
+    __syncthreads();
+    uint32_t* bins = s.bins[lane % kCopies];
+    each([&](uint32_t key, uint32_t j) {
+      if (begin + j * 64u < count && (key & known) == least) {
+        atomicAdd(&bins[key >> shift & mask], 1u);
+      }
+    });
+    __syncthreads();
+    // Two bins a thread, from the largest digit down.
+    uint32_t mine[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      mine[i] = 0;
+#pragma unroll
+      for (uint32_t copy = 0; copy < kCopies; ++copy) {
+        mine[i] += s.bins[copy][kBins - 1u - (2u * tid + i)];
+      }
+    }
+    const uint32_t upto = wave_scan(mine[0] + mine[1], Sum{});
+    uint32_t all;
+    uint32_t before = waves_before((uint32_t)__builtin_amdgcn_readlane((int)upto, 63), all,
+                                   s.waves);
+    before += upto - mine[0] - mine[1];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      if (before < want && want <= before + mine[i]) {
+        s.digit = kBins - 1u - (2u * tid + i);
+        s.above = before;
+      }
+      before += mine[i];
+    }
+    __syncthreads();
+    least |= s.digit << shift;
+    known |= mask << shift;
+    want -= s.above;
+  }
+  // How many larger and equal ones each wave has, then their places.
+  uint32_t larger = 0, equal = 0;
+  each([&](uint32_t key, uint32_t j) {
+    const bool is = begin + j * 64u < count;
+    larger += (uint32_t)__popcll(__ballot(is && key > least));
+    equal += (uint32_t)__popcll(__ballot(is && key == least));
+  });
+  uint32_t all;
+  uint32_t ties = waves_before(equal, all, s.waves);
+  uint32_t place = waves_before(larger, all, s.waves) + min(ties, want);
+  const uint64_t below = (uint64_t{1} << lane) - 1u;
+  each([&](uint32_t key, uint32_t j) {
+    const uint32_t i = begin + j * 64u;
+    const uint64_t same = __ballot(i < count && key == least);
+    const bool keep =
+      i < count && (key > least || (key == least && ties + (uint32_t)__popcll(same & below) < want));
+    const uint64_t kept_here = __ballot(keep);
+    if (keep) {
+      kept[place + (uint32_t)__popcll(kept_here & below)] = (int32_t)(first + i);
+    }
+    ties += (uint32_t)__popcll(same);
+    place += (uint32_t)__popcll(kept_here);
+  });
+}
+
+// One workgroup a sequence and KV head.
 __global__ __launch_bounds__(kSelectThreads) void select_keys_kernel(SelectKeysArgs a) {
-  __shared__ uint32_t bins[256], s[kSelectWaves];
-  __shared__ uint32_t digit, above;
+  __shared__ SelectScratch s;
   const uint32_t pair = blockIdx.x, sequence = pair / a.kv_heads, tid = threadIdx.x;
-  const uint32_t length = a.lengths[sequence];
+  const uint32_t length = a.lengths[sequence], keep = a.keep[sequence];
   if (length > a.max_keys) {
     return;
   }
-  const uint32_t k = min(a.keep[sequence], length);
+  const uint32_t k = min(keep, length);
   if (k > a.kept_stride) {
     return;
   }
@@ -53,9 +173,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_keys_kernel(SelectKeysA
   }
   // Positions [0, first) and [end, length) are kept, and `most` of those between.
   const uint32_t last = min(a.last, k), first = min(min(a.first, k - last), length - last);
-  const uint32_t end = length - last;
-  const uint32_t most = k - last - first;
-  const float* weights = a.weights + (size_t)pair * a.weight_stride;
+  const uint32_t end = length - last, most = k - last - first;
   int32_t* kept = a.kept + (size_t)pair * a.kept_stride;
   for (uint32_t i = tid; i < first; i += kSelectThreads) {
     kept[i] = (int32_t)i;
@@ -63,147 +181,192 @@ __global__ __launch_bounds__(kSelectThreads) void select_keys_kernel(SelectKeysA
   for (uint32_t i = tid; i < last; i += kSelectThreads) {
     kept[k - last + i] = (int32_t)(end + i);
   }
+  const float* weights = a.weights + (size_t)pair * a.weight_stride + first;
   if (most == 0) {
     return;
   }
-  uint32_t least = 0, want = most;  // `want` of those whose high digits are those of `least`
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256u) {
-      bins[tid] = 0;
-    }
-    __syncthreads();
-    for (uint32_t i = first + tid; i < end; i += kSelectThreads) {
-      const uint32_t key = key_of(weights[i]);
-      if (shift == 24 || key >> (shift + 8) == least >> (shift + 8)) {
-        atomicAdd(&bins[key >> shift & 255u], 1u);
-      }
-    }
-    __syncthreads();
-    // From the largest digit down.
-    const uint32_t mine = tid < 256u ? bins[255u - tid] : 0u;
-    uint32_t all;
-    const uint32_t before = block_before(mine, all, s);
-    if (before < want && want <= before + mine) {
-      digit = 255u - tid;
-      above = before;
-    }
-    __syncthreads();
-    least |= digit << shift;
-    want -= above;
-  }
-  uint32_t at = first, ties = 0;
-  for (uint32_t base = first; base < end; base += kSelectThreads) {
-    const uint32_t i = base + tid;
-    const uint32_t key = i < end ? key_of(weights[i]) : 0u;
-    const bool equal = i < end && key == least;
-    uint32_t all;
-    const uint32_t tie = ties + block_before(equal ? 1u : 0u, all, s);
-    ties += all;
-    const bool keep = i < end && (key > least || (equal && tie < want));
-    const uint32_t place = at + block_before(keep ? 1u : 0u, all, s);
-    at += all;
-    if (keep) {
-      kept[place] = (int32_t)i;
-    }
+  if (end - first <= kHeld * kSelectThreads) {
+    select_between<true>(weights, end - first, most, first, kept + first, s);
+  } else {
+    select_between<false>(weights, end - first, most, first, kept + first, s);
   }
 }
 
-// A kept token's place in the source pages; page -1 where there is none.
-struct Source {
-  int32_t page;
-  uint32_t slot;
-};
-
-__device__ __forceinline__ Source source_of(const GatherPagesArgs& a, uint32_t sequence,
-                                            int32_t position) {
-  const uint32_t shift = a.cache.page_shift;
-  if (position < 0 || (uint32_t)position >> shift >= a.width) {
-    return {-1, 0u};
-  }
-  const int32_t page = a.table[(size_t)sequence * a.width + ((uint32_t)position >> shift)];
-  return {page >= 0 && (uint32_t)page < a.cache.pages ? page : -1,
-          (uint32_t)position & ((1u << shift) - 1u)};
-}
+constexpr uint32_t kGatherThreads = 256;
+constexpr uint32_t kGatherWaves = kGatherThreads / 64u;
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
-// One workgroup a target page and KV head.
+// A code times a ratio, rounded to even, in the low byte: an addition of 3 2^22 leaves the
+// whole number there.  (At most 127 in size: no source's scale passes its new page's.)
+__device__ __forceinline__ uint32_t rescaled(int code, float ratio) {
+#pragma clang fp contract(off)
+  const float x = (float)code * ratio;
+  return __float_as_uint(x + 12582912.0f);
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u),
+                               __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
+
+__device__ __forceinline__ int code_at(uint32_t word, uint32_t byte) {
+  return (int)(word << (24u - 8u * byte)) >> 24;
+}
+
+// One workgroup a target page, KV head, and of keys and values: the two have scales of their
+// own.  A key's row is contiguous, 16 lanes of 16 bytes (head_dim 256) with one ratio.  Of
+// values eight tokens lie side by side for each dimension, in the source as in the target: a
+// wave builds a target run, a lane one dimension or two at a time from the eight sources' eight
+// bytes each, of which it takes one.  The sources are the wave's, so that places, bytes and
+// ratios are scalars.
+template <int D>
 __global__ __launch_bounds__(kGatherThreads) void gather_pages_kernel(GatherPagesArgs a,
                                                                       uint64_t items) {
-  __shared__ Source sources[128];
-  __shared__ float scales[2][128], ratio[2][128];
-  __shared__ float page_scale[2];
+  __shared__ uint2 places[128];  // of the source's row, or run of eight: its offset in bytes
+  __shared__ uint32_t slots[128];  // in its page; kNone: there is none
+  __shared__ float ratios[128];
+  __shared__ float most[kGatherWaves];
+  __shared__ uint32_t bad[kGatherWaves];
+  constexpr uint32_t kNone = 0xffffffffu;
   const PagedQ8Args& c = a.cache;
-  const uint32_t tid = threadIdx.x, page_tokens = 1u << c.page_shift, d = c.head_dim;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, shift = c.page_shift;
+  const uint32_t page_tokens = 1u << shift;
   for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
     __syncthreads();
-    const uint32_t head = (uint32_t)(item % c.kv_heads);
-    const uint64_t rest = item / c.kv_heads;
+    const bool of_values = item % 2u != 0u;
+    const uint64_t page_item = item / 2u;
+    const uint32_t head = (uint32_t)(page_item % c.kv_heads);
+    const uint64_t rest = page_item / c.kv_heads;
     const uint32_t p = (uint32_t)(rest % a.target_width);
     const uint32_t sequence = (uint32_t)(rest / a.target_width);
     const uint64_t pair = (uint64_t)sequence * c.kv_heads + head;
     const uint32_t n = a.kept_lengths[sequence];
-    const uint64_t begin = (uint64_t)p << c.page_shift;
-    if (begin >= n || n > a.kept_stride || n > (uint64_t)a.target_width << c.page_shift ||
+    const uint64_t begin = (uint64_t)p << shift;
+    if (begin >= n || n > a.kept_stride || n > (uint64_t)a.target_width << shift ||
         (a.weights != nullptr && n > a.weight_stride)) {
       continue;
     }
-    if (tid < page_tokens) {
-      Source from{-1, 0u};
-      if (begin + tid < n) {
-        const int32_t position = a.kept[pair * a.kept_stride + begin + tid];
-        from = source_of(a, sequence, position);
-        if (a.weights != nullptr) {
-          const float* weights = a.weights + pair * a.weight_stride;
-          a.weights_output[pair * a.weight_stride + begin + tid] =
-            position >= 0 && (uint32_t)position < a.weight_stride ? weights[position] : 0.0f;
+    const int32_t target = a.target_table[(size_t)sequence * a.target_width + p];
+    const bool writes = target >= 0 && (uint32_t)target < c.pages;
+    float scale = 0.0f;
+    uint32_t slot = kNone;
+    uint64_t place = 0;
+    if (tid < page_tokens && begin + tid < n) {
+      const int32_t position = a.kept[pair * a.kept_stride + begin + tid];
+      if (a.weights != nullptr && !of_values) {
+        const float* weights = a.weights + pair * a.weight_stride;
+        a.weights_output[pair * a.weight_stride + begin + tid] =
+          position >= 0 && (uint32_t)position < a.weight_stride ? weights[position] : 0.0f;
+      }
+      if (position >= 0 && (uint32_t)position >> shift < a.width) {
+        const int32_t page = a.table[(size_t)sequence * a.width + ((uint32_t)position >> shift)];
+        if (page >= 0 && (uint32_t)page < c.pages) {
+          slot = (uint32_t)position & (page_tokens - 1u);
+          place = (((uint64_t)page * c.kv_heads + head) << shift) * D +
+                  (of_values ? slot / 8u * (8u * D) : slot * D);
+          scale = (of_values ? c.value_scales : c.key_scales)[(size_t)page * c.kv_heads + head];
         }
       }
-      sources[tid] = from;
-      const size_t at = (size_t)max(from.page, 0) * c.kv_heads + head;
-      scales[0][tid] = from.page >= 0 ? c.key_scales[at] : 0.0f;
-      scales[1][tid] = from.page >= 0 ? c.value_scales[at] : 0.0f;
+    }
+    const bool not_finite = !finite(scale);
+    const float largest = halves_max(across8_max(reduce8_max(not_finite ? 0.0f : scale)));
+    const uint64_t spoiled = __ballot(not_finite);
+    if (lane == 0) {
+      most[wave] = largest;
+      bad[wave] = spoiled != 0;
     }
     __syncthreads();
-    const int32_t target = a.target_table[(size_t)sequence * a.target_width + p];
-    if (target < 0 || (uint32_t)target >= c.pages) {
+    if (!writes) {
       continue;
     }
-    const size_t page_head = (size_t)target * c.kv_heads + head;
-    if (tid < 2u) {
-      float most = 0.0f;
-      bool all = true;
-      for (uint32_t i = 0; i < page_tokens; ++i) {
-        most = fmaxf(most, scales[tid][i]);
-        all = all && finite(scales[tid][i]);
-      }
-      page_scale[tid] = all ? most : NAN;
-      (tid == 0 ? c.key_scales : c.value_scales)[page_head] = page_scale[tid];
-    }
-    __syncthreads();
-    if (tid < page_tokens) {
+    float page_scale = most[0];
+    uint32_t any = bad[0];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // Of a NaN page, and of equal scales (zeros too), the codes stay.
-        const float to = page_scale[i], from = scales[i][tid];
-        ratio[i][tid] = from == to || !finite(to) ? 1.0f : from / to;
-      }
+    for (uint32_t w = 1; w < kGatherWaves; ++w) {
+      page_scale = fmaxf(page_scale, most[w]);
+      any |= bad[w];
+    }
+    if (tid < page_tokens) {
+      places[tid] = make_uint2((uint32_t)place, (uint32_t)(place >> 32));
+      slots[tid] = slot;
+      // Of a page that becomes NaN, and of equal scales (zeros too), the codes stay.
+      ratios[tid] = scale == page_scale || any != 0 ? 1.0f : scale / page_scale;
+    }
+    const size_t page_head = (size_t)target * c.kv_heads + head;
+    if (tid == 0) {
+      (of_values ? c.value_scales : c.key_scales)[page_head] = any != 0 ? NAN : page_scale;
     }
     __syncthreads();
-    int8_t* keys = c.keys + (page_head << c.page_shift) * d;
-    int8_t* values = c.values + (page_head << c.page_shift) * d;
-    for (uint32_t e = tid; e < page_tokens * d; e += kGatherThreads) {
-      const uint32_t t = e / d, dim = e % d;
-      const Source from = sources[t];
-      int key = 0, value = 0;
-      if (from.page >= 0) {
-        const size_t base = (((size_t)from.page * c.kv_heads + head) << c.page_shift) * d;
-        key = c.keys[base + (size_t)from.slot * d + dim];
-        value = c.values[base + ((size_t)(from.slot / 8u) * d + dim) * 8u + from.slot % 8u];
+    if (!of_values) {
+      int8_t* to = c.keys + (page_head << shift) * D;
+      constexpr uint32_t kLanes = D / 16;  // of a row
+      constexpr uint32_t kRows = kGatherThreads / kLanes;
+      const uint32_t chunk = tid % kLanes * 16u;
+#pragma unroll 4
+      for (uint32_t t = tid / kLanes; t < page_tokens; t += kRows) {
+        const uint64_t from = (uint64_t)places[t].y << 32 | places[t].x;
+        const float ratio = ratios[t];
+        u32x4_t x = {0u, 0u, 0u, 0u};
+        if (slots[t] != kNone) {
+          x = *reinterpret_cast<const u32x4_t*>(c.keys + from + chunk);
+        }
+        if (ratio != 1.0f) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = low_bytes(rescaled(code_at(x[i], 0), ratio), rescaled(code_at(x[i], 1), ratio),
+                             rescaled(code_at(x[i], 2), ratio), rescaled(code_at(x[i], 3), ratio));
+          }
+        }
+        *reinterpret_cast<u32x4_t*>(to + t * D + chunk) = x;
       }
-      keys[e] = (int8_t)rintf((float)key * ratio[0][t]);
-      values[((size_t)(t / 8u) * d + dim) * 8u + t % 8u] =
-        (int8_t)rintf((float)value * ratio[1][t]);
+    } else {
+      int8_t* to = c.values + (page_head << shift) * D;
+      constexpr uint32_t kDims = D == 64 ? 1 : 2;      // of a lane at a time
+      constexpr uint32_t kTimes = D / (64u * kDims);
+      typedef uint32_t words_t __attribute__((ext_vector_type(2 * kDims)));
+      for (uint32_t run = wave; run < page_tokens / 8u; run += kGatherWaves) {
+        words_t x[kTimes][8];
+        uint32_t at[8];
+        float ratio[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+          const uint32_t t = 8u * run + i;
+          at[i] = (uint32_t)__builtin_amdgcn_readfirstlane((int)slots[t]);
+          ratio[i] =
+            __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(ratios[t])));
+          const uint64_t from =
+            (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)places[t].y) << 32 |
+            (uint32_t)__builtin_amdgcn_readfirstlane((int)places[t].x);
+#pragma unroll
+          for (uint32_t j = 0; j < kTimes; ++j) {
+            x[j][i] = words_t{};
+            if (at[i] != kNone) {  // uniform
+              x[j][i] = *reinterpret_cast<const words_t*>(c.values + from +
+                                                          (j * 64u + lane) * (8u * kDims));
+            }
+          }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kTimes; ++j) {
+          words_t out;
+#pragma unroll
+          for (uint32_t w = 0; w < 2u * kDims; ++w) {  // tokens 4 (w % 2) on of dimension w / 2
+            uint32_t y[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+              const uint32_t token = 4u * (w % 2u) + i;
+              const uint32_t word = (at[token] & 4u) != 0u ? x[j][token][w / 2u * 2u + 1u]
+                                                           : x[j][token][w / 2u * 2u];
+              y[i] = rescaled(code_at(word, at[token] & 3u), ratio[token]);
+            }
+            out[w] = low_bytes(y[0], y[1], y[2], y[3]);
+          }
+          *reinterpret_cast<words_t*>(to + (size_t)run * (8u * D) +
+                                      (j * 64u + lane) * (8u * kDims)) = out;
+        }
+      }
     }
   }
 }
@@ -216,9 +379,15 @@ hipError_t launch_select_keys(const SelectKeysArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_gather_pages(const GatherPagesArgs& a, hipStream_t stream) {
-  const uint64_t items = (uint64_t)a.sequences * a.cache.kv_heads * a.target_width;
-  const uint32_t blocks = (uint32_t)std::min<uint64_t>(items, uint64_t{1} << 20);
-  gather_pages_kernel<<<dim3(blocks), kGatherThreads, 0, stream>>>(a, items);
+  const uint64_t items = 2u * (uint64_t)a.sequences * a.cache.kv_heads * a.target_width;
+  const dim3 blocks((uint32_t)std::min<uint64_t>(items, uint64_t{1} << 20));
+  if (a.cache.head_dim == 256u) {
+    gather_pages_kernel<256><<<blocks, kGatherThreads, 0, stream>>>(a, items);
+  } else if (a.cache.head_dim == 128u) {
+    gather_pages_kernel<128><<<blocks, kGatherThreads, 0, stream>>>(a, items);
+  } else {
+    gather_pages_kernel<64><<<blocks, kGatherThreads, 0, stream>>>(a, items);
+  }
   return hipGetLastError();
 }
 
