@@ -934,8 +934,9 @@ KRAKEN_API int kraken_hip_key_weights_f16q_paged_q8_kv(
  * [sequences] receives k; entries from k on stay as they were.  A sequence longer than
  * max_keys, or with k above kept_stride, is left out: neither output of it is written.
  * lengths and keep are uint32 [sequences] in device memory, key_weights f32
- * [sequences][kv_heads][weight_stride] with weight_stride >= max_keys.  Up to 1048576
- * pairs of a sequence and a KV head, and 2^31 - 1 positions. */
+ * [sequences][kv_heads][weight_stride] with weight_stride >= max_keys.  Outputs overlap no
+ * input and not each other.  Up to 1048576 pairs of a sequence and a KV head, and 2^31 - 1
+ * positions. */
 KRAKEN_API int kraken_hip_select_keys_f32_i32(
   kraken_hip_context* context, kraken_buffer key_weights, size_t weight_stride,
   kraken_buffer lengths, kraken_buffer keep, size_t sequences, size_t kv_heads,
@@ -982,7 +983,8 @@ KRAKEN_API int kraken_hip_gather_kv_pages_q8(
  * count as no token (-inf; they stand last, behind -inf, by index, and are never among
  * the top), equal +inf logits share the whole weight, and a row without a logit above -inf
  * has entropy 0 and -inf throughout.  Sums leave the largest logit out, so that values
- * near zero keep f32's relative accuracy.  Up to 65535 rows of up to 4194304 logits.
+ * near zero keep f32's relative accuracy.  Outputs overlap no input and not each other.
+ * Up to 65535 rows of up to 4194304 logits.
  * Uses context workspace. */
 KRAKEN_API int kraken_hip_token_logprobs_f32(
   kraken_hip_context* context, kraken_buffer logits, size_t rows, size_t size,

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "context_internal.hpp"
@@ -239,10 +240,31 @@ int key_weights_entry(kraken_hip_context* ctx, const kraken_buffer& query,
   return finish(ctx, launch_key_weights(a, ctx->cu_count, ctx->workspace, ctx->stream), w);
 }
 
-// Whether two buffers share bytes.
-bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return x < y + b_bytes && y < x + a_bytes;
+struct Bytes {
+  const void* data;
+  size_t count;
+};
+
+bool overlap(const Bytes& a, const Bytes& b) {
+  const uintptr_t x = (uintptr_t)a.data, y = (uintptr_t)b.data;
+  return x != 0 && y != 0 && x < y + b.count && y < x + a.count;
+}
+
+// Whether an output shares bytes with an input or with another output.
+bool any_overlap(std::initializer_list<Bytes> outputs, std::initializer_list<Bytes> inputs) {
+  for (const Bytes* o = outputs.begin(); o != outputs.end(); ++o) {
+    for (const Bytes& i : inputs) {
+      if (overlap(*o, i)) {
+        return true;
+      }
+    }
+    for (const Bytes* other = outputs.begin(); other != o; ++other) {
+      if (overlap(*o, *other)) {
+        return true;
+      }
+    }
+  }
+  return false;
 }
 
 }  // namespace
@@ -482,6 +504,12 @@ KRAKEN_API int kraken_hip_select_keys_f32_i32(
   KRAKEN_TRY(validate_buffer(keep, sequences, sizeof(uint32_t), w, " keep"));
   KRAKEN_TRY(validate_buffer(kept_output, places, sizeof(int32_t), w, " output"));
   KRAKEN_TRY(validate_buffer(kept_lengths, sequences, sizeof(uint32_t), w, " output lengths"));
+  const size_t ids = sequences * sizeof(uint32_t);
+  if (any_overlap({{kept_output.data, places * sizeof(int32_t)}, {kept_lengths.data, ids}},
+                  {{key_weights.data, values * sizeof(float)}, {lengths.data, ids},
+                   {keep.data, ids}})) {
+    return refuse(w, " outputs must not overlap an input or each other");
+  }
   SelectKeysArgs a{};
   a.weights = static_cast<const float*>(key_weights.data);
   a.lengths = static_cast<const uint32_t*>(lengths.data);
@@ -541,9 +569,13 @@ KRAKEN_API int kraken_hip_gather_kv_pages_q8(
     }
     KRAKEN_TRY(validate_f32(key_weights, values, w, " weights"));
     KRAKEN_TRY(validate_f32(weights_output, values, w, " weights output"));
-    if (overlap(key_weights.data, values * sizeof(float), weights_output.data,
-                values * sizeof(float))) {
-      return refuse(w, " weights output must not overlap the weights");
+    if (any_overlap({{weights_output.data, values * sizeof(float)}},
+                    {{key_weights.data, values * sizeof(float)},
+                     {kept.data, places * sizeof(int32_t)},
+                     {kept_lengths.data, sequences * sizeof(uint32_t)},
+                     {page_table.data, sources * sizeof(int32_t)},
+                     {target_table.data, targets * sizeof(int32_t)}})) {
+      return refuse(w, " weights output must not overlap an input");
     }
   }
   a.table = static_cast<const int32_t*>(page_table.data);
@@ -611,6 +643,16 @@ KRAKEN_API int kraken_hip_token_logprobs_f32(
     if (o.buffer.data != nullptr) {
       KRAKEN_TRY(validate_buffer(o.buffer, o.values, 4u, w, o.name));
     }
+  }
+  const size_t row_bytes = rows * sizeof(float);
+  if (any_overlap({{logprob_output.data, row_bytes},
+                   {rank_output.data, row_bytes},
+                   {entropy_output.data, row_bytes},
+                   {top_token_output.data, row_bytes * top},
+                   {top_logprob_output.data, row_bytes * top}},
+                  {{logits.data, values * sizeof(float)}, {temperature.data, row_bytes},
+                   {tokens.data, row_bytes}})) {
+    return refuse(w, " outputs must not overlap an input or each other");
   }
   LogprobsArgs a{};
   a.logits = static_cast<const float*>(logits.data);

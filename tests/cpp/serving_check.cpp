@@ -50,8 +50,12 @@ struct Buffers {
   }
 };
 
+// Addresses that nothing reads, each buffer its own.
 HipBuffer fake(std::size_t bytes) {
-  return HipBuffer::borrow(reinterpret_cast<void*>(std::uintptr_t{4096}), bytes);
+  static std::uintptr_t next = 4096;
+  const std::uintptr_t at = next;
+  next += (bytes + 4095) / 4096 * 4096;
+  return HipBuffer::borrow(reinterpret_cast<void*>(at), bytes);
 }
 
 int run_cpu() {

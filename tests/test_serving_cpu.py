@@ -41,8 +41,8 @@ def weigh(f16=False, window=0, decay=1.0, stride=128, cache=None, batch=None, he
 
 def select(**over):
     a = dict(weights=fake(4 * 3 * 2 * 90), weight_stride=90, lengths=fake(12), keep=fake(12),
-             sequences=3, kv_heads=2, max_keys=80, first=4, last=5, kept=fake(4 * 3 * 2 * 40),
-             kept_stride=40, kept_lengths=fake(12))
+             sequences=3, kv_heads=2, max_keys=80, first=4, last=5, kept=fake(4 * 3 * 2 * 40, 0x100000),
+             kept_stride=40, kept_lengths=fake(12, 0x200000))
     a.update(over)
     return list(a.values())
 
@@ -57,8 +57,9 @@ def gather(**over):
 
 def score(**over):
     a = dict(logits=fake(4 * 25), rows=3, size=5, stride=10, temperature=fake(12),
-             tokens=fake(12), top=4, logprob=fake(12), rank=fake(12), entropy=fake(12),
-             top_tokens=fake(48), top_logprobs=fake(48))
+             tokens=fake(12), top=4, logprob=fake(12, 0x100000), rank=fake(12, 0x200000),
+             entropy=fake(12, 0x300000), top_tokens=fake(48, 0x400000),
+             top_logprobs=fake(48, 0x500000))
     a.update(over)
     return list(a.values())
 
@@ -157,6 +158,10 @@ def test_key_weight_refusals(vctx, kw, fragment, f16):
     (dict(keep=NO), "keep buffer is not initialized"),
     (dict(kept=fake(4 * 3 * 2 * 40 - 4)), "output buffer is too small"),
     (dict(kept_lengths=fake(8)), "output lengths buffer is too small"),
+    (dict(kept_lengths=fake(12)), "must not overlap"),  # the lengths in place
+    (dict(keep=fake(12, 0x200008)), "must not overlap"),
+    (dict(kept=fake(4 * 3 * 2 * 40, 0x1000 + 4 * 3 * 2 * 90 - 4)), "must not overlap"),
+    (dict(kept=fake(4 * 3 * 2 * 40, 0x200000 - 4 * 3 * 2 * 40 + 4)), "must not overlap"),
 ])
 def test_select_refusals(vctx, kw, fragment):
     refused(vctx, "select_keys_f32_i32", select(**kw), fragment)
@@ -182,6 +187,8 @@ def test_select_refusals(vctx, kw, fragment):
     (dict(output=fake(64, 0x100000)), "weights output buffer is too small"),
     (dict(output=fake(4 * 3 * 2 * 90)), "must not overlap"),
     (dict(output=fake(4 * 3 * 2 * 90, 0x1000 + 4 * 3 * 2 * 90 - 4)), "must not overlap"),
+    (dict(kept=fake(4 * 3 * 2 * 40, 0x100000)), "must not overlap"),
+    (dict(target=fake(12, 0x100000 + 4 * 3 * 2 * 90 - 4)), "must not overlap"),
 ])
 def test_gather_refusals(vctx, kw, fragment):
     refused(vctx, "gather_kv_pages_q8", gather(**kw), fragment)
@@ -208,7 +215,12 @@ def test_gather_refusals(vctx, kw, fragment):
     (dict(rank=fake(8)), "rank output buffer is too small"),
     (dict(entropy=fake(8)), "entropy output buffer is too small"),
     (dict(top_tokens=fake(44)), "top token output buffer is too small"),
-    (dict(top_logprobs=fake(44)), "top logprob output buffer is too small"),
+    (dict(top_logprobs=fake(44, 0x500000)), "top logprob output buffer is too small"),
+    (dict(rank=fake(12)), "must not overlap"),  # the tokens in place
+    (dict(entropy=fake(12, 0x1000 + 4 * 25 - 4)), "must not overlap"),
+    (dict(temperature=fake(12, 0x100008)), "must not overlap"),
+    (dict(rank=fake(12, 0x400000 + 44)), "must not overlap"),
+    (dict(top_logprobs=fake(48, 0x400000)), "must not overlap"),
 ])
 def test_logprob_refusals(vctx, kw, fragment):
     refused(vctx, "token_logprobs_f32", score(**kw), fragment)
