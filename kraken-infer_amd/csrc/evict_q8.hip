@@ -170,10 +170,10 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
   });
 }
 
-// One workgroup a sequence and KV head.  Not bytes but the three counts and their barriers are
+// One workgroup a sequence and KV head; kAny: with more keys than it can hold, too.  Not bytes but the three counts and their barriers are
 // what it spends its time on: 512 keys of one pair take 9.5 us, 4096 11.7, 32768 26.3; 64
 // sequences of 32768, two heads each, 26.5.
-template <uint32_t kThreads, uint32_t kCopies>
+template <uint32_t kThreads, uint32_t kCopies, bool kAny>
 __global__ __launch_bounds__(kThreads) void select_keys_kernel(SelectKeysArgs a) {
   __shared__ SelectScratch<kThreads, kCopies> s;
   const uint32_t pair = blockIdx.x, sequence = pair / a.kv_heads, tid = threadIdx.x;
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void select_keys_kernel(SelectKeysArgs a)
   if (most == 0) {
     return;
   }
-  if (end - first <= kHeld * kThreads) {
+  if (!kAny || end - first <= kHeld * kThreads) {
     select_between<kThreads, kCopies, true>(weights, end - first, most, first, kept + first, s);
   } else {
     select_between<kThreads, kCopies, false>(weights, end - first, most, first, kept + first, s);
@@ -395,9 +395,9 @@ hipError_t launch_select_keys(const SelectKeysArgs& a, hipStream_t stream) {
   // By the keys that the threads can hold: barriers and scans of half the waves are sooner done
   // (one pair: 4096 keys 11.7 us and 14.4, 16384 18.7 and 19.9).
   if (a.max_keys <= kHeld * 512u) {
-    select_keys_kernel<512, 2><<<pairs, 512, 0, stream>>>(a);
+    select_keys_kernel<512, 2, false><<<pairs, 512, 0, stream>>>(a);
   } else {
-    select_keys_kernel<1024, 4><<<pairs, 1024, 0, stream>>>(a);
+    select_keys_kernel<1024, 4, true><<<pairs, 1024, 0, stream>>>(a);
   }
   return hipGetLastError();
 }

@@ -76,7 +76,7 @@ __device__ __forceinline__ uint64_t quad_max(uint64_t x) {
 }
 
 constexpr uint32_t kGroups = kThreads / 4u;
-constexpr uint32_t kCandidates = 2048;
+constexpr uint32_t kCandidates = kMaxTopLogprobs * 4u * kPer;  // all that a chunk can have
 
 struct TopScratch {
   uint64_t groups[kGroups], candidates[kCandidates], s[kWaves];
@@ -103,16 +103,18 @@ __device__ __forceinline__ void list_by_rounds(uint64_t* list, uint32_t top, uin
 
 // The `top` first of the workgroup's places (all distinct) in order as list[0..top); 0 where
 // none is left.  `mine`: the first of the thread's, 0 for none; from(bound, take) hands the
-// thread's of at least `bound` to take; best(bound) is its first below `bound`.
+// thread's of at least `bound` to take; best(bound), for where there can be more candidates
+// than LDS holds, is its first below `bound`.
 //
 // The first places of 64 groups of threads are ranked: `top` of them, and so `top` places,
 // reach the one of rank top - 1, so that no place below it counts, and those that reach it lie
-// in `top` groups.  They are few as a rule (20 of 64 groups: 24 places, if groups are alike),
-// and ranked among themselves.  (64 rows of 32000, 20 places: 13.1 us, and 32.2 by 20 rounds of
-// the largest that is left in a workgroup, which stays for more candidates than threads.)
-template <class From, class Best>
+// in `top` groups: of a chunk no more than kCandidates.  They are few as a rule (20 of 64
+// groups: 24 places, if groups are alike), and ranked among themselves.  (64 rows of 32000, 20
+// places: 13.1 us, and 32.2 by 20 rounds of the largest that is left in a workgroup, which
+// stays for more candidates than threads.)
+template <class From, class... Best>
 __device__ __forceinline__ void list_top(uint64_t* list, uint32_t top, uint64_t mine,
-                                         TopScratch& s, From from, Best best) {
+                                         TopScratch& s, From from, Best... best) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint64_t first = quad_max<0x4e>(quad_max<0xb1>(mine));
   __syncthreads();
@@ -166,7 +168,7 @@ __device__ __forceinline__ void list_top(uint64_t* list, uint32_t top, uint64_t 
     if (tid >= count && tid < top) {
       list[tid] = 0;
     }
-  } else if (count <= kCandidates) {
+  } else if (sizeof...(best) == 0 || count <= kCandidates) {
     list_by_rounds(list, top, s.s, [&](uint64_t below) {
       uint64_t found = 0;
       for (uint32_t i = tid; i < count; i += kThreads) {
@@ -176,7 +178,7 @@ __device__ __forceinline__ void list_top(uint64_t* list, uint32_t top, uint64_t 
       return found;
     });
   } else {
-    list_by_rounds(list, top, s.s, best);
+    (list_by_rounds(list, top, s.s, best), ...);
   }
 }
 
@@ -306,15 +308,6 @@ __global__ __launch_bounds__(kThreads) void logprob_chunk_kernel(LogprobsArgs a,
             }
           }
         }
-      },
-      [&](uint64_t bound) {
-        uint64_t best = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) {
-          const uint64_t at = place_of(begin + i * kThreads + tid, x[i]);
-          best = x[i] == x[i] && at < bound && at > best ? at : best;
-        }
-        return best;
       });
   }
 }

@@ -206,3 +206,71 @@ def test_gather_beyond_32_bits(hip_ctx):
                                hip_ctx.buffer(np.array([[65999]], np.int32)), 1, None, 0, None)
     assert torch.equal(keys[65999], keys[65990]) and torch.equal(values[65999], values[65990])
     assert not bool(keys[:65990].any()) and not bool(keys[65991:65999].any())
+
+
+@pytest.mark.parametrize("max_keys", [16384, 16385, 32768, 32769, 40000])
+def test_select_around_what_threads_hold(hip_ctx, max_keys):
+    """Lengths at and about the bounds between the forms, and a bound far above the length."""
+    rng = np.random.default_rng(max_keys)
+    weights = heavy(rng, 4, 1, 40000)
+    check_select(hip_ctx, weights, [min(max_keys, 40000), 16384, 5000, 1], [4096, 2000, 5000, 1], 2,
+                 8, max_keys=max_keys)
+
+
+@pytest.mark.parametrize("page_tokens", [16, 64])
+def test_captured_eviction_replays(hip_ctx, page_tokens):
+    """Replays bring other weights, lengths, tables and positions; each equals the eager calls."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(page_tokens)
+    n, kv, d, most, stride = 3, 2, 128, 500, 520
+    width = -(-most // page_tokens)
+    pages = 2 * n * width
+    stream = torch.cuda.Stream()
+    ctx = kh.Context()
+    ctx.set_stream(stream.cuda_stream)
+    names = {"keys": ((pages, kv, page_tokens, d), torch.int8),
+             "values": ((pages, kv, page_tokens // 8, d, 8), torch.int8),
+             "ks": ((pages, kv), torch.float32), "vs": ((pages, kv), torch.float32),
+             "table": ((n, width), torch.int32), "target": ((n, width), torch.int32),
+             "lengths": ((n,), torch.int32), "keep": ((n,), torch.int32),
+             "w": ((n, kv, stride), torch.float32), "out": ((n, kv, stride), torch.float32),
+             "kept": ((n, kv, most), torch.int32), "counts": ((n,), torch.int32)}
+    sides = [{name: torch.zeros(*shape, dtype=kind, device="cuda")
+              for name, (shape, kind) in names.items()} for _ in range(2)]
+
+    def call(t):
+        ctx.select_keys_f32_i32(t["w"], stride, t["lengths"], t["keep"], n, kv, most, 2, 9, t["kept"],
+                                most, t["counts"])
+        b = [kh.as_buffer(t[name]) for name in ("keys", "values", "ks", "vs")]
+        ctx.gather_kv_pages_q8(kh.PagedQ8Cache(*b, pages, page_tokens, kv, d), t["table"], width,
+                               t["kept"], t["counts"], most, n, t["target"], width, t["w"], stride,
+                               t["out"])
+
+    torch.cuda.synchronize()
+    ctx.begin_graph()
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(sides[0])
+        for lengths, keep in (([500, 40, 0], [100, 40, 5]), ([1, 499, 300], [7, 0, 299]),
+                              ([500, 500, 500], [500, 1, 250]), ([501, 64, 65], [9, 64, 1])):
+            table, target = rng.permutation(pages).reshape(2, n, width)
+            arrays = {"keys": rng.integers(-127, 128, names["keys"][0]),
+                      "values": rng.integers(-127, 128, names["values"][0]),
+                      "ks": 0.1 + rng.random((pages, kv)), "vs": 0.1 + rng.random((pages, kv)),
+                      "table": table, "target": target, "lengths": np.array(lengths),
+                      "keep": np.array(keep), "w": heavy(rng, n, kv, stride)}
+            for t in sides:
+                for name, x in arrays.items():
+                    t[name].copy_(torch.from_numpy(x))
+                for name in ("kept", "counts", "out"):
+                    t[name].fill_(-7)
+            graph.replay()
+            call(sides[1])
+            stream.synchronize()
+            for name in names:
+                assert torch.equal(sides[0][name], sides[1][name]), name
+            want = so.select_keys(arrays["w"], lengths, keep, most, 2, 9, most)
+            np.testing.assert_array_equal(sides[0]["kept"].cpu().numpy(), want[0])
+    ctx.commit_graph()
+    ctx.close()

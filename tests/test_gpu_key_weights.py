@@ -272,3 +272,45 @@ def test_two_steps_add_up(hip_ctx):
         have = run(hip_ctx, cache, one, 4, query[i:i + 1], have, 0, 1.0)
     np.testing.assert_allclose(have, both, rtol=2e-6, atol=1e-12)
     assert math.isclose(float(both.sum()), 2 * 4, rel_tol=1e-5)
+
+
+@pytest.mark.parametrize("window", [0, 150])
+def test_groups_of_rows(hip_ctx, window):
+    """Bounds of a million keys: statistics of rows in groups (127 tokens here), which a
+    sequence's rows lie across, its earlier weight decayed once."""
+    rng = np.random.default_rng(19)
+    batch = Batch(rng, 64, [200, 1, 30, 0, 70], [100, 300, 0, 40, 90], gap=3)
+    cache = po.Pages(rng, batch.pages, 64, 1, 64)
+    stride = 1 << 20
+    table = np.full((5, stride // 64), -1, np.int32)
+    table[:, :batch.width] = batch.table
+    batch.table, batch.width, batch.max_keys = table, stride // 64, 1 << 30
+    query = rng.standard_normal((batch.tokens, 64, 64)).astype(np.float32)
+    old = np.zeros((5, 1, stride), np.float32)
+    old[..., :400] = rng.random((5, 1, 400))
+    got = run(hip_ctx, cache, batch, 64, query, old, window, 0.8)
+    want, tol = so.key_weights(cache, query, batch.plain(), 64, window, 0.8, old, stride)
+    untouched = tol == 0
+    assert np.array_equal(got[untouched], old[untouched])
+    off = np.abs(got - want)[~untouched] / tol[~untouched]
+    assert (off <= 1).all(), off.max()
+
+
+def test_bounds_too_loose_to_keep_scores(hip_ctx):
+    """Single tokens whose scores would take more than 1 GiB, as far as the bounds say."""
+    rng = np.random.default_rng(20)
+    batch = Batch(rng, 64, [1, 1, 2, 1], [100, 300, 7, 0])
+    cache = po.Pages(rng, batch.pages, 64, 4, 64)
+    stride = 1 << 21
+    table = np.full((4, stride // 64), -1, np.int32)
+    table[:, :batch.width] = batch.table
+    batch.table, batch.width, batch.max_keys = table, stride // 64, 1 << 30
+    query = rng.standard_normal((batch.tokens, 64, 64)).astype(np.float32)
+    old = np.zeros((4, 4, stride), np.float32)
+    old[..., :400] = rng.random((4, 4, 400))
+    got = run(hip_ctx, cache, batch, 64, query, old, 0, 0.8)
+    want, tol = so.key_weights(cache, query, batch.plain(), 64, 0, 0.8, old, stride)
+    untouched = tol == 0
+    assert np.array_equal(got[untouched], old[untouched])
+    off = np.abs(got - want)[~untouched] / tol[~untouched]
+    assert (off <= 1).all(), off.max()

@@ -198,3 +198,47 @@ def test_the_same_bits_in_any_batch_and_replay(hip_ctx):
                 assert torch.equal(a, b)
     ctx.commit_graph()
     ctx.close()
+
+
+@pytest.mark.parametrize("size,places,chunks", [
+    (4096, 124, 1), (4096, 128, 1), (9000, 124, 2), (40000, 128, 9), (200000, 128, 45),
+    (700000, 128, 170)])
+def test_top_places_that_crowd(hip_ctx, size, places, chunks):
+    """The largest logits in the same places of every 256 of a chunk of 4096: more candidates
+    than threads, in a chunk and over all chunks, and a list that rises from chunk to chunk."""
+    rng = np.random.default_rng(size + places)
+    rows = rng.standard_normal((3, size))
+    at = np.arange(size)
+    crowd = at % 256 < places
+    rows[0, crowd] += 100.0
+    # 28 in half of the chunks, by eights.
+    rows[1, (at // 4096 % 8 < 4) & (at % 4096 < 28)] += 100.0
+    rows[2] = at * 1e-4
+    assert -(-size // 4096) >= chunks
+    for top in (32, 20, 1):
+        check(hip_ctx, rows, rng.integers(0, size, 3), top)
+
+
+def test_single_outputs(hip_ctx):
+    """Each output alone is what it is among all."""
+    rng = np.random.default_rng(9)
+    rows, size, top = 5, 9001, 7
+    logits = hip_ctx.buffer((3 * rng.standard_normal((rows, size))).astype(np.float32))
+    tokens = hip_ctx.buffer(rng.integers(0, size, rows).astype(np.int32))
+
+    def outs():
+        return [hip_ctx.buffer(np.full(rows * n, -7, k)) for n, k in
+                ((1, np.float32), (1, np.int32), (1, np.float32), (top, np.int32), (top, np.float32))]
+
+    def call(bufs):
+        hip_ctx.token_logprobs_f32(logits, rows, size, size, None,
+                                   tokens if bufs[0] or bufs[1] else None,
+                                   top if bufs[3] or bufs[4] else 0, *bufs)
+
+    everything = outs()
+    call(everything)
+    for i in range(5):
+        one = [b if j == i else None for j, b in enumerate(outs())]
+        call(one)
+        np.testing.assert_array_equal(one[i].download(dtype=np.int32),
+                                      everything[i].download(dtype=np.int32))
