@@ -39,8 +39,8 @@ struct FewPlan {
 __device__ __forceinline__ bool takes_few(uint32_t rows) { return rows != 0 && rows <= kFewRows; }
 
 // (Whole numbers, the query as 31 bits in four columns of 8-bit products, spare the codes'
-// way to f16, and took as long: 64 sequences of up to 32768 keys, four rows, 138 us both.  The
-// call without its stores takes 111, the keys alone 97: the 34 MB of scores cost 27.)
+// way to f16, and took as long: 64 sequences of up to 32768 keys, four rows, 138 us both.
+// Without its stores the call would take 111: the 34 MB of scores cost 27.)
 template <int D, class T, bool kStacked>
 __global__ __launch_bounds__(kThreads, D == 256 && !kStacked ? 2 : 3) void few_scores_kernel(
   KeyWeightsArgs a, FewPlan p) {
