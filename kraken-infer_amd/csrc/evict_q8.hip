@@ -42,10 +42,17 @@ __device__ __forceinline__ uint32_t waves_before(uint32_t x, uint32_t& all, uint
   return before;
 }
 
-// kCopies: of the counts, by lane, so that lanes of one digit do not wait for each other.
+// How many lanes before this one are in the mask.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+}
+
+// Counts of each digit.  kCopies: of the first's, by lane, so that lanes of one digit do not
+// wait for each other; keys that have the digits before are few.
 template <uint32_t kThreads, uint32_t kCopies>
 struct SelectScratch {
-  uint32_t bins[kCopies][kBins];
+  uint32_t bins[kCopies + 2u][kBins];
   uint32_t waves[kThreads / 64u];
   uint32_t digit, above;
 };
@@ -61,19 +68,23 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t times = (count + kThreads - 1u) / kThreads;  // of a wave
   const uint32_t begin = wave * times * 64u + lane;
+  for (uint32_t i = tid; i < (kCopies + 2u) * kBins; i += kThreads) {
+    s.bins[0][i] = 0;
+  }
   uint32_t held[kInRegisters ? kHeld : 1];
   if constexpr (kInRegisters) {
     float x[kHeld];
 #pragma unroll
     for (uint32_t j = 0; j < kHeld; ++j) {
-      x[j] = j < times && begin + j * 64u < count ? weights[begin + j * 64u] : 0.0f;
+      x[j] = j < times && begin + j * 64u < count ? weights[begin + j * 64u] : NAN;
     }
 #pragma unroll
     for (uint32_t j = 0; j < kHeld; ++j) {
       held[j] = key_of(x[j]);
     }
   }
-  // f(key, time) for this lane's; it has to ask whether the place is one.
+  // f(key, time) for this lane's; it has to ask whether the place is one.  (Of held keys, those
+  // that are none are 0 and larger than nothing.)
   auto each = [&](auto f) {
     if constexpr (kInRegisters) {
 #pragma unroll
@@ -101,15 +112,10 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
   };
   // The least key that is kept; `want` of those equal to it are.
   uint32_t least = 0, known = 0, want = most;  // known: bits of `least` that are settled
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const uint32_t shift = pass == 0 ? 21u : pass == 1 ? 10u : 0u;
-    const uint32_t mask = pass == 2 ? 1023u : kBins - 1u;
-    for (uint32_t i = tid; i < kCopies * kBins; i += kThreads) {
-      s.bins[0][i] = 0;
-    }
+  auto settle = [&](auto copies, uint32_t* counts, uint32_t shift, uint32_t mask) {
+    constexpr uint32_t kOf = decltype(copies)::value;
+    uint32_t* bins = counts + lane % kOf * kBins;
     __syncthreads();
-    uint32_t* bins = s.bins[lane % kCopies];
     each([&](uint32_t key, uint32_t j) {
       if (begin + j * 64u < count && (key & known) == least) {
         atomicAdd(&bins[key >> shift & mask], 1u);
@@ -122,8 +128,8 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
     for (uint32_t i = 0; i < kPer; ++i) {
       mine[i] = 0;
 #pragma unroll
-      for (uint32_t copy = 0; copy < kCopies; ++copy) {
-        mine[i] += s.bins[copy][kBins - 1u - (kPer * tid + i)];
+      for (uint32_t copy = 0; copy < kOf; ++copy) {
+        mine[i] += counts[copy * kBins + kBins - 1u - (kPer * tid + i)];
       }
       sum += mine[i];
     }
@@ -144,35 +150,53 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
     least |= s.digit << shift;
     known |= mask << shift;
     want -= s.above;
-  }
+  };
+  using One = std::integral_constant<uint32_t, 1>;
+  settle(std::integral_constant<uint32_t, kCopies>{}, s.bins[0], 21u, kBins - 1u);
+  settle(One{}, s.bins[kCopies], 10u, kBins - 1u);
+  settle(One{}, s.bins[kCopies + 1u], 0u, 1023u);
   // How many larger and equal ones each wave has, then their places.
   uint32_t larger = 0, equal = 0;
   each([&](uint32_t key, uint32_t j) {
     const bool is = begin + j * 64u < count;
-    larger += (uint32_t)__popcll(__ballot(is && key > least));
-    equal += (uint32_t)__popcll(__ballot(is && key == least));
+    larger += (kInRegisters || is) && key > least ? 1u : 0u;
+    equal += is && key == least ? 1u : 0u;
   });
+  larger = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(larger, Sum{}), 63);
+  equal = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(equal, Sum{}), 63);
   uint32_t all;
   uint32_t ties = waves_before<kWaves>(equal, all, s.waves);
   uint32_t place = waves_before<kWaves>(larger, all, s.waves) + min(ties, want);
-  const uint64_t below = (uint64_t{1} << lane) - 1u;
+  if (equal == 0) {  // uniform, and so for nearly all waves where weights differ
+    each([&](uint32_t key, uint32_t j) {
+      const uint32_t i = begin + j * 64u;
+      const bool keep = (kInRegisters || i < count) && key > least;
+      const uint64_t kept_here = __ballot(keep);
+      if (keep) {
+        kept[place + lanes_below(kept_here)] = (int32_t)(first + i);
+      }
+      place += (uint32_t)__popcll(kept_here);
+    });
+    return;
+  }
   each([&](uint32_t key, uint32_t j) {
     const uint32_t i = begin + j * 64u;
     const uint64_t same = __ballot(i < count && key == least);
     const bool keep =
-      i < count && (key > least || (key == least && ties + (uint32_t)__popcll(same & below) < want));
+      i < count && (key > least || (key == least && ties + lanes_below(same) < want));
     const uint64_t kept_here = __ballot(keep);
     if (keep) {
-      kept[place + (uint32_t)__popcll(kept_here & below)] = (int32_t)(first + i);
+      kept[place + lanes_below(kept_here)] = (int32_t)(first + i);
     }
     ties += (uint32_t)__popcll(same);
     place += (uint32_t)__popcll(kept_here);
   });
 }
 
-// One workgroup a sequence and KV head; kAny: with more keys than it can hold, too.  Not bytes but the three counts and their barriers are
-// what it spends its time on: 512 keys of one pair take 9.5 us, 4096 11.7, 32768 26.3; 64
-// sequences of 32768, two heads each, 26.5.
+// One workgroup a sequence and KV head; kAny: with more keys than it can hold, too.  Not
+// bytes but the three counts, their barriers and the last pass over the keys are what it spends
+// its time on: 512 keys of one pair take 8.7 us, 4096 10.1, 32768 20.3, 131072 93; 64 sequences
+// of 32768, two heads each, 20.5.
 template <uint32_t kThreads, uint32_t kCopies, bool kAny>
 __global__ __launch_bounds__(kThreads) void select_keys_kernel(SelectKeysArgs a) {
   __shared__ SelectScratch<kThreads, kCopies> s;
@@ -393,7 +417,7 @@ __global__ __launch_bounds__(kGatherThreads) void gather_pages_kernel(GatherPage
 hipError_t launch_select_keys(const SelectKeysArgs& a, hipStream_t stream) {
   const dim3 pairs(a.sequences * a.kv_heads);
   // By the keys that the threads can hold: barriers and scans of half the waves are sooner done
-  // (one pair: 4096 keys 11.7 us and 14.4, 16384 18.7 and 19.9).
+  // (one pair: 512 keys 8.7 us and 11.4, 4096 10.1 and 12.1, 16384 15.6 and 15.7).
   if (a.max_keys <= kHeld * 512u) {
     select_keys_kernel<512, 2, false><<<pairs, 512, 0, stream>>>(a);
   } else {
