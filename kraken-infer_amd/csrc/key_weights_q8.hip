@@ -15,11 +15,11 @@
 // Launches: rows, first pass (maxima and sums by 256 keys), L of each row, second pass,
 // and where it splits the rows over workgroups their sums' sum.
 //
-// 1024 f32 rows of a sequence of 8192 (two KV heads of 256, groups of four): 156 us, traced
-// 66 the first pass, 85 the second, 19 the others.  The products are 129 GFLOP in f16, 98 us
-// at a large product's rate.  Without them the call takes 73, with half of them 107: their
-// time adds to the exponentials' and sums', although a SIMD has two waves.  With f16 queries
-// 105.  32 rows at the end of the same sequence: 28, five launches.
+// 1024 f32 rows of a sequence of 8192 (two KV heads of 256, groups of four): 139 us, traced
+// 65 for each pass, 19 the others.  A pass's products are 64 GFLOP in f16, 49 us at a large
+// product's rate, and their time hides the exponentials and sums (two waves a SIMD; without
+// those the pass takes as long).  With f16 queries 92.  32 rows at the end of the same
+// sequence: 26.5, five launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -296,7 +296,13 @@ __global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs
                     kSums ? p.logs[(size_t)kv_head * padded + row] : 0.0f};
     };
     Values values = values_of(begin_tile);
-    arrived();
+    // The compiler, which does not count the copies, is told that the values have come with
+    // them: a wait for a value behind the next copies would be one for these, too.
+    auto settled = [&]() {
+      arrived();
+      asm volatile("" : "+v"(values.visible), "+v"(values.factor), "+v"(values.log));
+    };
+    settled();
     for (uint32_t tile = begin_tile; tile < stop_tile; ++tile) {
       const uint32_t parity = (tile - begin_tile) & 1u;
       const uint32_t following = min(tile + 1u, stop_tile - 1u);
@@ -336,13 +342,15 @@ __global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs
         for (int b = 0; b < 2 * kSubs; ++b) {
           scaled[b] = factor * scale[b];
         }
-        // Keys that a row does not see add nothing, whatever their scores are.
+        // Keys that a row does not see add nothing, whatever their scores are: those from `left`
+        // on, counted from the lane's first (against which all 32 compare with constants).
+        const int left = (int)(seen - (first_key + 8u * h));
         auto soften = [&](auto masks) {
           constexpr bool kMasked = decltype(masks)::value;
           auto exponent = [&](int sub, int r, float base) {
             const int b = 2 * sub + r / 8;
             const float y = fmaf(score[sub][r], scaled[b], base);
-            return !kMasked || first_key + 16u * b + 8u * h + r % 8 < seen ? y : -INFINITY;
+            return !kMasked || 16 * b + r % 8 < left ? y : -INFINITY;
           };
           if constexpr (!kSums) {
             // (A scale is not negative: the largest score of a run of keys is that of its
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs
               float largest = -INFINITY;
 #pragma unroll
               for (int r = 8 * (b % 2); r < 8 * (b % 2) + 8; ++r) {
-                const bool sees = !kMasked || first_key + 16u * b + 8u * h + r % 8 < seen;
+                const bool sees = !kMasked || 16 * b + r % 8 < left;
                 largest = fmaxf(largest, sees ? score[b / 2][r] : -INFINITY);
               }
               const float y = fmaf(largest, scaled[b], offset[b]);
@@ -388,7 +396,7 @@ __global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs
           joined[parity][wave][n] = make_float2(top, sum);
         }
       }
-      arrived();
+      settled();
       if constexpr (!kSums) {
         // (The other parity's are written meanwhile, these again behind another barrier.)
         if (wave == 0 && h == 0 && own) {
