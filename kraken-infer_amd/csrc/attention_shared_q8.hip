@@ -463,7 +463,7 @@ void launch_join(const PagedAttentionArgs& a, const SharedPrefixArgs& p, const S
                  hipStream_t stream) {
   const uint32_t rows = a.batch.tokens * a.heads;
   // (Up to some seventy parts of a row.  128 rows: the call 53.7 us with four waves, 49.2 with
-  // sixteen; 512 rows 100 and 101; 3072 rows of a few parts 55.8 and 68.)
+  // sixteen; 512 rows 100 and 101; 192 tokens of sixteen heads, a few parts a row, 55.8 and 68.)
   if (rows <= 256u) {
     shared_join_kernel<D, T, 16>
       <<<dim3(rows), 1024, 0, stream>>>(a, s.work, p.groups, s.limits.decode_most);
