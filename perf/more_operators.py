@@ -247,6 +247,13 @@ def prepare(case, seed):
             s["cache"] = kh.PagedQ8Cache(b["keys"], b["values"], b["key_scales"],
                                          b["value_scales"], s["pages"], case["page_tokens"],
                                          case["kv_heads"], case["head_dim"])
+        if case["kind"] == "evict":
+            # A sequence is given the pages that its kept tokens reach into: what others held
+            # would be read back as it was.
+            first = torch.arange(s["target_width"], device="cuda") * case["page_tokens"]
+            has = first < torch.minimum(s["keep"], s["lengths"])[:, None]
+            s["given"] = torch.where(has, s["target"], -1)
+            b["target"] = kh.as_buffer(s["given"])
         if case["kind"] in ("shared", "weights"):
             s["batch"] = kh.PagedBatch(b["table"], b["starts"], b["lengths"], s["sequences"],
                                        s["width"], s["tokens"], s["max_query"], s["max_keys"])
