@@ -274,3 +274,14 @@ def test_captured_eviction_replays(hip_ctx, page_tokens):
             np.testing.assert_array_equal(sides[0]["kept"].cpu().numpy(), want[0])
     ctx.commit_graph()
     ctx.close()
+
+
+def test_gather_leaves_pages_behind_the_kept(hip_ctx):
+    """Target pages that no kept token reaches stay as they were."""
+    rng = np.random.default_rng(11)
+    cache, table, kept, target = scene(rng, 16, 2, 64, [100, 100, 100], [90, 17, 0], spare=20)
+    spare = np.setdiff1d(np.arange(cache.pages), np.concatenate([table.ravel(), target.ravel()]))
+    missing = np.argwhere(target < 0)
+    target[tuple(missing.T)] = spare[:len(missing)]
+    assert len(missing) > 5
+    check_gather(hip_ctx, cache, table, kept, [90, 17, 0], target)
