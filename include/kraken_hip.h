@@ -952,8 +952,8 @@ KRAKEN_API int kraken_hip_select_keys_f32_i32(
  * page.  A source whose scale is not finite makes its target page's scale NaN for that
  * head and keeps its codes.  A position outside the table's pages or a page outside the
  * pool gives zeros; codes behind the last kept token of its page become zeros.  A target
- * page outside the pool, or behind the last kept token's, is not written.  page_table is int32 [sequences][table_width],
- * target_table int32 [sequences][target_width], kept int32
+ * page outside the pool, or behind the last kept token's, is not written.  page_table is
+ * int32 [sequences][table_width], target_table int32 [sequences][target_width], kept int32
  * [sequences][kv_heads][kept_stride], kept_lengths uint32 [sequences]; a sequence whose
  * kept_lengths[b] passes kept_stride or target_width * page_tokens is left out.
  * A target page stands once in target_table and is no source page: shared pages stay as
