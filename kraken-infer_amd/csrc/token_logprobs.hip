@@ -43,7 +43,7 @@ struct Part {
 
 struct LogprobPlan {
   Part* parts;      // [rows][chunks]
-  uint64_t* lists;  // [rows][chunks][top]: falling keys
+  uint64_t* lists;  // [rows][top][chunks]: falling keys of each chunk
   uint32_t chunk, chunks;
 };
 
@@ -101,20 +101,16 @@ __device__ __forceinline__ void list_by_rounds(uint64_t* list, uint32_t top, uin
   }
 }
 
-// The `top` first of the workgroup's places (all distinct) in order as list[0..top); 0 where
-// none is left.  `mine`: the first of the thread's, 0 for none; from(bound, take) hands the
-// thread's of at least `bound` to take; best(bound), for where there can be more candidates
-// than LDS holds, is its first below `bound`.
+// Candidates for the `top` first of the workgroup's places (all distinct), as s.candidates,
+// and their number.  `mine`: the first of the thread's, 0 for none; from(bound, take) hands
+// the thread's of at least `bound` to take.
 //
 // The first places of 64 groups of threads are ranked: `top` of them, and so `top` places,
 // reach the one of rank top - 1, so that no place below it counts, and those that reach it lie
-// in `top` groups: of a chunk no more than kCandidates.  They are few as a rule (20 of 64
-// groups: 24 places, if groups are alike), and ranked among themselves.  (64 rows of 32000, 20
-// places: 13.1 us, and 32.2 by 20 rounds of the largest that is left in a workgroup, which
-// stays for more candidates than threads.)
-template <class From, class... Best>
-__device__ __forceinline__ void list_top(uint64_t* list, uint32_t top, uint64_t mine,
-                                         TopScratch& s, From from, Best... best) {
+// in `top` groups.  They are few where groups are alike (20 of 64 groups: 24 places).
+template <class From>
+__device__ __forceinline__ uint32_t collect(uint32_t top, uint64_t mine, TopScratch& s,
+                                            From from) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint64_t first = quad_max<0x4e>(quad_max<0xb1>(mine));
   __syncthreads();
@@ -154,29 +150,53 @@ __device__ __forceinline__ void list_top(uint64_t* list, uint32_t top, uint64_t 
     });
   }
   __syncthreads();
-  const uint32_t count = s.count;
+  return s.count;
+}
+
+// The `top` first of the workgroup's places in order as list[0], list[stride] ..; 0 where none
+// is left.  best(bound), for where there can be more candidates than LDS holds, is the thread's
+// first below `bound`.
+//
+// More candidates than threads are bounded again, in whatever order they have come: half of
+// the groups have no more than half of them.  (64 rows of 32000, 20 places: 13.1 us, and 32.2
+// by 20 rounds of the largest that is left in a workgroup, which stays for a row's lists that
+// do not fit.)
+template <class From, class... Best>
+__device__ __forceinline__ void list_top(uint64_t* list, size_t stride, uint32_t top,
+                                         uint64_t mine, TopScratch& s, From from, Best... best) {
+  const uint32_t tid = threadIdx.x;
+  uint32_t count = collect(top, mine, s, from);
+  while (count > kThreads && (sizeof...(best) == 0 || count <= kCandidates)) {
+    uint64_t x[kCandidates / kThreads];
+    mine = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kCandidates / kThreads; ++i) {
+      const uint32_t at = i * kThreads + tid;
+      x[i] = at < count ? s.candidates[at] : 0u;
+      mine = x[i] > mine ? x[i] : mine;
+    }
+    count = collect(top, mine, s, [&](uint64_t bound, auto take) {
+#pragma unroll
+      for (uint32_t i = 0; i < kCandidates / kThreads; ++i) {
+        if (x[i] >= bound) {
+          take(x[i]);
+        }
+      }
+    });
+  }
   if (count <= kThreads) {
     const uint64_t place = tid < count ? s.candidates[tid] : 0u;
-    rank = 0;
+    uint32_t rank = 0;
 #pragma unroll 4
     for (uint32_t i = 0; i < count; ++i) {
       rank += s.candidates[i] > place ? 1u : 0u;
     }
     if (tid < count && rank < top) {
-      list[rank] = place;
+      list[rank * stride] = place;
     }
     if (tid >= count && tid < top) {
-      list[tid] = 0;
+      list[tid * stride] = 0;
     }
-  } else if (sizeof...(best) == 0 || count <= kCandidates) {
-    list_by_rounds(list, top, s.s, [&](uint64_t below) {
-      uint64_t found = 0;
-      for (uint32_t i = tid; i < count; i += kThreads) {
-        const uint64_t at = s.candidates[i];
-        found = at < below && at > found ? at : found;
-      }
-      return found;
-    });
   } else {
     (list_by_rounds(list, top, s.s, best), ...);
   }
@@ -295,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void logprob_chunk_kernel(LogprobsArgs a,
       first = x[j] == mine ? place_of(begin + j * kThreads + tid, mine) : first;
     }
     list_top(
-      p.lists + ((size_t)row * p.chunks + chunk) * a.top, a.top, first, s,
+      p.lists + (size_t)row * p.chunks * a.top + chunk, p.chunks, a.top, first, s,
       [&](uint64_t bound, auto take) {
         const uint32_t key = (uint32_t)(bound >> 32);
         const float least = key != 0u ? logit_of(key) : -INFINITY;
@@ -384,7 +404,7 @@ __global__ __launch_bounds__(kThreads) void logprob_row_kernel(LogprobsArgs a, L
       return found;
     };
     list_top(
-      list, a.top, best(~uint64_t{0}), s,
+      list, 1, a.top, best(~uint64_t{0}), s,
       [&](uint64_t bound, auto take) {
         for (uint32_t i = tid; i < places; i += kThreads) {
           const uint64_t at = lists[i];
