@@ -392,10 +392,14 @@ FewPlan plan_of(const KeyWeightsArgs& a, int cu_count, size_t& bytes, void* work
   p.parts = (keys + p.part_keys - 1u) / p.part_keys;
   const double scores = (double)pairs * p.steps * p.rows * 128.0;
   const double stats = (double)pairs * p.parts * p.rows * sizeof(float2);
-  // (A single sequence of more rows is not worth a second pair of launches for where it brings
-  // fewer: 8192 keys, 128 rows 33.9 us with them, 29.8 without.)
-  if (p.group > kFewRows || scores + stats > (double)kMostBytes ||
-      (a.rows.batch.sequences == 1u && rows > kFewRows)) {
+  // Where some sequences have more rows, these launches come on top of theirs, which a single
+  // sequence and few keys are not worth: calls with both, and with all rows as many, of 24
+  // sequences (two KV heads of 256) of up to 1000 keys 44.5 and 32.3 us, 4000 (52 MB of keys)
+  // 60.1 and 46.9, 16000 (201 MB) 112 and 102; eight KV heads of 128: 37.2 and 25.7, 62.1 and
+  // 61.8 (103 MB), 143 and 171; four sequences of 16000 (66 MB) 43.3 and 46.7.
+  const double keys_bytes = (double)pairs * keys * a.rows.cache.head_dim;
+  const bool beside = rows > kFewRows && (a.rows.batch.sequences == 1u || keys_bytes < 64e6);
+  if (p.group > kFewRows || scores + stats > (double)kMostBytes || beside) {
     bytes = 0;
     return p;
   }

@@ -314,3 +314,28 @@ def test_bounds_too_loose_to_keep_scores(hip_ctx):
     assert np.array_equal(got[untouched], old[untouched])
     off = np.abs(got - want)[~untouched] / tol[~untouched]
     assert (off <= 1).all(), off.max()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("d", [64, 256])
+def test_few_and_many_rows_in_one_call(hip_ctx, d, f16):
+    """Bounds of so many keys that sequences of few rows have their own launches beside
+    those of many."""
+    rng = np.random.default_rng(21 + d)
+    batch = Batch(rng, 64, [1, 40, 2, 0, 4, 5, 130], [700, 300, 0, 40, 90, 1000, 5], gap=2)
+    cache = po.Pages(rng, batch.pages, 64, 2, d)
+    stride = 1 << 17
+    table = np.full((7, stride // 64), -1, np.int32)
+    table[:, :batch.width] = batch.table
+    batch.table, batch.width, batch.max_keys = table, stride // 64, 1 << 30
+    assert 7 * 2 * stride * d > 64e6
+    query = rng.standard_normal((batch.tokens, 8, d)).astype(np.float16 if f16 else np.float32)
+    old = np.zeros((7, 2, stride), np.float32)
+    old[..., :1100] = rng.random((7, 2, 1100))
+    for window in (0, 3, 33):
+        got = run(hip_ctx, cache, batch, 8, query, old, window, 0.8)
+        want, tol = so.key_weights(cache, query, batch.plain(), 8, window, 0.8, old, stride)
+        untouched = tol == 0
+        assert np.array_equal(got[untouched], old[untouched])
+        off = np.abs(got - want)[~untouched] / tol[~untouched]
+        assert (off <= 1).all(), (window, off.max())
