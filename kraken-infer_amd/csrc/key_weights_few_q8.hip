@@ -11,9 +11,8 @@
 // 2^(score - log2 of the row's sum) over the rows of each key.
 //
 // 64 sequences of up to 32768 keys, one token of four query heads for each of two KV heads of
-// 256: 138 us for 537 MB of keys, 34 of weights and 34 of scores there and back; traced, 124
-// (keys and scores at 4.6 TB/s) and 15.  One sequence of 4096: 11.6, two launches of some 7
-// and 4 us.
+// 256: 135 us for 537 MB of keys, 34 of weights and 34 of scores there and back, of which the
+// second launch takes 15.  One sequence of 4096: 11.5, two launches of some 7 and 4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -44,8 +43,8 @@ struct FewPlan {
 __device__ __forceinline__ bool takes_few(uint32_t rows) { return rows != 0 && rows <= kFewRows; }
 
 // (Whole numbers, the query as 31 bits in four columns of 8-bit products, spare the codes'
-// way to f16, and took as long: 64 sequences of up to 32768 keys, four rows, 138 us both.
-// Without its stores the call would take 111: the 34 MB of scores cost 27.)
+// way to f16, and took as long.  Without its stores the call of 64 sequences would take some
+// 27 us less, whether they go out step by step or, by way of LDS, at a part's end.)
 template <int D, class T, bool kStacked>
 __global__ __launch_bounds__(kThreads, D == 256 && !kStacked ? 2 : 3) void few_scores_kernel(
   KeyWeightsArgs a, FewPlan p) {
@@ -94,8 +93,11 @@ __global__ __launch_bounds__(kThreads, D == 256 && !kStacked ? 2 : 3) void few_s
   // of four, lie in as many places.  Two steps' keys are on their way at a time.
   auto turn = [](uint32_t r) { return ((r >> 3 & 3u) * 4u + (r & 3u)) & (kChunks - 1u); };
   u32x4_t k[2][2 * kLoads];
-  auto load_k = [&](auto parity, uint32_t i) {  // of the wave's step i
+  // (Past the wave's last step that one's again, which is in the caches.)
+  const uint32_t last = (max(steps, wave + 1u) - 1u - wave) / kWaves;
+  auto load_k = [&](auto parity, uint32_t of) {  // of the wave's step `of`
     constexpr int kBuffer = decltype(parity)::value;
+    const uint32_t i = min(of, last);
     const uint32_t key = first_key(wave + kWaves * i);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -384,10 +386,15 @@ FewPlan plan_of(const KeyWeightsArgs& a, int cu_count, size_t& bytes, void* work
   const uint64_t pairs = (uint64_t)a.rows.batch.sequences * a.rows.cache.kv_heads;
   const uint32_t keys = longest_length(a);
   p.steps = (keys + 31u) / 32u;
-  // Parts as the attention's decode kernel has them.
-  const uint64_t most = 11u * (uint64_t)cu_count;
-  uint64_t per = (pairs * keys + most - 1u) / most;
-  per = std::min<uint64_t>((std::max<uint64_t>(per, 128u) + 127u) / 128u * 128u, 4096u);
+  // Parts for eleven workgroups a CU (64 sequences of up to 32768 keys, two KV heads: 135 us,
+  // with six 140), but of 768 keys where those make six (up to 8192 keys: 40.4 us, 51.6 with
+  // 384), since a wave's way to its first keys is long; 512 at least where those give each CU
+  // one (one sequence of 65536: 16.4 us, 19.3 with 256, 26.8 with 128), else 256 (four of 8192:
+  // 15.0, 18.8 with 128, 16.7 with 512).
+  const uint64_t all = pairs * keys, cus = (uint64_t)cu_count;
+  uint64_t per = std::max(all / (11u * cus), std::min<uint64_t>(all / (6u * cus), 768u));
+  per = std::max<uint64_t>(per, all >= 512u * cus ? 512u : 256u);
+  per = std::min<uint64_t>((per + 127u) / 128u * 128u, 4096u);
   p.part_keys = (uint32_t)per;
   p.parts = (keys + p.part_keys - 1u) / p.part_keys;
   const double scores = (double)pairs * p.steps * p.rows * 128.0;
