@@ -914,9 +914,10 @@ KRAKEN_API int kraken_hip_attention_f16q_shared_paged_q8_kv(
  * for the attention, f32 or f16; the weights keep f32 accuracy in both, by the same
  * limits.  Sums go in one order, so that the same call gives the same bits; loose bounds
  * of the batch change it.  A NaN or an infinity in a query that counts or in the scale of
- * a key that it sees reaches all weights of its sequence and KV head.  decay
- * is finite and not negative.  query is 16-byte aligned; key_weights overlaps no input.
- * Up to 67108864 rows (tokens * heads).  Uses context workspace. */
+ * a key that it sees makes all weights of its sequence and KV head NaN, those of keys that
+ * the row does not see too.  decay is finite and not negative.  query is 16-byte aligned;
+ * key_weights overlaps no input.  Up to 67108864 rows (tokens * heads).  Uses context
+ * workspace. */
 KRAKEN_API int kraken_hip_key_weights_f32_paged_q8_kv(
   kraken_hip_context* context, kraken_buffer query, const kraken_paged_q8_cache* cache,
   const kraken_paged_batch* batch, size_t heads, size_t window, float decay,

@@ -315,6 +315,11 @@ __global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs
         copy(tile + 1u, parity ^ 1u);
       }
       float top = kLowestMax, sum = 0.0f;
+      if constexpr (kSums) {
+        // A row whose sum is NaN spoils all keys, those too that it does not see: its NaN stays
+        // in the sums of the wave's first key, for the end.
+        sums[0][0] = own && log != log ? log : sums[0][0];
+      }
       const bool any = __any(seen > first_key);  // else no row sees the wave's keys
       float16_t score[kSubs];
       // Fragments of the rows kRing ahead of the products that take them.
@@ -415,12 +420,14 @@ __global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs
     if constexpr (kSums) {
       // Over the rows, which are the lanes of each half; lane n keeps register n.
       static_assert(16 * kSubs == 32, "a register for each lane of a half");
-      float mine = 0.0f;
+      const float first = reduce32_sum(sums[0][0]);
+      float mine = first;
 #pragma unroll
-      for (int i = 0; i < 16 * kSubs; ++i) {
+      for (int i = 1; i < 16 * kSubs; ++i) {
         const float all = reduce32_sum(sums[i / 16][i % 16]);
         mine = n == (uint32_t)i ? all : mine;
       }
+      mine = first != first ? first : mine;
       const size_t pair = (size_t)found.index * kv_heads + kv_head;
       const uint32_t key = first_key + 16u * (n / 8u) + 8u * h + n % 8u;
       if (key < s.length) {
