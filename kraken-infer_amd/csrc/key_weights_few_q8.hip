@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kThreads, D == 256 && !kStacked ? 2 : 3) void few_s
     const int32_t page = a.rows.batch.table[(size_t)found.index * a.rows.batch.width +
                                             min(key >> shift, a.rows.batch.width - 1u)];
     pages = page >= 0 && (uint32_t)page < a.rows.cache.pages ? page : -1;
-    scales = a.rows.cache.key_scales[(size_t)max(pages, 0) * kv_heads + kv_head];
+    scales = finite_or_nan(a.rows.cache.key_scales[(size_t)max(pages, 0) * kv_heads + kv_head]);
   }
   // A load of the wave is 1024 bytes of keys as they lie, 64 / kChunks rows; through LDS, a
   // region for each wave, they get to the lanes whose operands they are.  Chunk c of key row
@@ -169,8 +169,9 @@ __global__ __launch_bounds__(kThreads, D == 256 && !kStacked ? 2 : 3) void few_s
     }
     largest = xor32_max(xor16_max(largest));
     const int e = query_exponent(largest);
-    // 1 / sqrt(D) in log2 units, over the row's power of two.
+    // 1 / sqrt(D) in log2 units, over the row's power of two; NaN for a row with an infinity.
     row_factor = ldexpf(kLog2e / (D == 64 ? 8.0f : D == 256 ? 16.0f : 11.313708498984761f), -e);
+    row_factor = largest < INFINITY ? row_factor : NAN;
 #pragma unroll
     for (int c = 0; c < kLoads; ++c) {
 #pragma unroll

@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 
 #include "attention_paged_q8_common.hpp"
@@ -25,6 +26,9 @@ __device__ __forceinline__ float decayed_weight(const KeyWeightsArgs& a, const f
                                                 bool had) {
   return a.decay > 0.0f && had ? a.decay * *at : 0.0f;
 }
+
+// A key's scale, NaN if it is infinite: the scores that it made -inf would vanish.
+__device__ __forceinline__ float finite_or_nan(float x) { return fabsf(x) < INFINITY ? x : NAN; }
 
 // What a length cannot pass.
 inline uint32_t longest_length(const KeyWeightsArgs& a) {

@@ -165,8 +165,10 @@ __global__ __launch_bounds__(kThreads) void weight_rows_kernel(KeyWeightsArgs a,
   const int e = query_exponent(most);
   const size_t place = ((size_t)kv_head * p.tiles + tile) * kTile + n;
   if (j == 0) {
-    p.factors[place] =
+    // (NaN for a row with an infinity.)
+    const float factor =
       ldexpf(kLog2e / (D == 64 ? 8.0f : D == 256 ? 16.0f : 11.313708498984761f), -e);
+    p.factors[place] = most < INFINITY ? factor : NAN;
     if (kv_head == 0) {
       p.visible[tile * kTile + n] = visible;
     }
@@ -271,8 +273,9 @@ __global__ __launch_bounds__(kThreads, 2) void weight_pass_kernel(KeyWeightsArgs
     float scale[2 * kSubs], offset[2 * kSubs];
     {
       const int32_t page = page_of(first_key + 16u * (lane & 3u));
-      const float held = inside(page) ? a.rows.cache.key_scales[(size_t)page * kv_heads + kv_head]
-                                      : 0.0f;
+      const float held =
+        inside(page) ? finite_or_nan(a.rows.cache.key_scales[(size_t)page * kv_heads + kv_head])
+                     : 0.0f;
       const float out = inside(page) ? 0.0f : -INFINITY;
 #pragma unroll
       for (int b = 0; b < 2 * kSubs; ++b) {

@@ -1,4 +1,4 @@
-"""What a NaN in a query or in a key's scale does to the weight that cached keys
+"""What a NaN or an infinity in a query or in a key's scale does to the weight that cached keys
 receive: all weights of its sequence and KV head become NaN, whichever form of the kernels the
 batch's rows and bounds choose, and no others change by a bit."""
 import numpy as np
@@ -10,7 +10,7 @@ from test_gpu_paged_q8 import Batch
 
 pytestmark = pytest.mark.gpu
 
-SPOILS = [np.nan]
+SPOILS = [np.nan, np.inf, -np.inf]
 # (new tokens, tokens before, query heads of a KV head, window, bound of keys or none).
 FORMS = {
     "single tokens": ([1, 1, 2], [300, 33, 700], 2, 0, None),
@@ -24,7 +24,8 @@ FORMS = {
 
 
 def scene(form, f16, signed):
-    """`signed`: queries above zero and keys below, so that each product is negative."""
+    """`signed`: queries above zero and keys below, so that each product is negative: an
+    infinite factor makes it -inf."""
     new, before, group, window, bound = FORMS[form]
     rng = np.random.default_rng(40 + len(form))
     batch = Batch(rng, 16, new, before, gap=2)
@@ -83,7 +84,7 @@ def test_of_a_query_before_the_window(hip_ctx, f16):
     want = run(hip_ctx, cache, batch, 2 * group, query, old, window, 0.5)
     bad = query.copy()
     for b, n in enumerate(batch.new):
-        bad[int(batch.starts[b]):int(batch.starts[b]) + n - min(n, window)] = np.nan
+        bad[int(batch.starts[b]):int(batch.starts[b]) + n - min(n, window)] = np.inf
     got = run(hip_ctx, cache, batch, 2 * group, bad, old, window, 0.5)
     np.testing.assert_array_equal(got, want)
 
@@ -99,7 +100,7 @@ def test_of_a_scale(hip_ctx, form, f16):
             last = -(-int(batch.lengths[b]) // 16) - 1
             for page in (batch.table[b, 0], batch.table[b, last]):
                 held = cache.scales["key"][page, 0]
-                for value in SPOILS:
+                for value in (np.nan, np.inf):
                     cache.scales["key"][page, 0] = value
                     got = run(hip_ctx, cache, batch, 2 * group, query, old, window, 0.0)
                     check(got, want, batch, {(b, 0)})
@@ -121,7 +122,7 @@ def test_across_groups_of_rows(hip_ctx, f16):
     old = np.zeros((3, 1, stride), np.float32)
     old[..., :400] = rng.random((3, 1, 400))
     want = run(hip_ctx, cache, batch, 64, query, old, 0, 0.8)
-    for value, b, row in ((np.nan, 0, 0), (np.nan, 0, 199), (np.nan, 2, 0)):
+    for value, b, row in ((np.nan, 0, 0), (np.inf, 0, 199), (-np.inf, 2, 0)):
         bad = query.copy()
         bad[int(batch.starts[b]) + row, 9, 3] = value
         got = run(hip_ctx, cache, batch, 64, bad, old, 0, 0.8)
