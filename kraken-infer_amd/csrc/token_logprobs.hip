@@ -343,8 +343,9 @@ __global__ __launch_bounds__(kThreads) void logprob_row_kernel(LogprobsArgs a, L
     if (!(top > -INFINITY) || logit != logit || logit == -INFINITY) {
       return -INFINITY;
     }
-    const float x = logit == top ? 0.0f : fmaf(logit, 0.5f, -0.5f * top) / t * 2.0f;
-    return x - log_sum;
+    // (Below an infinite logit -inf whatever the temperature, which may be infinite too.)
+    const float half = logit == top ? 0.0f : fmaf(logit, 0.5f, -0.5f * top);
+    return (half == -INFINITY ? half : half / t * 2.0f) - log_sum;
   };
   if (tid < 64u) {
     const uint32_t token = a.tokens != nullptr ? (uint32_t)a.tokens[row] : a.size;
