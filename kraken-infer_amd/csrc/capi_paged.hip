@@ -25,6 +25,39 @@ constexpr size_t kMaxSharedRows = size_t{1} << 20;
 
 int refuse(const char* w, const char* what) { return invalid(std::string("HIP ") + w + what); }
 
+struct Bytes {
+  const void* data;
+  size_t count;
+};
+
+bool overlap(const Bytes& a, const Bytes& b) {
+  const uintptr_t x = (uintptr_t)a.data, y = (uintptr_t)b.data;
+  return x != 0 && y != 0 && x < y + b.count && y < x + a.count;
+}
+
+// Whether an output shares bytes with an input or with another output.
+bool any_overlap(std::initializer_list<Bytes> outputs, std::initializer_list<Bytes> inputs) {
+  for (const Bytes* o = outputs.begin(); o != outputs.end(); ++o) {
+    for (const Bytes& i : inputs) {
+      if (overlap(*o, i)) {
+        return true;
+      }
+    }
+    for (const Bytes* other = outputs.begin(); other != o; ++other) {
+      if (overlap(*o, *other)) {
+        return true;
+      }
+    }
+  }
+  return false;
+}
+
+// Bytes of a cache's keys, as of its values, and of the scales of either.
+size_t code_bytes(const PagedQ8Args& c) {
+  return ((size_t)c.pages * c.kv_heads << c.page_shift) * c.head_dim;
+}
+size_t scale_bytes(const PagedQ8Args& c) { return (size_t)c.pages * c.kv_heads * sizeof(float); }
+
 // The cache's checks; `w` begins the messages.
 int cache_args(const kraken_paged_q8_cache* cache, const char* w, PagedQ8Args& c) {
   if (cache == nullptr) {
@@ -236,35 +269,22 @@ int key_weights_entry(kraken_hip_context* ctx, const kraken_buffer& query,
   a.stride = (uint32_t)std::min(stride, kInt32Max);
   a.row_stride = stride;
   KRAKEN_TRY(begin_launch(ctx));
+  // (Of a live context: one that only checks arguments may be given one address for all.)
+  const PagedQ8Args& c = a.rows.cache;
+  const PagedBatchArgs& b = a.rows.batch;
+  const size_t query_bytes = batch->tokens * heads * cache->head_dim *
+                             (f16 ? sizeof(uint16_t) : sizeof(float));
+  if (any_overlap({{weights.data, values * sizeof(float)}},
+                  {{query.data, query_bytes},
+                   {b.table, batch->sequences * batch->table_width * sizeof(int32_t)},
+                   {b.starts, (batch->sequences + 1u) * sizeof(uint32_t)},
+                   {b.lengths, batch->sequences * sizeof(uint32_t)},
+                   {c.keys, code_bytes(c)},
+                   {c.key_scales, scale_bytes(c)}})) {
+    return refuse(w, " output must not overlap an input");
+  }
   KRAKEN_TRY(ensure_workspace(ctx, key_weights_workspace_bytes(a, ctx->cu_count)));
   return finish(ctx, launch_key_weights(a, ctx->cu_count, ctx->workspace, ctx->stream), w);
-}
-
-struct Bytes {
-  const void* data;
-  size_t count;
-};
-
-bool overlap(const Bytes& a, const Bytes& b) {
-  const uintptr_t x = (uintptr_t)a.data, y = (uintptr_t)b.data;
-  return x != 0 && y != 0 && x < y + b.count && y < x + a.count;
-}
-
-// Whether an output shares bytes with an input or with another output.
-bool any_overlap(std::initializer_list<Bytes> outputs, std::initializer_list<Bytes> inputs) {
-  for (const Bytes* o = outputs.begin(); o != outputs.end(); ++o) {
-    for (const Bytes& i : inputs) {
-      if (overlap(*o, i)) {
-        return true;
-      }
-    }
-    for (const Bytes* other = outputs.begin(); other != o; ++other) {
-      if (overlap(*o, *other)) {
-        return true;
-      }
-    }
-  }
-  return false;
 }
 
 }  // namespace
