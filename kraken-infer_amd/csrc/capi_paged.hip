@@ -594,7 +594,11 @@ KRAKEN_API int kraken_hip_gather_kv_pages_q8(
                      {kept.data, places * sizeof(int32_t)},
                      {kept_lengths.data, sequences * sizeof(uint32_t)},
                      {page_table.data, sources * sizeof(int32_t)},
-                     {target_table.data, targets * sizeof(int32_t)}})) {
+                     {target_table.data, targets * sizeof(int32_t)},
+                     {a.cache.keys, code_bytes(a.cache)},
+                     {a.cache.values, code_bytes(a.cache)},
+                     {a.cache.key_scales, scale_bytes(a.cache)},
+                     {a.cache.value_scales, scale_bytes(a.cache)}})) {
       return refuse(w, " weights output must not overlap an input");
     }
   }

@@ -73,3 +73,41 @@ def test_key_weights(hip_ctx, f16):
     w = w.view(np.float32).reshape(SEQUENCES, KV, STRIDE)
     # Zero keys weigh alike: two query heads' one from each row.
     np.testing.assert_allclose(w.sum(-1), [[2.0] * KV, [4.0] * KV], rtol=1e-5)
+
+
+def test_gathered_weights(hip_ctx):
+    torch = pytest.importorskip("torch")
+    keep, width = 20, 2
+    arena = Arena(torch, {**POOL, "table": 4 * SEQUENCES * WIDTH, "kept": 4 * SEQUENCES * KV * keep,
+                          "counts": 4 * SEQUENCES, "target": 4 * SEQUENCES * width,
+                          "weights": 4 * SEQUENCES * KV * STRIDE,
+                          "moved": 4 * SEQUENCES * KV * STRIDE})
+    arena.fill("table", np.array([0, 1, 2, 0, 1, 3], np.int32))
+    arena.fill("target", np.arange(4, 8, dtype=np.int32))
+    arena.fill("counts", np.array([keep, 3], np.uint32))
+    arena.fill("kept", np.tile(2 * np.arange(keep, dtype=np.int32), (SEQUENCES, KV, 1)))
+    weights = np.arange(SEQUENCES * KV * STRIDE, dtype=np.float32).reshape(SEQUENCES, KV, STRIDE)
+    arena.fill("weights", weights)
+
+    def status(at=None):
+        v = arena.view
+        return hip_ctx.status("gather_kv_pages_q8", arena.cache(), v("table"), WIDTH, v("kept"),
+                              v("counts"), keep, SEQUENCES, v("target"), width, v("weights"), STRIDE,
+                              v("moved", at))
+
+    before = arena.memory.clone()
+    size = arena.sizes["moved"]
+    for other in (*POOL, "table", "kept", "counts", "target", "weights"):
+        first, end = arena.at[other], arena.at[other] + arena.sizes[other]
+        for at in (first, end - 4, first - size + 4):
+            assert status(at) == kh.INVALID_ARGUMENT, (other, at - first)
+            assert "must not overlap" in kh.last_error()
+    torch.cuda.synchronize()
+    assert torch.equal(arena.memory, before)
+    for at in (arena.at["key_scales"] - size, arena.at["values"] + arena.sizes["values"], None):
+        assert status(at) == kh.OK, kh.last_error()
+    got = arena.memory[arena.at["moved"] - arena.memory.data_ptr():][:size].cpu().numpy()
+    got = got.view(np.float32).reshape(weights.shape)
+    np.testing.assert_array_equal(got[0, :, :keep], weights[0, :, :2 * keep:2])
+    np.testing.assert_array_equal(got[1, :, :3], weights[1, :, :6:2])
+    assert (got[0, :, keep:] == 0).all() and (got[1, :, 3:] == 0).all()
