@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
 // wait for each other; keys that have the digits before are few.
 template <uint32_t kThreads, uint32_t kCopies>
 struct SelectScratch {
-  uint32_t bins[kCopies + 2u][kBins];
+  uint32_t bins[(kCopies + 2u) * kBins];
   uint32_t waves[kThreads / 64u];
   uint32_t digit, above;
 };
@@ -69,7 +69,7 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
   const uint32_t times = (count + kThreads - 1u) / kThreads;  // of a wave
   const uint32_t begin = wave * times * 64u + lane;
   for (uint32_t i = tid; i < (kCopies + 2u) * kBins; i += kThreads) {
-    s.bins[0][i] = 0;
+    s.bins[i] = 0;
   }
   uint32_t held[kInRegisters ? kHeld : 1];
   if constexpr (kInRegisters) {
@@ -152,9 +152,9 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
     want -= s.above;
   };
   using One = std::integral_constant<uint32_t, 1>;
-  settle(std::integral_constant<uint32_t, kCopies>{}, s.bins[0], 21u, kBins - 1u);
-  settle(One{}, s.bins[kCopies], 10u, kBins - 1u);
-  settle(One{}, s.bins[kCopies + 1u], 0u, 1023u);
+  settle(std::integral_constant<uint32_t, kCopies>{}, s.bins, 21u, kBins - 1u);
+  settle(One{}, s.bins + kCopies * kBins, 10u, kBins - 1u);
+  settle(One{}, s.bins + (kCopies + 1u) * kBins, 0u, 1023u);
   // How many larger and equal ones each wave has, then their places.
   uint32_t larger = 0, equal = 0;
   each([&](uint32_t key, uint32_t j) {
