@@ -398,9 +398,23 @@ struct SharedPlan {
 // MB (4 sequences of 4 rows, 8192 tokens of 1 KiB: 21.4 us and 21.6; 32768: 42.6 and 26.8), with
 // it about 100 MB (64 sequences, 2048 tokens: 48.8 and 45.6, 512 tokens 21 and 41; 8 of 32
 // rows, 2048 tokens: 29 and 48, 8192: 73 and 58).
+//
+// Not where the sequences' rows fill tiles of their own, at the mean: nothing is then read
+// again that counts, and rows pass through memory once more for the join.  Plain and shared,
+// f32, eight heads of 256 on two KV heads: 64 sequences of 10 tokens behind 8192 261 us and 155,
+// of 32 (128 rows) behind 4096 160 and 221; 8 of 512 behind 16384 1052 and 1163; a chunk of 512
+// beside 63 single tokens (36 rows at the mean) behind 16384 328 and 212, of 2048 (132) behind
+// 8192 433 and 459, of 512 beside 15 (132) behind 8192 144 and 131.  Sixteen heads of 128 on
+// eight: 16 sequences of 128 tokens behind 4096 165 and 232, 24 of 20 (40 rows) behind 8192 214
+// and 119; 32 chunks of 64 beside as many single tokens (65) behind 8192 359 and 385.
 bool worth_sharing(const PagedAttentionArgs& a, const SharedPrefixArgs& p) {
   const uint64_t group = a.heads / a.cache.kv_heads;
   const uint64_t own = a.batch.max_query * group, all = std::max(own, p.max_rows * group);
+  const uint64_t rows =
+    std::min((uint64_t)a.batch.tokens, (uint64_t)a.batch.sequences * a.batch.max_query) * group;
+  if (rows >= (uint64_t)kTileRows * a.batch.sequences) {
+    return false;
+  }
   const uint64_t blocks = own <= kDecodeBlock || own > kDecodeRows ? 1u : 2u;
   const double again = (double)(a.batch.sequences - p.groups) *
                        (double)std::min(p.max_prefix, a.batch.max_keys) *
