@@ -196,7 +196,8 @@ __device__ __forceinline__ void select_between(const float* weights, uint32_t co
 // One workgroup a sequence and KV head; kAny: with more keys than it can hold, too.  Not
 // bytes but the three counts, their barriers and the last pass over the keys are what it spends
 // its time on: 512 keys of one pair take 8.7 us, 4096 10.1, 32768 20.3, 131072 93; 64 sequences
-// of 32768, two heads each, 20.5.
+// of 32768, two heads each, 20.5.  (120 and 132 scalars are spilled, into lanes of vector
+// registers.)
 template <uint32_t kThreads, uint32_t kCopies, bool kAny>
 __global__ __launch_bounds__(kThreads) void select_keys_kernel(SelectKeysArgs a) {
   __shared__ SelectScratch<kThreads, kCopies> s;
@@ -263,9 +264,9 @@ __device__ __forceinline__ int code_at(uint32_t word, uint32_t byte) {
 // bytes each, of which it takes one.  The sources are the wave's, so that places, bytes and
 // ratios are scalars.
 //
-// 4096 of 32768 positions for 16 sequences of two heads of 256, one kept in eight: 62 us.  The
-// keys are 34 MB to read and 34 to write, and 29 us by themselves; of the values 176 MB are
-// read, the runs of eight that hold any, and 34 written.  Each load waits for the one that
+// 4096 positions of each of 16 sequences of 8192 to 32768, two heads of 256: 62 us.  The keys
+// are 34 MB to read and 34 to write, and 29 us by themselves; of the values 130 MB are read,
+// the runs of eight that hold any, and 34 written.  Each load waits for the one that
 // tells its place, four deep, and then for all of a page.  Asking for the rows before the
 // page's scale is known took 67 us (its registers cost a wave in four), workgroups of 128 or
 // 512 threads and stores or loads past the caches between 60 and 75.

@@ -11,8 +11,8 @@
 // 2^(score - log2 of the row's sum) over the rows of each key.
 //
 // 64 sequences of up to 32768 keys, one token of four query heads for each of two KV heads of
-// 256: 135 us for 537 MB of keys, 34 of weights and 34 of scores there and back, of which the
-// second launch takes 15.  One sequence of 4096: 11.5, two launches of some 7 and 4 us.
+// 256: 135 us for 537 MB of keys, 17 of weights read and written and 34 of scores each way, of
+// which the second launch takes 15.  One sequence of 4096: 11.5, two launches of some 7 and 4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

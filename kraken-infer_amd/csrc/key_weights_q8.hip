@@ -15,11 +15,12 @@
 // Launches: rows, first pass (maxima and sums by 256 keys), L of each row, second pass,
 // and where it splits the rows over workgroups their sums' sum.
 //
-// 1024 f32 rows of a sequence of 8192 (two KV heads of 256, groups of four): 139 us, traced
-// 65 for each pass, 19 the others.  A pass's products are 64 GFLOP in f16, 49 us at a large
-// product's rate, and their time hides the exponentials and sums (two waves a SIMD; without
-// those the pass takes as long).  With f16 queries 92.  32 rows at the end of the same
-// sequence: 26.5, five launches.
+// 1024 f32 rows of a sequence of 8192 (two KV heads of 256, groups of four): 140 us (150 on a
+// card of lower clocks), traced 65 for each pass (68 to 71), 19 the others.  A pass's products
+// are 64 GFLOP in f16, 49 us at a large product's rate, and their time hides the exponentials
+// and sums (two waves a SIMD; without those the pass takes as long).  With f16 queries 90 (94).
+// 32 rows at the end of the same sequence: 27, five launches.  No vector register is spilled;
+// 58 to 87 scalars of a pass are, into lanes of one (256 registers in all for f32 rows of 256).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
